@@ -14,3 +14,5 @@ from .tensor import (  # noqa: F401
     rand_tensor_uniform, rand_tensor_normal, runif, rnorm, any, all, diff, range_, is_finite, create_ones_like, all_equal,
     tensor_pow, permute, size, dim, as_vector, as_numeric, to_numeric, tensor_to_scalar, shares_memory, tensor_info,
     set_random_seed, gpu_available, gpu_info, gpu_memory_available, gpu_status, gpu_add, gpu_multiply, gpu_scale, gpu_dot)
+from .lm import (  # noqa: F401
+    quant4_encode, quant4_matvec, residual_norm, residual_norm_grad, token_logprob, token_logprob_grad)

@@ -51,16 +51,11 @@ class Desc(ctypes.Structure):
     ]
 
 
+_Dims = ctypes.c_int64 * MAX_DIMS
+
+
 def make_desc(ptr, dtype_code, shape, strides, offset=0):
-    d = Desc()
-    d.data = ptr
-    d.offset = offset
-    d.ndim = len(shape)
-    d.dtype = dtype_code
-    for i, (s, st) in enumerate(zip(shape, strides)):
-        d.shape[i] = s
-        d.stride[i] = st
-    return d
+    return Desc(ptr, offset, _Dims(*shape), _Dims(*strides), len(shape), dtype_code)
 
 
 _lib = None
@@ -112,6 +107,12 @@ def _bind(lib):
         "acd_fused_stats_keys": ([vp, dp, dp, f64, vp, vp, i64, vp], i32),
         "acd_permute_fused_stats_keys": ([vp, dp, dp, dp, f64, vp, vp, i64, vp], i32),
         "acd_copy_fanout": ([vp, vp, vp, vp, i64, vp], i32),
+        "acd_token_logprob": ([vp, dp, dp, dp, dp, dp, dp, dp, i32, f64, i32, vp], i32),
+        "acd_token_logprob_grad": ([vp, dp, dp, dp, i32, f64, dp, dp, dp, dp, dp, i32, vp], i32),
+        "acd_residual_norm": ([vp, dp, dp, dp, dp, dp, dp, dp, dp, dp, i32, f64, f64, vp], i32),
+        "acd_residual_norm_grad": ([vp] + [dp] * 14 + [i32, f64, vp], i32),
+        "acd_quant4_matvec": ([vp, dp, dp, dp, dp, dp, i32, vp], i32),
+        "acd_quant4_encode": ([vp, dp, dp, dp, dp, i32, vp], i32),
         "acd_selftest_fastdiv": ([u32, u32, P(u32)], i32),
         "acd_selftest_collapse": ([dp, dp, P(i64), P(i64), P(i64)], i32),
     }

@@ -1,0 +1,115 @@
+// Shared by the language-model row operators (logprob.cu, norm.cu): the view
+// of a tensor as rows along one axis, the accumulator type of an element type
+// and the checks of their small tensors.
+#pragma once
+
+#include <cfloat>
+#include <climits>
+
+#include "common.cuh"
+
+namespace acd {
+
+// Element type -> the type its sums and statistics are held in.
+template <typename T>
+struct AccOf { using type = float; };
+template <>
+struct AccOf<double> { using type = double; };
+
+__device__ __forceinline__ float to_acc(float x) { return x; }
+__device__ __forceinline__ float to_acc(__half x) { return __half2float(x); }
+__device__ __forceinline__ double to_acc(double x) { return x; }
+// One rounding to the storage type.
+template <typename T, typename A>
+__device__ __forceinline__ T from_acc(A x) { return (T)x; }
+template <>
+__device__ __forceinline__ __half from_acc<__half, float>(float x) { return __float2half_rn(x); }
+
+// Fused multiply-add and exponentials of the accumulator type.  (The library
+// is compiled without contraction, so a fused product is asked for by name.)
+__device__ __forceinline__ float fma_a(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double fma_a(double a, double b, double c) { return fma(a, b, c); }
+
+// A tensor as rows: element d of row r = l + L*o lies at p + l*sl + d*sd + o*so.
+struct Rows {
+  void *p = nullptr;
+  int64_t sl = 0, sd = 0, so = 0;
+};
+
+// Geometry shared by the tensors of one call.
+struct RowShape {
+  int64_t L = 1, D = 1, O = 1;
+  __host__ __device__ int64_t rows() const { return L * O; }
+};
+
+template <typename T>
+__device__ __forceinline__ T *row_ptr(const Rows &v, int64_t r, int64_t L) {
+  const int64_t o = L == 1 ? r : r / L, l = L == 1 ? 0 : r - o * L;
+  return static_cast<T *>(v.p) + l * v.sl + o * v.so;
+}
+
+// Views `d` around `axis`; the axes before it, and those after it, must each
+// merge into one (extents of 1 aside).  False when they do not.
+inline bool split_rows(const acd_desc *d, int axis, RowShape &s, Rows &v) {
+  auto merge = [&](int d0, int d1, int64_t &n, int64_t &st) {
+    n = 1;
+    st = 0;
+    int64_t next = 0;
+    bool first = true;
+    for (int k = d0; k < d1; ++k) {
+      if (d->shape[k] == 1) continue;
+      if (first) st = d->stride[k];
+      if (!first && d->stride[k] != next) return false;
+      next = d->stride[k] * d->shape[k];
+      n *= d->shape[k];
+      first = false;
+    }
+    return true;
+  };
+  if (!merge(0, axis, s.L, v.sl) || !merge(axis + 1, d->ndim, s.O, v.so)) return false;
+  s.D = d->shape[axis];
+  v.sd = d->stride[axis];
+  v.p = desc_ptr(d);
+  return true;
+}
+
+// A row tensor of `like` along `axis`: extents of `like` without the axis, or
+// with `k` on it; contiguous.
+inline acd_status check_row_tensor(const char *op, const char *name, const acd_desc *d, const acd_desc *like, int axis,
+                                   int64_t k = 1) {
+  ACD_TRY(check_desc(d, name));
+  bool ok = false;
+  if (d->ndim == like->ndim) {
+    ok = true;
+    for (int i = 0; i < like->ndim; ++i) ok = ok && d->shape[i] == (i == axis ? k : like->shape[i]);
+  }
+  if (!ok && k == 1 && d->ndim == like->ndim - 1) {
+    ok = true;
+    for (int i = 0; i < d->ndim; ++i) ok = ok && d->shape[i] == like->shape[i < axis ? i : i + 1];
+  }
+  // one row: a one-element tensor of any rank, as the reductions return it
+  if (!ok && k == 1 && like->ndim == 1) ok = desc_numel(d) == 1;
+  if (!ok) return fail(ACD_ERR_SHAPE, "%s: %s does not have one entry a row", op, name);
+  if (!desc_is_contiguous(d)) return fail(ACD_ERR_UNSUPPORTED, "%s: %s must be contiguous", op, name);
+  return ACD_OK;
+}
+
+inline bool same_shape(const acd_desc *a, const acd_desc *b) {
+  if (a->ndim != b->ndim) return false;
+  for (int k = 0; k < a->ndim; ++k)
+    if (a->shape[k] != b->shape[k]) return false;
+  return true;
+}
+
+// INT32 or INT64 values read and written as int64.
+__device__ __forceinline__ int64_t load_index(const void *p, bool wide, int64_t i) {
+  return wide ? static_cast<const int64_t *>(p)[i] : (int64_t) static_cast<const int32_t *>(p)[i];
+}
+__device__ __forceinline__ void store_index(void *p, bool wide, int64_t i, int64_t v) {
+  if (wide)
+    static_cast<int64_t *>(p)[i] = v;
+  else
+    static_cast<int32_t *>(p)[i] = (int32_t)v;
+}
+
+}  // namespace acd

@@ -380,6 +380,110 @@ acd_status acd_shard_finish(acd_ctx *ctx, int64_t *buf, int64_t nkeys, int32_t w
 acd_status acd_argmax_keys_decode(acd_ctx *ctx, const acd_desc *out_index, const int64_t *keys,
                                   int32_t one_based, acd_stream stream);
 
+/* ---- language-model rows ------------------------------------------------ */
+/* These operators work on rows: a row is all elements of a view along `axis`
+ * (0-based), rows are counted in column-major order of the other axes.  Every
+ * view must collapse to (lanes before the axis, axis, lanes after it), as for
+ * acd_softmax.  "Row tensors" hold one value a row: shape of the view without
+ * the axis, or with extent 1 there, contiguous.  Statistics are FLOAT32 for
+ * FLOAT16/FLOAT32 rows and FLOAT64 for FLOAT64 rows; sums are held in that
+ * type too.  The reference has none of these operators. */
+
+/* Log probability of one given token a row under softmax(scale * logits),
+ * with the entropy of that distribution, its log-sum-exp and its k most
+ * likely tokens; one pass over the logits (FLOAT32, FLOAT64 or FLOAT16):
+ *   lse     = log sum_v exp(scale * x_v)
+ *   logprob = scale * x_token - lse
+ *   entropy = -sum_v p_v log p_v,  p_v = exp(scale * x_v - lse)
+ * tokens: INT32 or INT64 row tensor, counted from 1 when one_based != 0.  A
+ * token one below the first (0, or -1) asks for nothing: logprob 0.  NA
+ * (INT32_MIN, INT64_MIN) and any other token outside the vocabulary: NaN.
+ * top_index (INT32 or INT64) and top_logprob have the logits' shape with
+ * extent k <= 32 on the axis, contiguous: the k largest logits in falling
+ * order, equal ones by rising index.  NaN is never among them; a place for
+ * which no token is left holds NA and NaN.
+ * A logit of -Inf is a token of probability 0.  A row without mass (every
+ * logit -Inf) has lse = logprob = -Inf and entropy 0.  A NaN or +Inf logit
+ * makes the row's lse, logprob and entropy NaN.
+ * Any output may be NULL; tokens and logprob go together, top_index and
+ * top_logprob too.  scale is positive and finite. */
+acd_status acd_token_logprob(acd_ctx *ctx, const acd_desc *logprob, const acd_desc *entropy, const acd_desc *lse,
+                             const acd_desc *top_index, const acd_desc *top_logprob, const acd_desc *logits,
+                             const acd_desc *tokens, int32_t axis, double scale, int32_t one_based,
+                             acd_stream stream);
+/* The gradient of acd_token_logprob's outputs with respect to the logits, from
+ * the lse and entropy it returned and the loss's gradients d_logprob,
+ * d_entropy, d_lse (row tensors; NULL: none, at least one is given):
+ *   grad_v = scale * ([v = token] d_logprob
+ *            + p_v (d_lse - d_logprob - d_entropy (log p_v + entropy)))
+ * grad has the logits' shape and dtype and may be the logits' own view
+ * (otherwise the two must not overlap).  A token that asks for nothing, and
+ * one outside the vocabulary, takes d_logprob as 0.  A row without mass has
+ * gradient 0, and so has one whose lse is below a quarter of the statistics
+ * type's lowest value (every logit masked by that value).  tokens goes with
+ * d_logprob, entropy with d_entropy. */
+acd_status acd_token_logprob_grad(acd_ctx *ctx, const acd_desc *grad, const acd_desc *logits, const acd_desc *tokens,
+                                  int32_t axis, double scale, const acd_desc *lse, const acd_desc *entropy,
+                                  const acd_desc *d_logprob, const acd_desc *d_entropy, const acd_desc *d_lse,
+                                  int32_t one_based, acd_stream stream);
+
+/* A residual update with the norms around it, rows of D elements along `axis`:
+ *   b' = block * rstd_block * w_post,  rstd_block = 1 / sqrt(mean(block^2) + eps)
+ *        (w_post NULL: b' = block)
+ *   h  = alpha * residual + gate * b'  (gate NULL: 1)
+ *   y  = h * rstd_h * w_pre,           rstd_h = 1 / sqrt(mean(h^2) + eps)
+ * h is the updated residual stream, y the normalised input of the next block;
+ * both are rounded once, y from the h before its rounding.  w_pre, w_post: D
+ * elements of the rows' dtype (FLOAT32, FLOAT64, FLOAT16), contiguous.  gate:
+ * D elements, or the residual's shape with extent 1 on any number of leading
+ * axes other than `axis`, so that each of its G rows of D elements holds for
+ * rows/G consecutive rows.  rstd_h and rstd_block are row tensors (either may
+ * be NULL) that the gradient takes.  h may be the residual's own view and y
+ * the block's; otherwise outputs must not overlap inputs. */
+acd_status acd_residual_norm(acd_ctx *ctx, const acd_desc *h, const acd_desc *y, const acd_desc *rstd_h,
+                             const acd_desc *rstd_block, const acd_desc *residual, const acd_desc *block,
+                             const acd_desc *w_pre, const acd_desc *w_post, const acd_desc *gate, int32_t axis,
+                             double alpha, double eps, acd_stream stream);
+/* Its gradients, with hn = h * rstd_h and bn = block * rstd_block:
+ *   t          = d_h + rstd_h (d_y w_pre - hn mean(d_y w_pre hn))
+ *   d_residual = alpha * t
+ *   u          = t * gate
+ *   d_block    = rstd_block (u w_post - bn mean(u w_post bn))   (w_post NULL: u)
+ *   d_w_pre = sum d_y hn,  d_w_post = sum u bn    over all rows
+ *   d_gate  = sum t b'                            over each gate row's rows
+ * d_h NULL: the loss sees h through y only.  d_w_pre, d_w_post, d_gate have
+ * their operand's shape, in the statistics' dtype, contiguous; each may be
+ * NULL.  Their sums run in an order set by the shapes alone: the same inputs
+ * give the same bits.  d_residual may be d_h's own view and d_block d_y's. */
+acd_status acd_residual_norm_grad(acd_ctx *ctx, const acd_desc *d_residual, const acd_desc *d_block,
+                                  const acd_desc *d_w_pre, const acd_desc *d_w_post, const acd_desc *d_gate,
+                                  const acd_desc *d_h, const acd_desc *d_y, const acd_desc *h, const acd_desc *block,
+                                  const acd_desc *rstd_h, const acd_desc *rstd_block, const acd_desc *w_pre,
+                                  const acd_desc *w_post, const acd_desc *gate, int32_t axis, double alpha,
+                                  acd_stream stream);
+
+/* ---- 4-bit weights ------------------------------------------------------- */
+/* out = W x for a matrix W of `out` rows and `in` columns held in 4 bits:
+ *   W[o, k] = scales[k / group, o] * (q[o, k] - z),  z = zeros[k / group, o], or 8
+ * weights: INT8 of shape [16 * ceil(in / 32), out], contiguous, 16-byte aligned:
+ * byte k/2 of column o holds q[o, k] in its low half for even k and in its
+ * high half for odd k; what lies beyond `in` is not used.  scales and zeros:
+ * FLOAT16 or FLOAT32 of shape [ceil(in / group), out], contiguous; zeros may
+ * be NULL.  group is a positive multiple of 32.  x: [in] or [in, n], out:
+ * [out] or [out, n], FLOAT16 or FLOAT32 each, any strides, not overlapping.
+ * Products are summed in float32 in an order set by the shapes alone. */
+acd_status acd_quant4_matvec(acd_ctx *ctx, const acd_desc *out, const acd_desc *weights, const acd_desc *scales,
+                             const acd_desc *zeros, const acd_desc *x, int32_t group, acd_stream stream);
+/* Makes weights, scales (and zeros) from w, an [out, in] view of FLOAT16,
+ * FLOAT32 or FLOAT64.  zeros NULL: scale = max|w| / 7 and q = round(w / scale)
+ * + 8.  Otherwise scale = (max(w, 0) - min(w, 0)) / 15, zero = round(-min(w, 0)
+ * / scale) and q = round(w / scale) + zero, both limited to 0..15.  Rounding
+ * is to nearest, ties to even, with the scale as it is stored; a group whose
+ * scale is 0 holds q = zero.  A group with a NaN or infinite weight gets a
+ * scale of NaN. */
+acd_status acd_quant4_encode(acd_ctx *ctx, const acd_desc *weights, const acd_desc *scales, const acd_desc *zeros,
+                             const acd_desc *w, int32_t group, acd_stream stream);
+
 #ifdef __cplusplus
 }
 #endif
