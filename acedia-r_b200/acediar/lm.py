@@ -6,8 +6,6 @@ computation is a call into libacediar_b200.so on the current torch stream.  The
 formulas and every rule on masked, missing and empty values stand beside the C
 functions in include/acd.h.  The reference has none of these operators.
 """
-import ctypes
-import math
 import numbers
 from collections import namedtuple
 
@@ -25,7 +23,16 @@ _UNSUPPORTED = 8
 
 
 def _new(shape, dtype, device):
-    return gpuTensor(torch.empty(max(math.prod(shape), 1), dtype=_TORCH[dtype], device=device), shape, dtype)
+    """An uninitialised tensor; shape is a tuple of ints.  (A small call's time is
+    its host time: the attributes are set without the constructor's checks.)"""
+    t = gpuTensor.__new__(gpuTensor)
+    n, strides = 1, []
+    for s in shape:
+        strides.append(n)
+        n *= s
+    t.storage = torch.empty(n or 1, dtype=_TORCH[dtype], device=device)
+    t.shape, t.dtype, t.strides, t.offset = shape, dtype, tuple(strides), 0
+    return t
 
 
 def _desc(t):
