@@ -112,4 +112,48 @@ __device__ __forceinline__ void store_index(void *p, bool wide, int64_t i, int64
     static_cast<int32_t *>(p)[i] = (int32_t)v;
 }
 
+// A row is read in pieces of V elements that start on 16-byte boundaries; it may
+// itself start (by `row_shift` elements) and end inside a piece.
+template <typename T, int V>
+__device__ __forceinline__ int row_shift(const T *x) {
+  return V == 1 ? 0 : (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % V);
+}
+
+// Elements first .. first + V - 1 of a row of D, `fill` beyond its ends.  V = 1:
+// any stride.
+template <typename T, typename A, int V>
+__device__ __forceinline__ void load_piece(const T *x, int64_t sd, int first, int D, A fill, A *out) {
+  if (V == 1) {
+    out[0] = first < D ? to_acc(x[first * sd]) : fill;
+  } else if (first >= 0 && first + V <= D) {
+    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(x + first);
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = to_acc(v.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = first + j >= 0 && first + j < D ? to_acc(x[first + j]) : fill;
+  }
+}
+
+template <typename T, typename A, int V>
+__device__ __forceinline__ void store_piece(T *x, int64_t sd, int first, int D, const A *v) {
+  if (V > 1 && first >= 0 && first + V <= D) {
+    Vec<T, V> w;
+#pragma unroll
+    for (int j = 0; j < V; ++j) w.v[j] = from_acc<T, A>(v[j]);
+    *reinterpret_cast<Vec<T, V> *>(x + first) = w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (first + j >= 0 && first + j < D) x[(first + j) * sd] = from_acc<T, A>(v[j]);
+  }
+}
+
+// Whether the pieces of V elements of `size` bytes of x and g coincide in every
+// row: same offset in 16 bytes, strides sx, sg that differ by whole pieces.
+inline bool pieces_match(const Rows &x, const Rows &g, int64_t sx, int64_t sg, int V, int size) {
+  const uintptr_t px = reinterpret_cast<uintptr_t>(x.p), pg = reinterpret_cast<uintptr_t>(g.p);
+  return (px - pg) % (uintptr_t)(V * size) == 0 && (sx - sg) % V == 0 && (x.so - g.so) % V == 0;
+}
+
 }  // namespace acd

@@ -14,8 +14,6 @@ namespace cg = cooperative_groups;
 
 namespace acd {
 
-__device__ __forceinline__ float lp_exp(float x) { return expf(x); }
-__device__ __forceinline__ double lp_exp(double x) { return exp(x); }
 __device__ __forceinline__ float lp_log(float x) { return logf(x); }
 __device__ __forceinline__ double lp_log(double x) { return log(x); }
 
@@ -289,23 +287,6 @@ __device__ __forceinline__ void asked_token(const LogprobArgs &a, int64_t r, con
 // ---------------------------------------------------------------------------
 // rows along the axis
 // ---------------------------------------------------------------------------
-// V consecutive logits of a row, 16 bytes wide where they lie in the row (the
-// row may start and end inside a 16-byte piece), -Inf beyond its ends.  V = 1:
-// any stride.
-template <typename T, typename A, int V>
-__device__ __forceinline__ void load_piece(const T *x, int64_t sd, int first, int D, A *out) {
-  if (V == 1) {
-    out[0] = first < D ? to_acc(x[first * sd]) : A(-INFINITY);
-  } else if (first >= 0 && first + V <= D) {
-    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(x + first);
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = to_acc(v.v[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = first + j >= 0 && first + j < D ? to_acc(x[first + j]) : A(-INFINITY);
-  }
-}
-
 // How many pieces of V logits a lane holds at once.
 template <typename T, int V>
 struct BatchU { static constexpr int value = V == 1 ? 8 : 4; };
@@ -322,17 +303,12 @@ __device__ __forceinline__ void read_batches(const T *x, int64_t sd, int D, int 
     const int base = b * (U * V * 32) - shift;
     A xs[U * V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_piece<T, A, V>(x, sd, base + (u * 32 + lane) * V, D, xs + u * V);
+    for (int u = 0; u < U; ++u) load_piece<T, A, V>(x, sd, base + (u * 32 + lane) * V, D, A(-INFINITY), xs + u * V);
     st.batch(xs, base, D, c, k, TOP && floor ? *floor : A(-INFINITY));
     // any warp's entry k - 1 will do as floor: the value decides how much is
     // looked at, never the result
     if (TOP && floor && lane == 0 && st.top.ki != kNone && st.top.kv > *floor) *floor = st.top.kv;
   }
-}
-
-template <typename T, int V>
-__device__ __forceinline__ int row_shift(const T *x) {
-  return V == 1 ? 0 : (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % V);
 }
 
 // One warp a row.
@@ -603,11 +579,14 @@ struct LogprobGradArgs {
   bool wide_token, one_based;
 };
 
-// Coefficients of a row: grad_v = p_v (a0 - a1 (lp_v + H)) + [v = token] gt.
+// A row's coefficients, scale included.  With d = c x_v - lse = log p_v:
+//   grad_v = p_v (a0 - a1 d) + [v = t] gt,  a0 = c (g_lse - g - g_H H), a1 = c g_H.
+// d is rounded once (fma) before the exponential, so its error is that of its
+// own size and not of the logit's.
 template <typename A>
 struct GradRow {
-  A lse, H, a0, a1, gt;
-  int64_t t;
+  A lse, a0, a1, gt;
+  int t;
 };
 
 template <typename A>
@@ -620,41 +599,111 @@ __device__ __forceinline__ GradRow<A> grad_row(const LogprobGradArgs &a, int64_t
   if (a.d_logprob) {
     const int64_t t = load_index(a.tokens, a.wide_token, r) - (a.one_based ? 1 : 0);
     if (t >= 0 && t < a.s.D) {
-      g.t = t;
+      g.t = (int)t;
       g.gt = c * static_cast<const A *>(a.d_logprob)[r];
     }
   }
-  g.a1 = a.d_entropy ? c * static_cast<const A *>(a.d_entropy)[r] : A(0);
-  g.H = a.d_entropy ? static_cast<const A *>(a.entropy)[r] : A(0);
   g.a0 = (a.d_lse ? c * static_cast<const A *>(a.d_lse)[r] : A(0)) - g.gt;
+  g.a1 = A(0);
+  if (a.d_entropy) {
+    g.a1 = c * static_cast<const A *>(a.d_entropy)[r];
+    g.a0 = fma_a(-g.a1, static_cast<const A *>(a.entropy)[r], g.a0);
+  }
   // a row without mass: p = 0 everywhere and no token term.  So is one masked
   // throughout by the type's lowest value: its lse has no digits left for ln S.
   if (g.lse <= (std::is_same<A, double>::value ? (A)(-DBL_MAX / 4) : (A)(-FLT_MAX / 4))) {
     g.lse = A(INFINITY);
-    g.t = -1;
+    g.a0 = g.a1 = g.gt = A(0);
   }
   return g;
 }
 
 template <typename A>
-__device__ __forceinline__ A grad_value(const GradRow<A> &g, A x, A c, bool is_token) {
-  const A lp = fma_a(c, x, -g.lse);
-  const A p = lp_exp(lp);
-  // p = 0 (a logit of -Inf, or far below the maximum): 0 log 0 = 0
-  A v = p == A(0) ? A(0) : p * fma_a(-g.a1, lp + g.H, g.a0);
-  return is_token ? v + g.gt : v;
+__device__ __forceinline__ A grad_value(const GradRow<A> &g, A x, A c);
+template <>
+__device__ __forceinline__ float grad_value<float>(const GradRow<float> &g, float x, float c) {
+  using M = LpMath<float>;
+  const float d = M::floor_z(fmaf(c, x, -g.lse));  // p = 0 where d is below the floor: 0 log 0 = 0
+  return M::ex(d * 1.44269504088896341f) * fmaf(-g.a1, d, g.a0);
+}
+template <>
+__device__ __forceinline__ double grad_value<double>(const GradRow<double> &g, double x, double c) {
+  const double d = LpMath<double>::floor_z(fma(c, x, -g.lse));
+  return exp(d) * fma(-g.a1, d, g.a0);
 }
 
-// One element a thread, along the lanes first: any strides.
-template <typename T>
-__global__ void __launch_bounds__(256) k_logprob_grad(LogprobGradArgs a) {
+// Rows along the axis: a warp takes U pieces a lane of one row, 16 bytes each
+// (V logits; the row may start and end inside a piece), reads them all and
+// then writes.  V = 1: any strides.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) k_logprob_grad_rows(LogprobGradArgs a, uint32_t segs, uint32_t tasks) {
   using A = typename AccOf<T>::type;
-  for (int64_t r = blockIdx.x; r < a.s.rows(); r += gridDim.x) {
-    const GradRow<A> g = grad_row<A>(a, r);
+  constexpr int U = BatchU<T, V>::value;
+  const int lane = threadIdx.x & 31;
+  const A c = (A)a.scale;
+  const int D = (int)a.s.D;
+  for (uint32_t task = blockIdx.x * 8 + (threadIdx.x >> 5); task < tasks; task += gridDim.x * 8) {
+    const uint32_t r = task / segs, seg = task - r * segs;
     const T *x = row_ptr<T>(a.x, r, a.s.L);
     T *out = row_ptr<T>(a.g, r, a.s.L);
-    for (int64_t d = threadIdx.x; d < a.s.D; d += 256)
-      out[d * a.g.sd] = from_acc<T, A>(grad_value<A>(g, to_acc(x[d * a.x.sd]), (A)a.scale, d == g.t));
+    const int base = (int)seg * (U * V * 32) - row_shift<T, V>(x);
+    A xs[U * V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_piece<T, A, V>(x, a.x.sd, base + (u * 32 + lane) * V, D, A(-INFINITY), xs + u * V);
+    const GradRow<A> g = grad_row<A>(a, r);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int first = base + (u * 32 + lane) * V;
+      A v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = grad_value<A>(g, xs[u * V + j], c);
+      if (g.t >= first && g.t < first + V) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (first + j == g.t) v[j] += g.gt;
+      }
+      store_piece<T, A, V>(out, a.g.sd, first, D, v);
+    }
+  }
+}
+
+// Rows across the lanes: a thread keeps the coefficients of V neighbouring
+// rows and walks along the steps, so that a warp reads and writes 32 * V
+// neighbouring logits at a time.  A block is bx threads along the lanes by
+// 256 / bx along the steps, and takes `chunk` steps.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) k_logprob_grad_lanes(LogprobGradArgs a, int bx_log2, int64_t lblocks,
+                                                            int64_t chunk) {
+  using A = typename AccOf<T>::type;
+  constexpr int UN = 4;
+  const int bx = 1 << bx_log2, by = 256 >> bx_log2;
+  const int64_t lb = blockIdx.x % lblocks, o = blockIdx.x / lblocks;
+  const int64_t l = (lb * bx + (threadIdx.x & (bx - 1))) * V;
+  if (l >= a.s.L) return;
+  const A c = (A)a.scale;
+  GradRow<A> g[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) g[j] = grad_row<A>(a, o * a.s.L + l + j);
+  const T *x = static_cast<const T *>(a.x.p) + o * a.x.so + l;
+  T *out = static_cast<T *>(a.g.p) + o * a.g.so + l;
+  int64_t s = blockIdx.y * chunk;
+  const int64_t s1 = s + chunk < a.s.D ? s + chunk : a.s.D;
+  for (s += threadIdx.x >> bx_log2; s < s1; s += UN * by) {
+    Vec<T, V> w[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (s + u * by < s1) w[u] = *reinterpret_cast<const Vec<T, V> *>(x + (s + u * by) * a.x.sd);
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (s + u * by >= s1) break;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        A v = grad_value<A>(g[j], to_acc(w[u].v[j]), c);
+        if (g[j].t == (int)(s + u * by)) v += g[j].gt;
+        w[u].v[j] = from_acc<T, A>(v);
+      }
+      *reinterpret_cast<Vec<T, V> *>(out + (s + u * by) * a.g.sd) = w[u];
+    }
   }
 }
 
@@ -747,11 +796,52 @@ static acd_status launch_logprob(acd_ctx *ctx, const LogprobArgs &a, cudaStream_
   return a.k ? launch_rows<T, 1, true>(ctx, a, s) : launch_rows<T, 1, false>(ctx, a, s);
 }
 
+template <typename T, int V>
+static acd_status launch_grad_rows(acd_ctx *ctx, const LogprobGradArgs &a, cudaStream_t s) {
+  constexpr int64_t batch = (int64_t)BatchU<T, V>::value * V * 32;
+  const int64_t segs = (a.s.D + (V - 1) + batch - 1) / batch, tasks = segs * a.s.rows();
+  // tasks are counted in 32 bits, with room for the last stride of the grid
+  if (tasks > (int64_t)UINT32_MAX - (1 << 20))
+    return fail(ACD_ERR_UNSUPPORTED, "acd_token_logprob_grad: too many rows");
+  const int grid = persistent_grid(ctx, k_logprob_grad_rows<T, V>, 256, 0, (tasks + 7) / 8);
+  k_logprob_grad_rows<T, V><<<grid, 256, 0, s>>>(a, (uint32_t)segs, (uint32_t)tasks);
+  return ACD_OK;
+}
+
+template <typename T, int V>
+static acd_status launch_grad_lanes(acd_ctx *ctx, const LogprobGradArgs &a, cudaStream_t s) {
+  const int64_t nl = (a.s.L + V - 1) / V;
+  int bx_log2 = 0;
+  while (bx_log2 < 5 && (1 << bx_log2) < nl) ++bx_log2;
+  const int64_t bx = 1 << bx_log2, by = 256 >> bx_log2, lblocks = (nl + bx - 1) / bx, blocks = lblocks * a.s.O;
+  // 64 steps a thread pay for its coefficients; fewer where blocks are wanted
+  int64_t chunk = by * 64;
+  while (chunk > by * 8 && blocks * ((a.s.D + chunk - 1) / chunk) < (int64_t)ctx->sm_count * 16) chunk /= 2;
+  while ((a.s.D + chunk - 1) / chunk > 65535) chunk *= 2;
+  if (blocks > INT32_MAX) return fail(ACD_ERR_UNSUPPORTED, "acd_token_logprob_grad: too many rows");
+  const dim3 grid((unsigned)blocks, (unsigned)((a.s.D + chunk - 1) / chunk));
+  k_logprob_grad_lanes<T, V><<<grid, 256, 0, s>>>(a, bx_log2, lblocks, chunk);
+  return ACD_OK;
+}
+
 template <typename T>
 static acd_status launch_logprob_grad(acd_ctx *ctx, const LogprobGradArgs &a, cudaStream_t s) {
-  const int grid = persistent_grid(ctx, k_logprob_grad<T>, 256, 0, a.s.rows());
-  k_logprob_grad<T><<<grid, 256, 0, s>>>(a);
-  return ACD_OK;
+  constexpr int V = 16 / sizeof(T);
+  const int size = sizeof(T);
+  if (a.x.sd != 1 && a.x.sl == 1 && a.g.sl == 1 && a.s.L >= 8) {
+    auto wide = [&](int v) {  // every step starts on a boundary of v elements
+      return a.s.L % v == 0 && aligned_to<char>(a.x.p, v * size) && a.x.sd % v == 0 && a.x.so % v == 0 &&
+             pieces_match(a.x, a.g, a.x.sd, a.g.sd, v, size);
+    };
+    if (wide(V)) return launch_grad_lanes<T, V>(ctx, a, s);
+    if constexpr (sizeof(T) == 2) {
+      if (wide(2)) return launch_grad_lanes<T, 2>(ctx, a, s);
+    }
+    return launch_grad_lanes<T, 1>(ctx, a, s);
+  }
+  if (a.x.sd == 1 && a.g.sd == 1 && pieces_match(a.x, a.g, a.x.sl, a.g.sl, V, size))
+    return launch_grad_rows<T, V>(ctx, a, s);
+  return launch_grad_rows<T, 1>(ctx, a, s);
 }
 
 }  // namespace acd
