@@ -205,16 +205,450 @@ __global__ void __launch_bounds__(256) k_norm_grad_cols(NormGradArgs a, const ty
   }
 }
 
+// ---------------------------------------------------------------------------
+// contiguous rows
+// ---------------------------------------------------------------------------
+// The V columns of a row that thread `tid` of TPR has in its n-th piece.
+// WHOLE: 16 consecutive bytes; every row, weight and gate row starts on a
+// 16-byte boundary and D is a multiple of V.  Otherwise TPR apart, so that a
+// warp still reads neighbouring elements: any alignment, width and stride, and
+// a thread's columns are the same in every row (a piece moved by each row's
+// misalignment would not be, and its weights would be read 16 bytes apart).
+template <int V, int TPR, bool WHOLE>
+__device__ __forceinline__ int column(int tid, int n, int j) {
+  return WHOLE ? (n * TPR + tid) * V + j : (n * V + j) * TPR + tid;
+}
+
+template <typename T, typename A, int V, int TPR, bool WHOLE>
+__device__ __forceinline__ void load_cols(const T *x, int64_t sd, int tid, int n, int D, A *out) {
+  if (WHOLE) {
+    const int first = column<V, TPR, true>(tid, n, 0);
+    if (first < D) {
+      const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(x + first);
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[j] = to_acc(v.v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[j] = A(0);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int d = column<V, TPR, false>(tid, n, j);
+      out[j] = d < D ? to_acc(x[d * sd]) : A(0);
+    }
+  }
+}
+
+template <typename T, typename A, int V, int TPR, bool WHOLE>
+__device__ __forceinline__ void store_cols(T *x, int64_t sd, int tid, int n, int D, const A *v) {
+  if (WHOLE) {
+    const int first = column<V, TPR, true>(tid, n, 0);
+    if (first < D) {
+      Vec<T, V> w;
+#pragma unroll
+      for (int j = 0; j < V; ++j) w.v[j] = from_acc<T, A>(v[j]);
+      *reinterpret_cast<Vec<T, V> *>(x + first) = w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int d = column<V, TPR, false>(tid, n, j);
+      if (d < D) x[d * sd] = from_acc<T, A>(v[j]);
+    }
+  }
+}
+
+// Sums of N values over the TPR threads of a row, in every one of them.  sh
+// holds one set for each warp; two sets alternate, so that one barrier a sum
+// is enough.
+template <typename A, int N, int TPR>
+__device__ __forceinline__ void row_sum(A (&v)[N], A *sh) {
+#pragma unroll
+  for (int q = 16; q; q >>= 1)
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(~0u, v[j], q);
+  if (TPR > 32) {
+    constexpr int NW = TPR / 32;
+    const int warp = threadIdx.x >> 5, first = warp / NW * NW, lane = threadIdx.x & 31;
+    if (lane == 0)
+#pragma unroll
+      for (int j = 0; j < N; ++j) sh[warp * N + j] = v[j];
+    __syncthreads();
+    // the lanes take a warp's sum each
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = lane < NW ? sh[(first + lane) * N + j] : A(0);
+#pragma unroll
+    for (int q = 16; q; q >>= 1)
+      if (q < NW)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(~0u, v[j], q);
+    if (NW < 32)
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = __shfl_sync(~0u, v[j], 0);
+  }
+}
+
+// TPR threads a row, NV pieces of V columns a thread; the row stays in registers between
+// the two sums.
+template <typename T, int TPR, int NV, bool WHOLE>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = 16 / sizeof(T), BLOCK = TPR < 256 ? 256 : TPR;
+  __shared__ A sh[2][BLOCK / 32];
+  const int64_t row = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
+  const bool ok = row < a.s.rows();  // whole warps: a row has at least one
+  const int64_t rr = ok ? row : 0;
+  const int tid = threadIdx.x % TPR;
+  const int D = ok ? (int)a.s.D : 0;
+  const T *r = row_ptr<T>(a.r, rr, a.s.L), *b = row_ptr<T>(a.b, rr, a.s.L);
+  const T *w_pre = static_cast<const T *>(a.w_pre), *w_post = static_cast<const T *>(a.w_post);
+  const A alpha = (A)a.alpha, eps = (A)a.eps, inv = A(1) / (A)a.s.D;
+  A bv[NV][V], rv[NV][V];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    load_cols<T, A, V, TPR, WHOLE>(b, a.b.sd, tid, n, D, bv[n]);
+    load_cols<T, A, V, TPR, WHOLE>(r, a.r.sd, tid, n, D, rv[n]);
+  }
+  A rb = 1;
+  if (w_post) {
+    A q[1] = {A(0)};
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[0] = fma_a(bv[n][j], bv[n][j], q[0]);
+    row_sum<A, 1, TPR>(q, sh[0]);
+    rb = rsqrt_a(q[0] * inv + eps);
+  }
+  A q[1] = {A(0)};
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    A w[V];
+    if (w_post) {
+      load_cols<T, A, V, TPR, WHOLE>(w_post, 1, tid, n, D, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) bv[n][j] *= rb * w[j];
+    }
+    if (a.gate) {
+      load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + rr / a.per * a.gate_sg, a.gate_sd, tid, n, D, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) bv[n][j] *= w[j];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      bv[n][j] = fma_a(alpha, rv[n][j], bv[n][j]);
+      q[0] = fma_a(bv[n][j], bv[n][j], q[0]);
+    }
+  }
+  row_sum<A, 1, TPR>(q, sh[1]);
+  const A rh = rsqrt_a(q[0] * inv + eps);
+  if (!ok) return;
+  T *h = row_ptr<T>(a.h, rr, a.s.L), *y = row_ptr<T>(a.y, rr, a.s.L);
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    A w[V];
+    load_cols<T, A, V, TPR, WHOLE>(w_pre, 1, tid, n, D, w);
+    store_cols<T, A, V, TPR, WHOLE>(h, a.h.sd, tid, n, D, bv[n]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j] *= bv[n][j] * rh;
+    store_cols<T, A, V, TPR, WHOLE>(y, a.y.sd, tid, n, D, w);
+  }
+  if (tid == 0) {
+    if (a.rstd_h) static_cast<A *>(a.rstd_h)[row] = rh;
+    if (a.rstd_b) static_cast<A *>(a.rstd_b)[row] = rb;
+  }
+}
+
+// How the rows of a gradient call are dealt out: `parts` units a gate row,
+// unit u = (group u / parts, part u % parts); a block takes units u, u + grid,
+// ...  The column sums of a block's rows go to its own row of the partial
+// arrays, a unit's gate sums to the unit's row, and k_norm_grad_join adds them
+// in order.
+struct GradPlan {
+  int64_t groups, parts, per;
+  void *pre, *post;  // [grid][D]
+  void *gate;        // [groups * parts][D], or d_gate itself where parts = 1
+  int64_t gate_sd, gate_su;
+};
+
+// Which rows a unit has.
+__device__ __forceinline__ void unit_rows(const GradPlan &p, int64_t u, int64_t &r0, int64_t &r1) {
+  const int64_t g = u / p.parts, part = u - g * p.parts;
+  r0 = g * p.per + part * p.per / p.parts;
+  r1 = g * p.per + (part + 1) * p.per / p.parts;
+}
+
+// One piece of a row's gradient, in two steps around the row's sums.  With
+//   q = d_h + rs_h d_y w_pre,  hn = h rs_h,  bn = b rs_b,  e = gate w_post bn
+// t = q - rs_h hn m1, so that mean(u w_post bn) = mean(q e) - m1 mean(rs_h hn e)
+// comes from the same pass as m1 = mean(d_y w_pre hn): one reduction a row.
+template <typename T, typename A, int V, int TPR, bool WHOLE>
+struct GradPiece {
+  A dh[V], dy[V], h[V], b[V];
+  __device__ __forceinline__ void load(const NormGradArgs &a, int64_t row, int tid, int D) {
+    if (a.dh.p) {
+      load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dh, row, a.s.L), a.dh.sd, tid, 0, D, dh);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) dh[j] = A(0);
+    }
+    load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dy, row, a.s.L), a.dy.sd, tid, 0, D, dy);
+    load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.h, row, a.s.L), a.h.sd, tid, 0, D, h);
+    load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.b, row, a.s.L), a.b.sd, tid, 0, D, b);
+  }
+  __device__ __forceinline__ void sums(const A *wp, const A *wo, const A *g, A rh, A rb, A (&s)[3]) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const A hn = h[j] * rh, u = dy[j] * wp[j], e = g[j] * wo[j] * (b[j] * rb);
+      s[0] = fma_a(u, hn, s[0]);
+      s[1] = fma_a(fma_a(rh, u, dh[j]), e, s[1]);
+      s[2] = fma_a(rh * hn, e, s[2]);
+    }
+  }
+  // Leaves alpha t in dh and the block's gradient in dy; adds to the sums.
+  __device__ __forceinline__ void finish(const A *wp, const A *wo, const A *g, A rh, A rb, A m1, A m2, A alpha,
+                                         bool post, A *pre, A *pst, A *gte) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const A hn = h[j] * rh, bn = b[j] * rb;
+      const A t = fma_a(rh, fma_a(dy[j], wp[j], -(hn * m1)), dh[j]);
+      const A u = t * g[j];
+      pre[j] = fma_a(dy[j], hn, pre[j]);
+      pst[j] = fma_a(u, bn, pst[j]);
+      gte[j] = fma_a(t, bn * wo[j], gte[j]);
+      dh[j] = alpha * t;
+      dy[j] = post ? rb * fma_a(u, wo[j], -(bn * m2)) : u;
+    }
+  }
+};
+
+template <typename A, int V>
+__device__ __forceinline__ void ones(A *v) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = A(1);
+}
+
+// One piece a thread, TPR threads a row; the column sums stay in registers.
+template <typename T, int TPR, bool WHOLE>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_grad_vec(NormGradArgs a, GradPlan plan) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = 16 / sizeof(T), BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
+  __shared__ A sh[2][BLOCK / 32 * 3];
+  __shared__ A join[RPB > 1 ? BLOCK : 1][V];
+  const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int D = (int)a.s.D;
+  const T *w_pre = static_cast<const T *>(a.w_pre), *w_post = static_cast<const T *>(a.w_post);
+  const A alpha = (A)a.alpha, inv = A(1) / (A)a.s.D;
+  A pre[V] = {}, pst[V] = {};
+  int flip = 0;
+  for (int64_t u = blockIdx.x; u < plan.groups * plan.parts; u += gridDim.x) {
+    int64_t r0, r1;
+    unit_rows(plan, u, r0, r1);
+    A gte[V] = {};
+    for (int64_t rr = r0; rr < r1; rr += RPB) {
+      const int64_t row = rr + sub;
+      const bool ok = row < r1;
+      GradPiece<T, A, V, TPR, WHOLE> p;
+      p.load(a, ok ? row : r0, tid, ok ? D : 0);
+      A wp[V], wo[V], g[V];
+      load_cols<T, A, V, TPR, WHOLE>(w_pre, 1, tid, 0, D, wp);
+      if (w_post)
+        load_cols<T, A, V, TPR, WHOLE>(w_post, 1, tid, 0, D, wo);
+      else
+        ones<A, V>(wo);
+      if (a.gate)
+        load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + r0 / a.per * a.gate_sg, a.gate_sd, tid, 0, D, g);
+      else
+        ones<A, V>(g);
+      const A rh = ok ? static_cast<const A *>(a.rstd_h)[row] : A(0);
+      const A rb = w_post && ok ? static_cast<const A *>(a.rstd_b)[row] : A(1);
+      A s[3] = {};
+      p.sums(wp, wo, g, rh, rb, s);
+      row_sum<A, 3, TPR>(s, sh[flip]);
+      flip ^= 1;
+      const A m1 = s[0] * inv, m2 = (s[1] - m1 * s[2]) * inv;
+      p.finish(wp, wo, g, rh, rb, m1, m2, alpha, w_post != nullptr, pre, pst, gte);
+      if (ok) {
+        store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dr, row, a.s.L), a.dr.sd, tid, 0, D, p.dh);
+        store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.db, row, a.s.L), a.db.sd, tid, 0, D, p.dy);
+      }
+    }
+    if (plan.gate) {
+      if (RPB > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) join[threadIdx.x][j] = gte[j];
+        __syncthreads();
+        if (sub == 0)
+          for (int q = 1; q < RPB; ++q)
+#pragma unroll
+            for (int j = 0; j < V; ++j) gte[j] += join[q * TPR + tid][j];
+      }
+      if (sub == 0)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (column<V, TPR, WHOLE>(tid, 0, j) < D)
+            static_cast<A *>(plan.gate)[u * plan.gate_su + column<V, TPR, WHOLE>(tid, 0, j) * plan.gate_sd] = gte[j];
+    }
+  }
+  for (int w = 0; w < 2; ++w) {
+    A *dst = static_cast<A *>(w ? plan.post : plan.pre);
+    A *acc = w ? pst : pre;
+    if (!dst) continue;
+    if (RPB > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < V; ++j) join[threadIdx.x][j] = acc[j];
+      __syncthreads();
+      if (sub == 0)
+        for (int q = 1; q < RPB; ++q)
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] += join[q * TPR + tid][j];
+    }
+    if (sub == 0)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (column<V, TPR, WHOLE>(tid, 0, j) < D)
+          dst[(int64_t)blockIdx.x * D + column<V, TPR, WHOLE>(tid, 0, j)] = acc[j];
+  }
+}
+
+// Column sums of `n` partial rows: 32 columns a block, its 8 warps split the
+// rows and are added in order.
+template <typename A>
+struct JoinArgs {
+  const A *src[3];
+  A *dst[3];
+  int64_t n[3], sd[3], sg[3];  // rows a sum, strides of dst along the row and over its groups
+  int64_t D;
+};
+
+template <typename A>
+__global__ void __launch_bounds__(256) k_norm_grad_join(JoinArgs<A> a) {
+  __shared__ A sh[8][32];
+  // blockIdx.y: 0 pre, 1 post, 2 + g gate row g
+  const int w = blockIdx.y < 2 ? blockIdx.y : 2;
+  const int64_t g = w == 2 ? blockIdx.y - 2 : 0;
+  if (!a.dst[w]) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t d = (int64_t)blockIdx.x * 32 + lane, n = a.n[w];
+  A s = 0;
+  if (d < a.D) {
+    const A *p = a.src[w] + g * n * a.D + d;
+#pragma unroll 8
+    for (int64_t i = warp; i < n; i += 8) s += p[i * a.D];
+  }
+  sh[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && d < a.D) {
+    for (int q = 1; q < 8; ++q) s += sh[q][lane];
+    a.dst[w][d * a.sd[w] + g * a.sg[w]] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+// Whether the rows of `v` are contiguous and start on 16-byte boundaries (the
+// width is checked once, for all of them).
+static bool whole_rows(const Rows &v, int V) {
+  return v.sd == 1 && aligned_to<char>(v.p, 16) && v.sl % V == 0 && v.so % V == 0;
+}
+// Weights and gate rows too.
+static bool whole_weights(const void *w_pre, const void *w_post, const void *gate, int64_t sd, int64_t sg, int V) {
+  return aligned_to<char>(w_pre, 16) && (!w_post || aligned_to<char>(w_post, 16)) &&
+         (!gate || (aligned_to<char>(gate, 16) && sd == 1 && sg % V == 0));
+}
+
+template <typename T, int TPR, int NV>
+static acd_status launch_norm_vec(const NormArgs &a, bool whole, cudaStream_t s) {
+  constexpr int BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
+  const int64_t grid = (a.s.rows() + RPB - 1) / RPB;
+  if (whole)
+    k_norm_vec<T, TPR, NV, true><<<(unsigned)grid, BLOCK, 0, s>>>(a);
+  else
+    k_norm_vec<T, TPR, NV, false><<<(unsigned)grid, BLOCK, 0, s>>>(a);
+  return ACD_OK;
+}
+
 template <typename T>
 static acd_status launch_norm(acd_ctx *ctx, const NormArgs &a, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool whole = a.s.D % V == 0 && whole_rows(a.r, V) && whole_rows(a.b, V) && whole_rows(a.h, V) &&
+                     whole_rows(a.y, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
+  const int64_t pieces = (a.s.D + V - 1) / V;
+  if (pieces <= 4096) {
+    if (pieces <= 32) return launch_norm_vec<T, 32, 1>(a, whole, s);
+    if (pieces <= 64) return launch_norm_vec<T, 32, 2>(a, whole, s);
+    if (pieces <= 256) return launch_norm_vec<T, 128, 2>(a, whole, s);
+    if (pieces <= 512) return launch_norm_vec<T, 256, 2>(a, whole, s);
+    if (pieces <= 1024) return launch_norm_vec<T, 512, 2>(a, whole, s);
+    if (pieces <= 2048) return launch_norm_vec<T, 1024, 2>(a, whole, s);
+    return launch_norm_vec<T, 1024, 4>(a, whole, s);
+  }
   const int grid = persistent_grid(ctx, k_norm_rows<T>, 256, 0, a.s.rows());
   k_norm_rows<T><<<grid, 256, 0, s>>>(a);
+  return ACD_OK;
+}
+
+template <typename T, int TPR>
+static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool whole, cudaStream_t s) {
+  using A = typename AccOf<T>::type;
+  constexpr int BLOCK = TPR < 256 ? 256 : TPR;
+  auto kern = whole ? k_norm_grad_vec<T, TPR, true> : k_norm_grad_vec<T, TPR, false>;
+  const int64_t rows = a.s.rows(), D = a.s.D;
+  int64_t grid = (int64_t)ctx->sm_count * resident_blocks(reinterpret_cast<const void *>(kern), BLOCK, 0);
+  GradPlan p{};
+  p.per = a.per;
+  p.groups = rows / a.per;
+  p.parts = grid / p.groups;
+  if (p.parts > (p.per + BLOCK / TPR - 1) / (BLOCK / TPR)) p.parts = (p.per + BLOCK / TPR - 1) / (BLOCK / TPR);
+  if (p.parts < 1) p.parts = 1;
+  if (grid > p.groups * p.parts) grid = p.groups * p.parts;
+  const bool gate_part = a.d_gate && p.parts > 1;
+  const size_t cols = sizeof(A) * (size_t)D;
+  void *scratch;
+  ACD_TRY(get_scratch(ctx, cols * (2 * grid + (gate_part ? p.groups * p.parts : 0)), s, &scratch));
+  A *pre = static_cast<A *>(scratch), *post = pre + grid * D, *gate = post + grid * D;
+  p.pre = a.d_w_pre ? pre : nullptr;
+  p.post = a.d_w_post ? post : nullptr;
+  p.gate = a.d_gate ? (gate_part ? gate : a.d_gate) : nullptr;
+  p.gate_sd = gate_part ? 1 : a.gate_sd;
+  p.gate_su = gate_part ? D : a.gate_sg;
+  kern<<<(unsigned)grid, BLOCK, 0, s>>>(a, p);
+  JoinArgs<A> j{};
+  j.D = D;
+  j.src[0] = pre;
+  j.src[1] = post;
+  j.src[2] = gate;
+  j.dst[0] = static_cast<A *>(a.d_w_pre);
+  j.dst[1] = static_cast<A *>(a.d_w_post);
+  j.dst[2] = gate_part ? static_cast<A *>(a.d_gate) : nullptr;
+  j.n[0] = j.n[1] = grid;
+  j.n[2] = p.parts;
+  j.sd[0] = j.sd[1] = 1;
+  j.sd[2] = a.gate_sd;
+  j.sg[2] = a.gate_sg;
+  if (j.dst[0] || j.dst[1] || j.dst[2])
+    k_norm_grad_join<A><<<dim3((unsigned)((D + 31) / 32), (unsigned)(2 + (gate_part ? p.groups : 0))), 256, 0, s>>>(j);
   return ACD_OK;
 }
 
 template <typename T>
 static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStream_t s) {
   using A = typename AccOf<T>::type;
+  constexpr int V = 16 / sizeof(T);
+  const bool whole = a.s.D % V == 0 && whole_rows(a.dr, V) && whole_rows(a.db, V) &&
+                     (!a.dh.p || whole_rows(a.dh, V)) && whole_rows(a.dy, V) && whole_rows(a.h, V) &&
+                     whole_rows(a.b, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
+  const int64_t pieces = (a.s.D + V - 1) / V;
+  if (pieces <= 1024) {
+    if (pieces <= 32) return launch_norm_grad_vec<T, 32>(ctx, a, whole, s);
+    if (pieces <= 128) return launch_norm_grad_vec<T, 128>(ctx, a, whole, s);
+    if (pieces <= 256) return launch_norm_grad_vec<T, 256>(ctx, a, whole, s);
+    if (pieces <= 512) return launch_norm_grad_vec<T, 512>(ctx, a, whole, s);
+    return launch_norm_grad_vec<T, 1024>(ctx, a, whole, s);
+  }
   void *scratch;
   ACD_TRY(get_scratch(ctx, sizeof(A) * (size_t)a.s.rows(), s, &scratch));
   A *means = static_cast<A *>(scratch);
