@@ -127,6 +127,15 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, u
       : "memory");
 }
 
+// 2-D tiled load of one box.
+__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+          "r"(smem_addr(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(smem_addr(bar))
+      : "memory");
+}
+
 // 3-D tiled store of one box from shared memory (bulk-group completion).
 // Parts of the box outside the tensor are not written.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void *src, int c0, int c1, int c2) {
@@ -160,6 +169,12 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 bool encode_tensor_map_3d(CUtensorMap *map, const void *base, int elem_bytes, const int64_t dims[3],
                           const int64_t strides_elems[2], const uint32_t box[3], bool swizzle128 = true,
                           bool promote256 = true);
+
+// Host: `rows` rows of `width` bytes, `pitch` bytes apart (base 16-byte aligned,
+// pitch a multiple of 16), as boxes of 128 bytes by box_rows rows, 128-byte
+// swizzle.
+bool encode_tensor_map_bytes(CUtensorMap *map, const void *base, int64_t width, int64_t rows, int64_t pitch,
+                             uint32_t box_rows);
 
 // Host: TMA-staged transpose of 4-byte elements, out(i,j,k) = in(i,j,k) with
 // out contiguous along i (extent n0, j stride os1, k stride os2) and in

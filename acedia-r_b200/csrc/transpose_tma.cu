@@ -200,6 +200,17 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 
 }  // namespace
 
+bool encode_tensor_map_bytes(CUtensorMap *map, const void *base, int64_t width, int64_t rows, int64_t pitch,
+                             uint32_t box_rows) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  const cuuint64_t gd[2] = {(cuuint64_t)width, (cuuint64_t)rows}, gs[1] = {(cuuint64_t)pitch};
+  const cuuint32_t bx[2] = {128, box_rows}, es[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), gd, gs, bx, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool encode_tensor_map_3d(CUtensorMap *map, const void *base, int elem_bytes, const int64_t dims[3],
                           const int64_t strides_elems[2], const uint32_t box[3], bool swizzle128,
                           bool promote256) {

@@ -165,7 +165,8 @@ acd_status acd_ctx_set_allocator(acd_ctx *ctx, acd_alloc_fn alloc, acd_free_fn f
  * Returns ACD_ERR_DEVICE and fills *code when a kernel reported an error:
  * 1 = the scan's look-back wait expired, 2 = a wait of the TMA transpose
  * pipeline expired, 3 = the TMA load wait of the cluster softmax expired,
- * 4 = the row softmax's wait for a lane group's statistics expired. */
+ * 4 = the row softmax's wait for a lane group's statistics expired, 5 = the
+ * 4-bit product's wait for its weights expired. */
 acd_status acd_ctx_check(acd_ctx *ctx, acd_stream stream, int32_t *code);
 /* Test hook for the bounded look-back wait of the scan: when `tile` >= 0,
  * the scan kernel's tile with that index never publishes its prefix, so the
@@ -471,7 +472,9 @@ acd_status acd_residual_norm_grad(acd_ctx *ctx, const acd_desc *d_residual, cons
  * FLOAT16 or FLOAT32 of shape [ceil(in / group), out], contiguous; zeros may
  * be NULL.  group is a positive multiple of 32.  x: [in] or [in, n], out:
  * [out] or [out, n], FLOAT16 or FLOAT32 each, any strides, not overlapping.
- * Products are summed in float32 in an order set by the shapes alone. */
+ * Products are summed in float32 in an order set by the shapes alone.  An
+ * infinite or NaN activation reaches its own column only; with zeros an
+ * infinite one may give NaN (the zero points are summed apart). */
 acd_status acd_quant4_matvec(acd_ctx *ctx, const acd_desc *out, const acd_desc *weights, const acd_desc *scales,
                              const acd_desc *zeros, const acd_desc *x, int32_t group, acd_stream stream);
 /* Makes weights, scales (and zeros) from w, an [out, in] view of FLOAT16,
