@@ -38,43 +38,56 @@ __device__ __forceinline__ void store_f(void *p, bool half, int64_t i, float v) 
 // ---------------------------------------------------------------------------
 // the product
 // ---------------------------------------------------------------------------
-// A block takes 128 outputs and a range of the inputs. One thread brings the
-// weights in by TMA, 128 outputs x 128 bytes (256 inputs) at a time through a
-// ring of stages; eight warps of 16 outputs each multiply them with the legacy
-// matrix instruction m16n8k16 (a product with a few columns is bound by the
-// bytes of its weights: a tcgen05 tile of 128 columns would be empty but for
-// these).  The order of the inputs inside the instruction is free as long as
-// weights and activations agree, so the four threads of a row take 8
-// consecutive inputs each, one 4-byte word, of every 32: a group's inputs never
-// share an instruction with another group's.
+// A block takes 64 outputs at a time and a range of the inputs.  One thread
+// brings the weights in by TMA through a ring of stages of 64 outputs x 256
+// bytes (two tiles of 256 inputs); eight warps multiply them, 16 outputs by one
+// of the two tiles each, with the legacy matrix instruction m16n8k16 (a product
+// with a few columns is bound by the bytes of its weights: a tcgen05 tile of
+// 128 columns would be empty but for these).  The order of the inputs inside
+// the instruction is free as long as weights and activations agree, so the four
+// threads of a row take 8 consecutive inputs each, one 4-byte word, of every
+// 32: a group's inputs never share an instruction with another group's.
 //   Weights become exact small integers n - 8 in float16 (bfloat16 for float32
 // activations) by putting the four bits into the mantissa of 1024 (128) and
-// subtracting; scales are applied to the float32 sums of 32 inputs:
-//   y += s (sum (n - 8) x + (8 - z) sum x).
-//   float32 activations are split into three bfloat16 parts that hold all 24
-// bits, which go in as three columns.
-constexpr int kRowsPerBlock = 128;
-constexpr int kTileBytes = 128;               // of one output: 256 inputs, 8 chunks of 32
-constexpr int kStageBytes = kRowsPerBlock * kTileBytes;
+// subtracting; scales are applied to the float32 sums of SUB * 32 inputs:
+//   y = sum_groups s sum (n - 8) x  +  sum_groups s (8 - z) sum x,
+// the second term from sums of x that are made once.  float32 activations are
+// split into three bfloat16 parts that hold all 24 bits, which go in as three
+// columns.
+constexpr int kRowsPerBlock = 64;
+constexpr int kTileBytes = 128;                       // of one output: 256 inputs, 8 chunks of 32
+constexpr int kBoxBytes = kRowsPerBlock * kTileBytes;
+constexpr int kStageBytes = 2 * kBoxBytes;
 constexpr int kStages = 4;
-constexpr int kXBytes = 44 * 1024;            // activations of a segment, and their sums
 constexpr uint64_t kQWaitNs = 1000000000ull;  // 1 s
 constexpr int kQWaitCode = 5;
 
 struct Quant4Plan {
-  int ktiles, tper;    // tiles of 256 inputs: in all, a block
+  int mblocks;         // blocks of 64 outputs
+  int ktiles, tper;    // tiles of 256 inputs: in all, a block of a cluster (even, or all)
   int seg;             // tiles whose activations are in shared memory at once
   int vectors;         // columns of x a block (gridDim.y blocks of them)
   int cols;            // matrix columns: vectors, or three for each
-  FastDiv chunks;      // chunks of 32 inputs a group
+  int group;           // chunks of 32 inputs a group
+  FastDiv chunks;      // the same, to divide by
+  bool wide;           // a lane's scales of a tile are one aligned load
 };
+
+// Columns of x that 8 NT matrix columns hold.
+template <bool X16, int NT>
+struct Q4Vectors { static constexpr int value = X16 ? 8 * NT : 8 * NT / 3; };
 
 template <bool X16>
 struct Q4Type { using H2 = __half2; };
 template <>
 struct Q4Type<false> { using H2 = __nv_bfloat162; };
 
-__device__ __forceinline__ uint32_t and_or(uint32_t q, uint32_t m, uint32_t o) { return (q & m) | o; }
+// (q & m) | o in one instruction (the truth table of a lop3).
+__device__ __forceinline__ uint32_t and_or(uint32_t q, uint32_t m, uint32_t o) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(q), "r"(m), "r"(o));
+  return r;
+}
 
 // Eight weights of a word: w[i] holds inputs i and i + 4 as n - 8.
 template <bool X16>
@@ -106,15 +119,31 @@ template <bool X16>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   if constexpr (X16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The first product of a sum.
+template <bool X16>
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  if constexpr (X16)
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+  else
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Inputs i and i + 4 of eight side by side, as unpack8 leaves the weights.
@@ -137,15 +166,29 @@ __device__ __forceinline__ uint16_t take_bf16(float &x) {
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
+// Shared memory by its 32-bit address, so that the compiler neither widens it
+// nor adds a base to every access.  volatile: not moved over the waits.
+template <int OFFSET>
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(r) : "r"(at), "n"(OFFSET) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
+
 struct Quant4Shared {
   uint64_t full[kStages], empty[kStages];
   int abort;
 };
 
 // Activations of the chunks of tiles [tile, tile + n) in the order of the
-// instruction's operand, [chunk][thread of a row][column] of 16 bytes, and
-// their sums, [chunk][8 NT].
-template <bool X16, int NT>
+// instruction's operand, [chunk][thread of a row][column] of 16 bytes, and the
+// sums of SUB chunks each, [.][VS].
+template <bool X16, int SUB, int VS, bool ZEROS>
 __device__ __forceinline__ void stage_x(const Quant4Args &a, const Quant4Plan &p, int tile, int n, int v0, uint4 *xf,
                                         float *sx) {
   const int vectors = a.N - v0 < p.vectors ? (int)(a.N - v0) : p.vectors;
@@ -188,33 +231,43 @@ __device__ __forceinline__ void stage_x(const Quant4Args &a, const Quant4Plan &p
         }
       }
     }
-    sum += __shfl_xor_sync(~0u, sum, 1);
-    sum += __shfl_xor_sync(~0u, sum, 2);
-    if (i < items && (it & 3) == 0) {
-      float *s = sx + (it >> 2) * (8 * NT) + (X16 ? v : 3 * v);
-      s[0] = sum;
-      if (!X16) s[1] = s[2] = 0.0f;
+    if (ZEROS) {
+      // four items a chunk, side by side; 4 SUB of them divide a warp
+#pragma unroll
+      for (int q = 1; q < 4 * SUB; q <<= 1) sum += __shfl_xor_sync(~0u, sum, q);
+      if (i < items && it % (4 * SUB) == 0) sx[it / (4 * SUB) * VS + v] = sum;
     }
   }
 }
 
+// The value of an output's column v from its sums.
 template <bool X16, int NT, bool ZEROS>
+__device__ __forceinline__ float row_value(const float *red, int v) {
+  const float y = X16 ? red[v] : red[3 * v] + (red[3 * v + 1] + red[3 * v + 2]);
+  return ZEROS ? y + red[8 * NT + v] : y;
+}
+
+template <bool X16, int NT, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ CUtensorMap map, Quant4Args a,
                                                        Quant4Plan p, Control *control) {
+  constexpr int VS = Q4Vectors<X16, NT>::value, RED = 8 * NT + (ZEROS ? VS : 0), SLOTS = 4 / SUB;
   extern __shared__ unsigned char smem[];
   __shared__ Quant4Shared sh;
   // the swizzle goes by the address: stages start on 1024 bytes
   unsigned char *stages = smem + ((1024u - (smem_addr(smem) & 1023u)) & 1023u);
-  uint4 *xf = reinterpret_cast<uint4 *>(stages + kStages * kStageBytes);
+  float *red = reinterpret_cast<float *>(stages + kStages * kStageBytes);  // [64][RED]
+  uint4 *xf = reinterpret_cast<uint4 *>(red + kRowsPerBlock * RED);
   float *sx = reinterpret_cast<float *>(xf + p.seg * 32 * p.cols);
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t o0 = (int64_t)(blockIdx.x / C) * kRowsPerBlock;
+  const int mstep = gridDim.x / C;
   const int v0 = blockIdx.y * p.vectors;
+  const int vectors = a.N - v0 < p.vectors ? (int)(a.N - v0) : p.vectors;
   const int t0 = rank * p.tper;
   int nt = p.ktiles - t0;
   nt = nt > p.tper ? p.tper : nt < 0 ? 0 : nt;
+  const int ns = (nt + 1) / 2;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh.full[i], 1);
@@ -224,145 +277,241 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
     mbar_init_fence();
   }
   __syncthreads();
-  float tot[NT][4] = {};
   if (warp == 8) {
     if (lane == 0) {
-      int i = 0;
-      for (; i < nt; ++i) {
-        const int slot = i % kStages;
-        if (i >= kStages && !mbar_wait_thread(&sh.empty[slot], (uint32_t)(i / kStages - 1) & 1u, &sh.abort, control,
-                                              kQWaitCode, kQWaitNs))
-          break;
-        mbar_arrive_expect_tx(&sh.full[slot], kStageBytes);
-        tma_load_2d(stages + slot * kStageBytes, &map, &sh.full[slot], (t0 + i) * kTileBytes, (int)o0);
-      }
+      int n = 0;  // stages filled so far
+      bool go = true;
+      for (int mb = blockIdx.x / C; go && mb < p.mblocks; mb += mstep)
+        for (int i = 0; i < ns; ++i, ++n) {
+          const int slot = n % kStages;
+          if (n >= kStages && !mbar_wait_thread(&sh.empty[slot], (uint32_t)(n / kStages - 1) & 1u, &sh.abort, control,
+                                                kQWaitCode, kQWaitNs)) {
+            go = false;
+            break;
+          }
+          const bool two = 2 * i + 1 < nt;  // a tile past the range is not loaded
+          unsigned char *st = stages + slot * kStageBytes;
+          mbar_arrive_expect_tx(&sh.full[slot], two ? kStageBytes : kBoxBytes);
+          tma_load_2d(st, &map, &sh.full[slot], (t0 + 2 * i) * kTileBytes, mb * kRowsPerBlock);
+          if (two) tma_load_2d(st + kBoxBytes, &map, &sh.full[slot], (t0 + 2 * i + 1) * kTileBytes, mb * kRowsPerBlock);
+        }
       // given up: the copies in flight land before the block may end
       if (*reinterpret_cast<volatile int *>(&sh.abort))
-        for (int q = i > kStages ? i - kStages : 0; q < i; ++q)
+        for (int q = n > kStages ? n - kStages : 0; q < n; ++q)
           mbar_wait_bounded(&sh.full[q % kStages], (uint32_t)(q / kStages) & 1u, kQWaitNs);
     }
   } else {
-    const int g = lane >> 2, t = lane & 3;
-    // Scales of a tile: lane 2 r + h holds row r's chunks 4 h .. 4 h + 3.
-    float sc[4], zc[4];
-    const int64_t srow = o0 + warp * 16 + (lane >> 1);
-    auto load_scales = [&](int tile) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t gi = p.chunks.div((uint32_t)(tile * 8 + (lane & 1) * 4 + q));
-        const bool ok = srow < a.M && gi < a.ngroups;
-        const int64_t at = srow * a.ngroups + gi;
-        sc[q] = ok ? load_f(a.scales, a.scale16, at) : 0.0f;
-        if (ZEROS) zc[q] = ok ? sc[q] * (8.0f - load_f(a.zeros, a.scale16, at)) : 0.0f;
-      }
-    };
-    bool dead = false;
-    for (int i = 0; i < nt; ++i) {
-      if (i % p.seg == 0) {
-        if (i) consumer_sync();  // the segment before has been read
-        stage_x<X16, NT>(a, p, t0 + i, nt - i < p.seg ? nt - i : p.seg, v0, xf, sx);
-        consumer_sync();
-      }
-      load_scales(t0 + i);
-      const int slot = i % kStages;
-      // once given up, the warps go on without waiting: all of them reach the barriers
-      dead = dead || !mbar_wait_warp(&sh.full[slot], (uint32_t)(i / kStages) & 1u, &sh.abort, control, kQWaitCode,
-                                     kQWaitNs);
-      const unsigned char *st = stages + slot * kStageBytes + (warp * 16 + g) * kTileBytes + t * 4;
-      const uint4 *xc = xf + (i % p.seg) * 32 * p.cols + t * p.cols;
-      const float *sc_x = sx + (i % p.seg) * 8 * (8 * NT) + 2 * t;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const uint32_t q0 = *reinterpret_cast<const uint32_t *>(st + ((c ^ g) << 4));
-        const uint32_t q1 = *reinterpret_cast<const uint32_t *>(st + 8 * kTileBytes + ((c ^ g) << 4));
-        uint32_t w0[4], w1[4];
-        unpack8<X16>(q0, w0);
-        unpack8<X16>(q1, w1);
-        const float s0 = __shfl_sync(~0u, sc[c & 3], 2 * g + (c >> 2)), s1 = __shfl_sync(~0u, sc[c & 3], 2 * g + 16 + (c >> 2));
-        float z0 = 0, z1 = 0;
-        if (ZEROS) {
-          z0 = __shfl_sync(~0u, zc[c & 3], 2 * g + (c >> 2));
-          z1 = __shfl_sync(~0u, zc[c & 3], 2 * g + 16 + (c >> 2));
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          uint4 b = make_uint4(0, 0, 0, 0);
-          if (n * 8 + g < p.cols) b = xc[c * 4 * p.cols + n * 8 + g];
-          float part[4] = {};
-          mma16816<X16>(part, w0[0], w1[0], w0[1], w1[1], b.x, b.y);
-          mma16816<X16>(part, w0[2], w1[2], w0[3], w1[3], b.z, b.w);
-          tot[n][0] = fmaf(s0, part[0], tot[n][0]);
-          tot[n][1] = fmaf(s0, part[1], tot[n][1]);
-          tot[n][2] = fmaf(s1, part[2], tot[n][2]);
-          tot[n][3] = fmaf(s1, part[3], tot[n][3]);
-          if (ZEROS) {
-            const float2 x = *reinterpret_cast<const float2 *>(sc_x + c * (8 * NT) + n * 8);
-            tot[n][0] = fmaf(z0, x.x, tot[n][0]);
-            tot[n][1] = fmaf(z0, x.y, tot[n][1]);
-            tot[n][2] = fmaf(z1, x.x, tot[n][2]);
-            tot[n][3] = fmaf(z1, x.y, tot[n][3]);
-          }
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[slot]);
-    }
-  }
-  // the blocks of a cluster hold sums of different inputs of the same outputs
-  __syncthreads();
-  float *red = reinterpret_cast<float *>(stages);  // [128][8 NT], over the stages
-  if (warp < 8) {
-    const int g = lane >> 2, t = lane & 3;
+    const int g = lane >> 2, t = lane & 3, half = warp >> 2, row0 = (warp & 3) * 16;
+    // activation columns of this lane; beyond the last one any finite address
+    // does, their results are not stored
+    uint32_t xcol[NT];
+    const uint32_t xstep = 4 * 16 * p.cols;  // bytes of a chunk
 #pragma unroll
     for (int n = 0; n < NT; ++n)
+      xcol[n] = smem_addr(xf) + 16 * (t * p.cols + (n * 8 + g < p.cols ? n * 8 + g : p.cols - 1));
+    // scales of a tile: lane 2 r + h holds row r's of chunks 4 h .. 4 h + 3
+    // (the next tile's as loaded: converting them would wait for the load)
+    float sc[SLOTS], zc[SLOTS];
+    uint32_t sn[SLOTS], zn[SLOTS];
+    auto load_raw = [&](const void *x, int64_t i) -> uint32_t {
+      return a.scale16 ? static_cast<const uint16_t *>(x)[i] : static_cast<const uint32_t *>(x)[i];
+    };
+    auto value = [&](uint32_t raw) {
+      return a.scale16 ? __half2float(__ushort_as_half((uint16_t)raw)) : __uint_as_float(raw);
+    };
+    const uint32_t ng = (uint32_t)a.ngroups;
+    int64_t srow = 0;  // this lane's row of scales
+    bool sok = false;
+    auto scale_row = [&](int mb) {
+      const int64_t o = (int64_t)mb * kRowsPerBlock + row0 + (lane >> 1);
+      srow = o * a.ngroups;
+      sok = o < a.M;
+    };
+    auto load_scales = [&](int tile) {
+      const uint32_t chunk = tile * 8 + (lane & 1) * 4;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        red[(warp * 16 + g + 8 * (q >> 1)) * (8 * NT) + n * 8 + 2 * t + (q & 1)] = tot[n][q];
+      for (int q = 0; q < SLOTS; ++q) sn[q] = zn[q] = 0;
+      if (SUB < 4 && p.wide) {  // groups of SUB chunks, their number a multiple of the lane's
+        const uint32_t gi = chunk / SUB;
+        if (sok && gi < ng) {
+          using S = Vec<uint16_t, SLOTS>;
+          const S s = *reinterpret_cast<const S *>(static_cast<const uint16_t *>(a.scales) + srow + gi);
+#pragma unroll
+          for (int q = 0; q < SLOTS; ++q) sn[q] = s.v[q];
+          if (ZEROS) {
+            const S z = *reinterpret_cast<const S *>(static_cast<const uint16_t *>(a.zeros) + srow + gi);
+#pragma unroll
+            for (int q = 0; q < SLOTS; ++q) zn[q] = z.v[q];
+          }
+        }
+        return;
+      }
+#pragma unroll
+      for (int q = 0; q < SLOTS; ++q) {
+        const uint32_t gi = p.chunks.div(chunk + q * SUB);
+        if (sok && gi < ng) {
+          sn[q] = load_raw(a.scales, srow + gi);
+          if (ZEROS) zn[q] = load_raw(a.zeros, srow + gi);
+        }
+      }
+    };
+    const uint32_t lane_addr = smem_addr(stages) + half * kBoxBytes + (row0 + g) * kTileBytes + (g << 4) + t * 4;
+    bool dead = false;
+    int slot = 0, staged = -1;  // staged: first tile of the activations in shared memory
+    uint32_t phase = 0;
+    scale_row(blockIdx.x / C);
+    if (half < nt) load_scales(t0 + half);
+    for (int mb = blockIdx.x / C; mb < p.mblocks; mb += mstep) {
+      float tot[NT][4] = {};
+      float corr[ZEROS ? VS : 1] = {};
+      int seg0 = 0;
+      for (int i = 0; i < ns; ++i) {
+        const int tile = 2 * i + half;  // of this block's range
+        if (2 * i >= seg0 + p.seg) seg0 += p.seg;
+        if (seg0 != staged) {
+          if (staged >= 0) consumer_sync();  // the segment before has been read
+          stage_x<X16, SUB, VS, ZEROS>(a, p, t0 + seg0, nt - seg0 < p.seg ? nt - seg0 : p.seg, v0, xf, sx);
+          consumer_sync();
+          staged = seg0;
+        }
+#pragma unroll
+        for (int q = 0; q < SLOTS; ++q) {
+          sc[q] = value(sn[q]);
+          zc[q] = sc[q] * (8.0f - value(zn[q]));
+        }
+        // the next tile's scales are on their way while this one is worked on
+        if (tile + 2 < nt) {
+          load_scales(t0 + tile + 2);
+        } else if (i + 1 == ns && mb + mstep < p.mblocks && half < nt) {
+          scale_row(mb + mstep);
+          load_scales(t0 + half);
+        }
+        // once given up, the warps go on without waiting: all of them reach the barriers
+        dead = dead || !mbar_wait_warp(&sh.full[slot], phase, &sh.abort, control, kQWaitCode, kQWaitNs);
+        if (tile < nt) {
+          const uint32_t st = lane_addr + slot * kStageBytes;
+          uint32_t xt[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + (tile - seg0) * 8 * xstep;
+          float part[NT][4];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t w0[4], w1[4];
+            const uint32_t q0 = lds32<0>(st ^ (c << 4)), q1 = lds32<8 * kTileBytes>(st ^ (c << 4));
+            unpack8<X16>(q0, w0);
+            unpack8<X16>(q1, w1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint4 b = lds128(xt[n]);
+              xt[n] += xstep;
+              if (c % SUB == 0)
+                mma16816_zero<X16>(part[n], w0[0], w1[0], w0[1], w1[1], b.x, b.y);
+              else
+                mma16816<X16>(part[n], w0[0], w1[0], w0[1], w1[1], b.x, b.y);
+              mma16816<X16>(part[n], w0[2], w1[2], w0[3], w1[3], b.z, b.w);
+            }
+            if (c % SUB == SUB - 1) {
+              const float s0 = __shfl_sync(~0u, sc[(c & 3) / SUB], 2 * g + (c >> 2));
+              const float s1 = __shfl_sync(~0u, sc[(c & 3) / SUB], 2 * g + 16 + (c >> 2));
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                tot[n][0] = fmaf(s0, part[n][0], tot[n][0]);
+                tot[n][1] = fmaf(s0, part[n][1], tot[n][1]);
+                tot[n][2] = fmaf(s1, part[n][2], tot[n][2]);
+                tot[n][3] = fmaf(s1, part[n][3], tot[n][3]);
+              }
+            }
+          }
+          if (ZEROS) {
+            const float *s = sx + ((tile - seg0) * (8 / SUB) + (lane & 1) * SLOTS) * VS;
+#pragma unroll
+            for (int v = 0; v < VS; ++v) {
+              if (v >= vectors) break;
+#pragma unroll
+              for (int q = 0; q < SLOTS; ++q) corr[v] = fmaf(zc[q], s[q * VS + v], corr[v]);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[slot]);
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+      // the second tiles' sums join the first ones'
+      auto exchange = [&](auto f) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            f(red[(row0 + g + 8 * (q >> 1)) * RED + n * 8 + 2 * t + (q & 1)], tot[n][q]);
+        if (ZEROS && (lane & 1) == 0)
+#pragma unroll
+          for (int v = 0; v < VS; ++v) f(red[(row0 + (lane >> 1)) * RED + 8 * NT + v], corr[v]);
+      };
+      if (ZEROS)
+#pragma unroll
+        for (int v = 0; v < VS; ++v) corr[v] += __shfl_xor_sync(~0u, corr[v], 1);
+      if (half) exchange([](float &r, float x) { r = x; });
+      consumer_sync();
+      if (!half) {
+        exchange([](float &r, float x) { r += x; });
+        __syncwarp();
+        if (C == 1)
+          for (int i = lane; i < 16 * vectors; i += 32) {
+            const int r = row0 + (i & 15), v = i >> 4;
+            const int64_t o = (int64_t)mb * kRowsPerBlock + r;
+            if (o < a.M) store_f(a.out, a.out16, o * a.os + (v0 + v) * a.oc, row_value<X16, NT, ZEROS>(red + r * RED, v));
+          }
+      }
+      if (mb + mstep < p.mblocks) consumer_sync();  // red is written again
+    }
   }
-  if (C > 1)
-    cluster.sync();
-  else
-    __syncthreads();
-  const int rows = kRowsPerBlock / C;
-  const int vectors = a.N - v0 < p.vectors ? (int)(a.N - v0) : p.vectors;
+  if (C == 1) return;
+  // the blocks of a cluster hold sums over different inputs of the same outputs
+  cluster.sync();
+  const int mb = blockIdx.x / C, r0 = rank * kRowsPerBlock / C, rows = (rank + 1) * kRowsPerBlock / C - r0;
   for (int i = threadIdx.x; i < rows * vectors; i += 288) {
-    const int v = i / rows, r = rank * rows + i - v * rows;
-    const int64_t o = o0 + r;
+    const int v = i / rows, r = r0 + i - v * rows;
+    const int64_t o = (int64_t)mb * kRowsPerBlock + r;
     if (o >= a.M) continue;
     float y = 0;
-    for (int q = 0; q < C; ++q) {
-      const float *other = C > 1 ? cluster.map_shared_rank(red, q) : red;
-      if (X16) {
-        y += other[r * (8 * NT) + v];
-      } else {
-#pragma unroll
-        for (int w = 2; w >= 0; --w) y += other[r * (8 * NT) + 3 * v + w];
-      }
-    }
+    for (int q = 0; q < C; ++q) y += row_value<X16, NT, ZEROS>(cluster.map_shared_rank(red, q) + r * RED, v);
     store_f(a.out, a.out16, o * a.os + (v0 + v) * a.oc, y);
   }
-  if (C > 1) cluster.sync();  // no block leaves while its shared memory is read
+  cluster.sync();  // no block leaves while its shared memory is read
 }
 
-template <bool X16, int NT, bool ZEROS>
-static acd_status launch_mma(acd_ctx *ctx, const Quant4Args &a, Quant4Plan &p, int cluster, const CUtensorMap &map,
+constexpr int kBlockSmem = 112 * 1024;   // two blocks an SM
+constexpr int kWholeSmem = 226 * 1024;   // one
+
+template <bool X16, int NT, int SUB, bool ZEROS>
+static acd_status launch_mma(acd_ctx *ctx, const Quant4Args &a, Quant4Plan &p, int C, const CUtensorMap &map,
                              cudaStream_t s) {
-  // a tile of x: 32 pieces of 16 bytes a column, 8 sums a column
-  const int per = 32 * 16 * p.cols + 8 * 4 * 8 * NT;
-  p.seg = kXBytes / per;
-  if (p.seg > p.tper) p.seg = p.tper;
-  const int dyn = 1024 + kStages * kStageBytes + p.seg * per;
-  auto kern = k_quant4_mma<X16, NT, ZEROS>;
+  constexpr int VS = Q4Vectors<X16, NT>::value, RED = 8 * NT + (ZEROS ? VS : 0);
+  // a tile of x: 32 pieces of 16 bytes a column, 8 / SUB sums
+  const int per = 32 * 16 * p.cols + (ZEROS ? 8 / SUB * 4 * VS : 0);
+  const int fixed = 1024 + kStages * kStageBytes + kRowsPerBlock * RED * 4;
+  const int64_t blocks = (int64_t)p.mblocks * C, columns = (a.N + p.vectors - 1) / p.vectors;
+  // an even number of tiles, so that a stage's two are in one segment
+  const bool whole = blocks * columns <= ctx->sm_count || (kBlockSmem - fixed) / per < 2;
+  p.seg = ((whole ? kWholeSmem : kBlockSmem) - fixed) / per & ~1;
+  if (p.seg > ((p.tper + 1) & ~1)) p.seg = (p.tper + 1) & ~1;
+  const int dyn = fixed + p.seg * per;
+  auto kern = k_quant4_mma<X16, NT, SUB, ZEROS>;
   ACD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn));
+  int64_t grid = blocks;
+  const int64_t resident = (int64_t)ctx->sm_count * (dyn > kBlockSmem ? 1 : 2);
+  if (C == 1 && grid > resident) grid = resident;  // persistent
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.M + kRowsPerBlock - 1) / kRowsPerBlock * cluster),
-                     (unsigned)((a.N + p.vectors - 1) / p.vectors), 1);
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)columns, 1);
   cfg.blockDim = dim3(288, 1, 1);
   cfg.dynamicSmemBytes = dyn;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.x = C;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -374,12 +523,26 @@ static acd_status launch_mma(acd_ctx *ctx, const Quant4Args &a, Quant4Plan &p, i
 static acd_status launch_quant4(acd_ctx *ctx, const Quant4Args &a, cudaStream_t s) {
   Quant4Plan p{};
   p.ktiles = (int)((a.K + 255) / 256);
-  p.chunks = FastDiv((uint32_t)(a.group / 32));
-  // blocks along the inputs: while two blocks an SM are not reached
-  const int64_t mblocks = (a.M + kRowsPerBlock - 1) / kRowsPerBlock;
+  p.mblocks = (int)((a.M + kRowsPerBlock - 1) / kRowsPerBlock);
+  p.group = a.group / 32;
+  p.chunks = FastDiv((uint32_t)p.group);
+  const int sub = p.group % 4 == 0 ? 4 : p.group % 2 == 0 ? 2 : 1;
+  const int slots = 4 / sub;
+  p.wide = p.group == sub && a.scale16 && a.ngroups % slots == 0 && aligned_to<char>(a.scales, 2 * slots) &&
+           (!a.zeros || aligned_to<char>(a.zeros, 2 * slots));
+  // blocks a cluster, along the inputs: an SM works through its blocks' stages
+  // and about two stages' time of starting and joining each
   int C = 1;
-  while (C < 8 && mblocks * C * 2 <= ctx->sm_count * 2 && p.ktiles >= C * 2) C *= 2;
-  p.tper = (p.ktiles + C - 1) / C;
+  int64_t best = INT64_MAX;
+  for (int c = 1; c <= 8 && c <= (p.ktiles + 1) / 2; ++c) {
+    const int64_t stages = ((p.ktiles + 1) / 2 + c - 1) / c;
+    const int64_t cost = ((int64_t)p.mblocks * c + ctx->sm_count - 1) / ctx->sm_count * (stages + 2);
+    if (cost < best) {
+      best = cost;
+      C = c;
+    }
+  }
+  p.tper = C == 1 ? p.ktiles : ((p.ktiles + 1) / 2 + C - 1) / C * 2;
   const int most = a.x16 ? 32 : 10;  // columns of four instructions
   p.vectors = a.N < most ? (int)a.N : most;
   p.cols = a.x16 ? p.vectors : 3 * p.vectors;
@@ -387,15 +550,22 @@ static acd_status launch_quant4(acd_ctx *ctx, const Quant4Args &a, cudaStream_t 
   CUtensorMap map;
   if (!encode_tensor_map_bytes(&map, a.w, a.pitch, a.M, a.pitch, kRowsPerBlock))
     return fail(ACD_ERR_CUDA, "acd_quant4_matvec: the driver rejects the weights' tensor map");
-  auto go = [&](auto x16, auto n) {
-    return a.zeros ? launch_mma<decltype(x16)::value, decltype(n)::value, true>(ctx, a, p, C, map, s)
-                   : launch_mma<decltype(x16)::value, decltype(n)::value, false>(ctx, a, p, C, map, s);
+  auto go = [&](auto x16, auto n, auto sb) {
+    constexpr bool X = decltype(x16)::value;
+    constexpr int NT = decltype(n)::value, SUB = decltype(sb)::value;
+    return a.zeros ? launch_mma<X, NT, SUB, true>(ctx, a, p, C, map, s)
+                   : launch_mma<X, NT, SUB, false>(ctx, a, p, C, map, s);
+  };
+  auto grouped = [&](auto x16, auto n) {
+    if (sub == 4) return go(x16, n, std::integral_constant<int, 4>());
+    if (sub == 2) return go(x16, n, std::integral_constant<int, 2>());
+    return go(x16, n, std::integral_constant<int, 1>());
   };
   auto width = [&](auto x16) {
-    if (p.cols <= 8) return go(x16, std::integral_constant<int, 1>());
-    if (p.cols <= 16) return go(x16, std::integral_constant<int, 2>());
-    if (p.cols <= 24) return go(x16, std::integral_constant<int, 3>());
-    return go(x16, std::integral_constant<int, 4>());
+    if (p.cols <= 8) return grouped(x16, std::integral_constant<int, 1>());
+    if (p.cols <= 16) return grouped(x16, std::integral_constant<int, 2>());
+    if (p.cols <= 24) return grouped(x16, std::integral_constant<int, 3>());
+    return grouped(x16, std::integral_constant<int, 4>());
   };
   return a.x16 ? width(std::true_type()) : width(std::false_type());
 }
