@@ -6,6 +6,8 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <cfloat>
+
 #include "common.cuh"
 #include "tma.cuh"
 
@@ -40,8 +42,8 @@ __device__ __forceinline__ void store_f(void *p, bool half, int64_t i, float v) 
 // ---------------------------------------------------------------------------
 // A block takes 64 outputs at a time and a range of the inputs.  One thread
 // brings the weights in by TMA through a ring of stages of 64 outputs x 256
-// bytes (two tiles of 256 inputs); eight warps multiply them, 16 outputs by one
-// of the two tiles each, with the legacy matrix instruction m16n8k16 (a product
+// bytes (two tiles of 256 inputs); eight warps multiply them, 16 outputs a warp,
+// every second stage each, with the legacy matrix instruction m16n8k16 (a product
 // with a few columns is bound by the bytes of its weights: a tcgen05 tile of
 // 128 columns would be empty but for these).  The order of the inputs inside
 // the instruction is free as long as weights and activations agree, so the four
@@ -58,7 +60,6 @@ constexpr int kRowsPerBlock = 64;
 constexpr int kTileBytes = 128;                       // of one output: 256 inputs, 8 chunks of 32
 constexpr int kBoxBytes = kRowsPerBlock * kTileBytes;
 constexpr int kStageBytes = 2 * kBoxBytes;
-constexpr int kStages = 4;
 constexpr uint64_t kQWaitNs = 1000000000ull;  // 1 s
 constexpr int kQWaitCode = 5;
 
@@ -68,10 +69,15 @@ struct Quant4Plan {
   int seg;             // tiles whose activations are in shared memory at once
   int vectors;         // columns of x a block (gridDim.y blocks of them)
   int cols;            // matrix columns: vectors, or three for each
+  int xcols;           // places for them: 2 more than a multiple of 4, whose 16-byte reads meet no bank twice
   int group;           // chunks of 32 inputs a group
   FastDiv chunks;      // the same, to divide by
-  bool wide;           // a lane's scales of a tile are one aligned load
+  bool wide;           // a tile's scales are one aligned load
 };
+
+// Stages of the ring: with more columns their activations want the room.
+template <int NT>
+struct Q4Stages { static constexpr int value = NT == 1 ? 4 : 3; };
 
 // Columns of x that 8 NT matrix columns hold.
 template <bool X16, int NT>
@@ -152,16 +158,17 @@ __device__ __forceinline__ uint4 interleave8(const uint16_t (&h)[8]) {
                     h[3] | (uint32_t)h[7] << 16);
 }
 
-// Truncates to bfloat16; what is cut off is exact in float32.  Infinities and
-// NaN are whole in the first part.
-__device__ __forceinline__ uint16_t take_bf16(float &x) {
-  const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7F800000u) == 0x7F800000u) {
-    x = 0.0f;
-    return (uint16_t)((u >> 16) | ((u & 0x7FFFFFu) ? 0x40u : 0u));
+// Eight float32 activations as a bfloat16 part each, side by side like
+// interleave8; f is left with what the part cuts off, exact in float32.
+__device__ __forceinline__ uint4 take_bf16(float (&f)[8]) {
+  uint32_t u[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    u[j] = __float_as_uint(f[j]);
+    f[j] -= __uint_as_float(u[j] & 0xFFFF0000u);
   }
-  x -= __uint_as_float(u & 0xFFFF0000u);
-  return (uint16_t)(u >> 16);
+  return make_uint4(__byte_perm(u[0], u[4], 0x7632), __byte_perm(u[1], u[5], 0x7632), __byte_perm(u[2], u[6], 0x7632),
+                    __byte_perm(u[3], u[7], 0x7632));
 }
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -180,8 +187,9 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
   return r;
 }
 
+template <int STAGES>
 struct Quant4Shared {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[STAGES], empty[STAGES];
   int abort;
 };
 
@@ -213,22 +221,33 @@ __device__ __forceinline__ void stage_x(const Quant4Args &a, const Quant4Plan &p
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += __half2float(__ushort_as_half(h[j]));
-        xf[it * p.cols + v] = interleave8(h);
+        xf[it * p.xcols + v] = interleave8(h);
       } else {
         const float *x = static_cast<const float *>(a.x) + at;
         float f[8];
+        if (a.xs == 1 && k + 8 <= a.K && aligned_to<char>(x, 16)) {
+          const float4 lo = reinterpret_cast<const float4 *>(x)[0], hi = reinterpret_cast<const float4 *>(x)[1];
+          f[0] = lo.x, f[1] = lo.y, f[2] = lo.z, f[3] = lo.w;
+          f[4] = hi.x, f[5] = hi.y, f[6] = hi.z, f[7] = hi.w;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          f[j] = k + j < a.K ? x[j * a.xs] : 0.0f;
-          sum += f[j];
+          for (int j = 0; j < 8; ++j) f[j] = k + j < a.K ? x[j * a.xs] : 0.0f;
         }
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
-          uint16_t h[8];
+        for (int j = 0; j < 8; ++j) sum += f[j];
+        const bool fine = fabsf(sum) <= FLT_MAX;  // else an infinity or NaN may be among them
+        uint4 *to = xf + it * p.xcols + 3 * v;
+        if (!fine) {  // a NaN whose set bits would be cut off
 #pragma unroll
-          for (int j = 0; j < 8; ++j) h[j] = take_bf16(f[j]);
-          xf[it * p.cols + 3 * v + q] = interleave8(h);
+          for (int j = 0; j < 8; ++j) f[j] = f[j] != f[j] ? NAN : f[j];
         }
+        to[0] = take_bf16(f);
+        if (!fine) {  // whole in the first part: Inf - Inf is not to be added
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = f[j] != f[j] ? 0.0f : f[j];
+        }
+        to[1] = take_bf16(f);
+        to[2] = take_bf16(f);
       }
     }
     if (ZEROS) {
@@ -240,6 +259,12 @@ __device__ __forceinline__ void stage_x(const Quant4Args &a, const Quant4Plan &p
   }
 }
 
+// Floats between two outputs' sums in shared memory: 8 more than a multiple of
+// 32, so that the 8 rows and 4 column pairs that a warp writes at once lie in
+// different banks.
+template <int N>
+struct SumsStride { static constexpr int value = N <= 8 ? 8 : (N - 8 + 31) / 32 * 32 + 8; };
+
 // The value of an output's column v from its sums.
 template <bool X16, int NT, bool ZEROS>
 __device__ __forceinline__ float row_value(const float *red, int v) {
@@ -250,14 +275,15 @@ __device__ __forceinline__ float row_value(const float *red, int v) {
 template <bool X16, int NT, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ CUtensorMap map, Quant4Args a,
                                                        Quant4Plan p, Control *control) {
-  constexpr int VS = Q4Vectors<X16, NT>::value, RED = 8 * NT + (ZEROS ? VS : 0), SLOTS = 4 / SUB;
+  constexpr int VS = Q4Vectors<X16, NT>::value, RED = SumsStride<8 * NT + (ZEROS ? VS : 0)>::value, SLOTS = 8 / SUB;
+  constexpr int kStages = Q4Stages<NT>::value;
   extern __shared__ unsigned char smem[];
-  __shared__ Quant4Shared sh;
+  __shared__ Quant4Shared<kStages> sh;
   // the swizzle goes by the address: stages start on 1024 bytes
   unsigned char *stages = smem + ((1024u - (smem_addr(smem) & 1023u)) & 1023u);
   float *red = reinterpret_cast<float *>(stages + kStages * kStageBytes);  // [64][RED]
   uint4 *xf = reinterpret_cast<uint4 *>(red + kRowsPerBlock * RED);
-  float *sx = reinterpret_cast<float *>(xf + p.seg * 32 * p.cols);
+  float *sx = reinterpret_cast<float *>(xf + p.seg * 32 * p.xcols);
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -271,7 +297,7 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 8);
+      mbar_init(&sh.empty[i], 4);
     }
     sh.abort = 0;
     mbar_init_fence();
@@ -301,16 +327,16 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
           mbar_wait_bounded(&sh.full[q % kStages], (uint32_t)(q / kStages) & 1u, kQWaitNs);
     }
   } else {
-    const int g = lane >> 2, t = lane & 3, half = warp >> 2, row0 = (warp & 3) * 16;
+    const int g = lane >> 2, t = lane & 3, odd = warp >> 2, row0 = (warp & 3) * 16;
     // activation columns of this lane; beyond the last one any finite address
     // does, their results are not stored
     uint32_t xcol[NT];
-    const uint32_t xstep = 4 * 16 * p.cols;  // bytes of a chunk
+    const uint32_t xstep = 4 * 16 * p.xcols;  // bytes of a chunk
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      xcol[n] = smem_addr(xf) + 16 * (t * p.cols + (n * 8 + g < p.cols ? n * 8 + g : p.cols - 1));
-    // scales of a tile: lane 2 r + h holds row r's of chunks 4 h .. 4 h + 3
-    // (the next tile's as loaded: converting them would wait for the load)
+      xcol[n] = smem_addr(xf) + 16 * (t * p.xcols + (n * 8 + g < p.cols ? n * 8 + g : p.cols - 1));
+    // scales of a stage: lane 2 r + h holds row r's of its tile h (the next
+    // stage's as loaded: converting them would wait for the load)
     float sc[SLOTS], zc[SLOTS];
     uint32_t sn[SLOTS], zn[SLOTS];
     auto load_raw = [&](const void *x, int64_t i) -> uint32_t {
@@ -328,10 +354,10 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
       sok = o < a.M;
     };
     auto load_scales = [&](int tile) {
-      const uint32_t chunk = tile * 8 + (lane & 1) * 4;
+      const uint32_t chunk = (tile + (lane & 1)) * 8;
 #pragma unroll
       for (int q = 0; q < SLOTS; ++q) sn[q] = zn[q] = 0;
-      if (SUB < 4 && p.wide) {  // groups of SUB chunks, their number a multiple of the lane's
+      if (p.wide) {  // groups of SUB chunks, their number a multiple of a tile's
         const uint32_t gi = chunk / SUB;
         if (sok && gi < ng) {
           using S = Vec<uint16_t, SLOTS>;
@@ -355,44 +381,48 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
         }
       }
     };
-    const uint32_t lane_addr = smem_addr(stages) + half * kBoxBytes + (row0 + g) * kTileBytes + (g << 4) + t * 4;
+    const uint32_t lane_addr = smem_addr(stages) + (row0 + g) * kTileBytes + (g << 4) + t * 4;
     bool dead = false;
-    int slot = 0, staged = -1;  // staged: first tile of the activations in shared memory
-    uint32_t phase = 0;
+    int staged = -1;     // first tile of the activations in shared memory
+    uint32_t stage = 0;  // stages of the blocks before
     scale_row(blockIdx.x / C);
-    if (half < nt) load_scales(t0 + half);
-    for (int mb = blockIdx.x / C; mb < p.mblocks; mb += mstep) {
+    if (odd < ns) load_scales(t0 + 2 * odd);
+    for (int mb = blockIdx.x / C; mb < p.mblocks; mb += mstep, stage += ns) {
       float tot[NT][4] = {};
       float corr[ZEROS ? VS : 1] = {};
       int seg0 = 0;
-      for (int i = 0; i < ns; ++i) {
-        const int tile = 2 * i + half;  // of this block's range
-        if (2 * i >= seg0 + p.seg) seg0 += p.seg;
+      for (int j = 0; j < ns; j += 2) {
+        const int i = j + odd, tile = 2 * i;  // this warp's stage, and its tiles of this block's range
+        if (2 * j >= seg0 + p.seg) seg0 += p.seg;
         if (seg0 != staged) {
           if (staged >= 0) consumer_sync();  // the segment before has been read
           stage_x<X16, SUB, VS, ZEROS>(a, p, t0 + seg0, nt - seg0 < p.seg ? nt - seg0 : p.seg, v0, xf, sx);
           consumer_sync();
           staged = seg0;
         }
+        if (i >= ns) continue;
 #pragma unroll
         for (int q = 0; q < SLOTS; ++q) {
           sc[q] = value(sn[q]);
           zc[q] = sc[q] * (8.0f - value(zn[q]));
         }
-        // the next tile's scales are on their way while this one is worked on
-        if (tile + 2 < nt) {
-          load_scales(t0 + tile + 2);
-        } else if (i + 1 == ns && mb + mstep < p.mblocks && half < nt) {
+        // the next stage's scales are on their way while this one is worked on
+        if (i + 2 < ns) {
+          load_scales(t0 + tile + 4);
+        } else if (mb + mstep < p.mblocks) {
           scale_row(mb + mstep);
-          load_scales(t0 + half);
+          load_scales(t0 + 2 * odd);
         }
+        const uint32_t slot = (stage + i) % kStages;
         // once given up, the warps go on without waiting: all of them reach the barriers
-        dead = dead || !mbar_wait_warp(&sh.full[slot], phase, &sh.abort, control, kQWaitCode, kQWaitNs);
-        if (tile < nt) {
-          const uint32_t st = lane_addr + slot * kStageBytes;
-          uint32_t xt[NT];
+        dead = dead || !mbar_wait_warp(&sh.full[slot], (stage + i) / kStages & 1u, &sh.abort, control, kQWaitCode,
+                                       kQWaitNs);
+        uint32_t xt[NT];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + (tile - seg0) * 8 * xstep;
+        for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + (tile - seg0) * 8 * xstep;
+#pragma unroll 1
+        for (int h = 0; h < 2 && tile + h < nt; ++h) {
+          const uint32_t st = lane_addr + slot * kStageBytes + h * kBoxBytes;
           float part[NT][4];
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
@@ -411,8 +441,7 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
               mma16816<X16>(part[n], w0[2], w1[2], w0[3], w1[3], b.z, b.w);
             }
             if (c % SUB == SUB - 1) {
-              const float s0 = __shfl_sync(~0u, sc[(c & 3) / SUB], 2 * g + (c >> 2));
-              const float s1 = __shfl_sync(~0u, sc[(c & 3) / SUB], 2 * g + 16 + (c >> 2));
+              const float s0 = __shfl_sync(~0u, sc[c / SUB], 2 * g + h), s1 = __shfl_sync(~0u, sc[c / SUB], 2 * g + 16 + h);
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 tot[n][0] = fmaf(s0, part[n][0], tot[n][0]);
@@ -422,24 +451,20 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
               }
             }
           }
-          if (ZEROS) {
-            const float *s = sx + ((tile - seg0) * (8 / SUB) + (lane & 1) * SLOTS) * VS;
+        }
+        if (ZEROS && tile + (lane & 1) < nt) {
+          const float *s = sx + (tile + (lane & 1) - seg0) * SLOTS * VS;
 #pragma unroll
-            for (int v = 0; v < VS; ++v) {
-              if (v >= vectors) break;
+          for (int v = 0; v < VS; ++v) {
+            if (v >= vectors) break;
 #pragma unroll
-              for (int q = 0; q < SLOTS; ++q) corr[v] = fmaf(zc[q], s[q * VS + v], corr[v]);
-            }
+            for (int q = 0; q < SLOTS; ++q) corr[v] = fmaf(zc[q], s[q * VS + v], corr[v]);
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.empty[slot]);
-        if (++slot == kStages) {
-          slot = 0;
-          phase ^= 1u;
-        }
       }
-      // the second tiles' sums join the first ones'
+      // the odd stages' sums join the even ones'
       auto exchange = [&](auto f) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -453,9 +478,9 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
       if (ZEROS)
 #pragma unroll
         for (int v = 0; v < VS; ++v) corr[v] += __shfl_xor_sync(~0u, corr[v], 1);
-      if (half) exchange([](float &r, float x) { r = x; });
+      if (odd) exchange([](float &r, float x) { r = x; });
       consumer_sync();
-      if (!half) {
+      if (!odd) {
         exchange([](float &r, float x) { r += x; });
         __syncwarp();
         if (C == 1)
@@ -489,15 +514,16 @@ constexpr int kWholeSmem = 226 * 1024;   // one
 template <bool X16, int NT, int SUB, bool ZEROS>
 static acd_status launch_mma(acd_ctx *ctx, const Quant4Args &a, Quant4Plan &p, int C, const CUtensorMap &map,
                              cudaStream_t s) {
-  constexpr int VS = Q4Vectors<X16, NT>::value, RED = 8 * NT + (ZEROS ? VS : 0);
+  constexpr int VS = Q4Vectors<X16, NT>::value, RED = SumsStride<8 * NT + (ZEROS ? VS : 0)>::value;
+  constexpr int kStages = Q4Stages<NT>::value;
   // a tile of x: 32 pieces of 16 bytes a column, 8 / SUB sums
-  const int per = 32 * 16 * p.cols + (ZEROS ? 8 / SUB * 4 * VS : 0);
+  const int per = 32 * 16 * p.xcols + (ZEROS ? 8 / SUB * 4 * VS : 0);
   const int fixed = 1024 + kStages * kStageBytes + kRowsPerBlock * RED * 4;
   const int64_t blocks = (int64_t)p.mblocks * C, columns = (a.N + p.vectors - 1) / p.vectors;
-  // an even number of tiles, so that a stage's two are in one segment
-  const bool whole = blocks * columns <= ctx->sm_count || (kBlockSmem - fixed) / per < 2;
-  p.seg = ((whole ? kWholeSmem : kBlockSmem) - fixed) / per & ~1;
-  if (p.seg > ((p.tper + 1) & ~1)) p.seg = (p.tper + 1) & ~1;
+  // whole pairs of stages, of which the warps take one each
+  const bool whole = blocks * columns <= ctx->sm_count || (kBlockSmem - fixed) / per < 4;
+  p.seg = ((whole ? kWholeSmem : kBlockSmem) - fixed) / per & ~3;
+  if (p.seg > ((p.tper + 3) & ~3)) p.seg = (p.tper + 3) & ~3;
   const int dyn = fixed + p.seg * per;
   auto kern = k_quant4_mma<X16, NT, SUB, ZEROS>;
   ACD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn));
@@ -527,7 +553,7 @@ static acd_status launch_quant4(acd_ctx *ctx, const Quant4Args &a, cudaStream_t 
   p.group = a.group / 32;
   p.chunks = FastDiv((uint32_t)p.group);
   const int sub = p.group % 4 == 0 ? 4 : p.group % 2 == 0 ? 2 : 1;
-  const int slots = 4 / sub;
+  const int slots = 8 / sub;
   p.wide = p.group == sub && a.scale16 && a.ngroups % slots == 0 && aligned_to<char>(a.scales, 2 * slots) &&
            (!a.zeros || aligned_to<char>(a.zeros, 2 * slots));
   // blocks a cluster, along the inputs: an SM works through its blocks' stages
@@ -546,6 +572,7 @@ static acd_status launch_quant4(acd_ctx *ctx, const Quant4Args &a, cudaStream_t 
   const int most = a.x16 ? 32 : 10;  // columns of four instructions
   p.vectors = a.N < most ? (int)a.N : most;
   p.cols = a.x16 ? p.vectors : 3 * p.vectors;
+  p.xcols = p.cols == 1 ? 1 : (p.cols + 1) / 4 * 4 + 2;
   if ((a.N + most - 1) / most > 65535) return fail(ACD_ERR_UNSUPPORTED, "acd_quant4_matvec: too many columns");
   CUtensorMap map;
   if (!encode_tensor_map_bytes(&map, a.w, a.pitch, a.M, a.pitch, kRowsPerBlock))
