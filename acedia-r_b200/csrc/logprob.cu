@@ -56,6 +56,31 @@ struct LpMath<float> {
   static __device__ __forceinline__ float lowest() { return -FLT_MAX; }
   static __device__ __forceinline__ float max2(float a, float b) { return fmaxf(a, b); }
 };
+// Two float32 values in one register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 template <>
 struct LpMath<double> {
   static constexpr double kUnit = 1.0;
@@ -65,6 +90,41 @@ struct LpMath<double> {
   static __device__ __forceinline__ double lowest() { return -DBL_MAX; }
   static __device__ __forceinline__ double max2(double a, double b) { return fmax(a, b); }
 };
+
+// V neighbouring logits as they lie in memory; float16 pairs as words, so that
+// they take no more registers than bytes until they are widened.
+template <typename T, int V>
+struct Piece {
+  Vec<T, V> d;
+  template <typename A>
+  __device__ __forceinline__ void widen(A *f) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = to_acc(d.v[j]);
+  }
+  __device__ __forceinline__ void set(int j, T x) { d.v[j] = x; }
+};
+template <int V>
+struct Half2Piece {
+  Vec<uint32_t, V / 2> d;
+  __device__ __forceinline__ void widen(float *f) const {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&d.v[j / 2]));
+      f[j] = p.x;
+      f[j + 1] = p.y;
+    }
+  }
+  __device__ __forceinline__ void set(int j, __half x) {
+    const uint32_t h = __half_as_ushort(x);
+    d.v[j / 2] = j % 2 ? (d.v[j / 2] & 0xFFFFu) | h << 16 : (d.v[j / 2] & 0xFFFF0000u) | h;
+  }
+};
+template <>
+struct Piece<__half, 2> : Half2Piece<2> {};
+template <>
+struct Piece<__half, 4> : Half2Piece<4> {};
+template <>
+struct Piece<__half, 8> : Half2Piece<8> {};
 
 // m starts at the lowest finite value, so that -Inf - m is -Inf and never NaN:
 // a part of -Inf only keeps S = 0.  floor_z keeps T free of 0 * Inf.  A NaN
@@ -83,20 +143,39 @@ struct Part {
     s *= f;
     m = mn;
   }
-  // N logits whose maximum is bm: one rescaling for all of them.
+  // N logits against the present m.
   template <int N>
-  __device__ __forceinline__ void add(const A (&x)[N], A bm, A c) {
-    rescale(LpMath<A>::max2(m, bm), c);
-    A ls = 0, lt = 0;
+  __device__ __forceinline__ void sum(const A (&x)[N], A c) {
+    if constexpr (std::is_same<A, float>::value && N % 2 == 0) {
+      const uint64_t nm = pack2(-m, -m), cc = pack2(c, c);
+      uint64_t s2 = pack2(0.0f, 0.0f), t2 = s2;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const A z = LpMath<A>::floor_z((x[j] - m) * c);
-      const A e = LpMath<A>::ex(z);
-      ls += e;
-      lt = fma_a(e, z, lt);
+      for (int j = 0; j < N; j += 2) {
+        float z0, z1;
+        unpack2(mul2(add2(pack2(x[j], x[j + 1]), nm), cc), z0, z1);
+        z0 = LpMath<A>::floor_z(z0);
+        z1 = LpMath<A>::floor_z(z1);
+        const uint64_t e = pack2(LpMath<A>::ex(z0), LpMath<A>::ex(z1));
+        s2 = add2(s2, e);
+        t2 = fma2(e, pack2(z0, z1), t2);
+      }
+      float a0, a1;
+      unpack2(s2, a0, a1);
+      s += a0 + a1;
+      unpack2(t2, a0, a1);
+      t += a0 + a1;
+    } else {
+      A ls = 0, lt = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const A z = LpMath<A>::floor_z((x[j] - m) * c);
+        const A e = LpMath<A>::ex(z);
+        ls += e;
+        lt = fma_a(e, z, lt);
+      }
+      s += ls;
+      t += lt;
     }
-    s += ls;
-    t += lt;
   }
   __device__ __forceinline__ void merge(Part o, A c) {
     const A mn = LpMath<A>::max2(m, o.m);
@@ -167,6 +246,23 @@ struct TopList {
       mask &= __ballot_sync(~0u, better(x, xi, kv, ki));
     }
   }
+  // 32 unsorted logits, one a lane: sorted the other way round, then merged.
+  __device__ __forceinline__ void merge_unsorted(A x, int xi) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+      for (int q = size >> 1; q; q >>= 1) {
+        const A ov = __shfl_xor_sync(~0u, x, q);
+        const int oi = __shfl_xor_sync(~0u, xi, q);
+        const bool worse = ((lane & size) == 0) == ((lane & q) == 0);  // this lane keeps the worse one
+        if (worse == better(x, xi, ov, oi)) {
+          x = ov;
+          xi = oi;
+        }
+      }
+    merge_reversed(x, xi);
+  }
   // Another sorted list, lane q holding its entry 31 - q: the better of each
   // pair is a bitonic sequence of the 32 best; five exchanges sort it.
   __device__ __forceinline__ void merge_reversed(A ov, int oi) {
@@ -202,86 +298,113 @@ __device__ __forceinline__ A kth_of_lanes(A x, int k) {
   return __shfl_sync(~0u, x, k - 1);
 }
 
-// What one warp knows of the part of a row that it has read.  A batch is N =
-// U * V logits a lane: lane l holds elements base + u*32*V + l*V + j.  Batches
-// come with rising base, so a later logit that equals entry k - 1 never wins.
-// `floor`: some k logits of the row are at least this large.
-template <typename A, int U, int V, bool TOP>
+// Looks through a batch of U * V values a lane for what belongs to the list:
+// lane l holds elements base + u*32*V + l*V + j, bm is its largest.  Batches
+// come with rising base, so a later value that equals entry k - 1 never wins.
+// `floor`: some k values are at least this large.  Only lanes whose largest
+// value can enter the list are looked at, one after the other, the warp reading
+// such a lane's values together from `spread` in shared memory.
+template <typename A, int U, int V>
+__device__ __forceinline__ void search_batch(TopList<A> &top, const A (&x)[U * V], A bm, int base, int D, int k, A floor,
+                                             A *spread) {
+  const bool first = top.ki == kNone;
+  if (!first && !__any_sync(~0u, bm > top.kv && bm >= floor)) return;
+  // k lanes' maxima are at least as large as the k-th of them
+  if (first) floor = LpMath<A>::max2(floor, kth_of_lanes(bm, k));
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < V; ++j) spread[(u * 32 + lane) * V + j] = x[u * V + j];
+  __syncwarp();
+  unsigned mask = __ballot_sync(~0u, bm >= floor && (first || bm > top.kv));
+#pragma unroll 1
+  while (mask) {
+    const int src = __ffs(mask) - 1, at = (lane / V * 32 + src) * V + lane % V, xi = base + at;
+    const bool mine = lane < U * V && xi >= 0 && xi < D;
+    top.offer(mine ? spread[at] : A(0), xi, mine, floor, k);
+    mask &= mask - 1;
+    mask &= __ballot_sync(~0u, bm >= top.kv);
+  }
+  __syncwarp();
+}
+
+template <typename A, int N>
+__device__ __forceinline__ A largest(const A (&x)[N]) {
+  A m = LpMath<A>::max2(x[0], A(-INFINITY));
+#pragma unroll
+  for (int j = 1; j < N; ++j) m = LpMath<A>::max2(m, x[j]);
+  return m;
+}
+
+// What one warp knows of the part of a row that it has read.
+template <typename T, int U, int V, bool TOP>
 struct RowState {
+  using A = typename AccOf<T>::type;
   Part<A> p;
   TopList<A> top;
   __device__ __forceinline__ void init() {
     p.init();
     if (TOP) top.init();
   }
-  __device__ __forceinline__ void batch(const A (&x)[U * V], int base, int D, A c, int k, A floor) {
-    A vm[U], bm;
+  __device__ __forceinline__ void batch(const Piece<T, V> (&raw)[U], int base, int D, A c, int k, A floor, A *spread) {
+    A x[U * V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      vm[u] = x[u * V];
-#pragma unroll
-      for (int j = 1; j < V; ++j) vm[u] = LpMath<A>::max2(vm[u], x[u * V + j]);
-      bm = u ? LpMath<A>::max2(bm, vm[u]) : LpMath<A>::max2(vm[0], A(-INFINITY));
-    }
-    p.add(x, bm, c);
-    if (TOP) {
-      const bool first = top.ki == kNone;
-      if (!first && !__any_sync(~0u, bm > top.kv && bm >= floor)) return;
-      // k lanes' maxima are at least as large as the k-th of them
-      if (first) floor = LpMath<A>::max2(floor, kth_of_lanes(bm, k));
-      const int lane = threadIdx.x & 31;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!__any_sync(~0u, vm[u] >= floor && vm[u] >= top.kv)) continue;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int xi = base + (u * 32 + lane) * V + j;
-          top.offer(x[u * V + j], xi, xi >= 0 && xi < D, floor, k);
-        }
-      }
-    }
+    for (int u = 0; u < U; ++u) raw[u].widen(x + u * V);
+    const A bm = largest(x);
+    p.rescale(LpMath<A>::max2(p.m, bm), c);  // once for all of them
+    p.sum(x, c);
+    if (TOP) search_batch<A, U, V>(top, x, bm, base, D, k, floor, spread);
   }
 };
 
-// The row's results from what is known of all of it; called by a whole warp.
-template <typename A, bool TOP>
-__device__ __forceinline__ void finish_row(const LogprobArgs &a, int64_t r, const Part<A> &p, A v, int i, int64_t t,
-                                           A xt) {
-  const int lane = threadIdx.x & 31;
-  const bool empty = p.s == A(0);  // every logit -Inf
-  const A c = (A)a.scale;
-  const A log_s = empty ? A(0) : lp_log(p.s);
-  if (lane == 0) {
-    if (a.lse) static_cast<A *>(a.lse)[r] = empty ? A(-INFINITY) : fma_a(c, p.m, log_s);
+// A row's results from what is known of all of it: statistics by one thread,
+// alternatives one by one.
+template <typename A>
+struct RowResult {
+  A m, log_s;
+  __device__ __forceinline__ RowResult(const LogprobArgs &a, const Part<A> &p)
+      : m(p.m), log_s(p.s == A(0) ? A(0) : lp_log(p.s)) {}
+  __device__ __forceinline__ void stats(const LogprobArgs &a, int64_t r, const Part<A> &p, int64_t t, A xt) const {
+    const bool empty = p.s == A(0);  // every logit -Inf
+    const A c = (A)a.scale;
+    if (a.lse) static_cast<A *>(a.lse)[r] = empty ? A(-INFINITY) : fma_a(c, m, log_s);
     if (a.entropy) static_cast<A *>(a.entropy)[r] = empty ? A(0) : log_s - LpMath<A>::kUnit * (p.t / p.s);
     if (a.logprob) {
       A lp = A(NAN);
       if (t == -1)
         lp = A(0);
       else if (t >= 0 && t < a.s.D)
-        lp = empty ? A(-INFINITY) : c * (xt - p.m) - log_s;
+        lp = empty ? A(-INFINITY) : c * (xt - m) - log_s;
       static_cast<A *>(a.logprob)[r] = lp;
     }
   }
-  if (TOP && lane < a.k) {
-    const int64_t o = r / a.s.L, l = r - o * a.s.L;
-    const int64_t at = l + a.s.L * (lane + a.k * o);
+  __device__ __forceinline__ void alternative(const LogprobArgs &a, int64_t r, int j, A v, int i) const {
+    const int64_t o = a.s.L == 1 ? r : r / a.s.L, l = r - o * a.s.L;
+    const int64_t at = l + a.s.L * (j + a.k * o);
     const bool none = i == kNone;
     store_index(a.top_index, a.wide_index, at,
                 none ? (a.wide_index ? INT64_MIN : (int64_t)INT32_MIN) : (int64_t)i + (a.one_based ? 1 : 0));
-    static_cast<A *>(a.top_logprob)[at] = none ? A(NAN) : c * (v - p.m) - log_s;
+    static_cast<A *>(a.top_logprob)[at] = none ? A(NAN) : (A)a.scale * (v - m) - log_s;
   }
+};
+
+template <typename A, bool TOP>
+__device__ __forceinline__ void finish_row(const LogprobArgs &a, int64_t r, const Part<A> &p, A v, int i, int64_t t,
+                                           A xt) {
+  const int lane = threadIdx.x & 31;
+  const RowResult<A> res(a, p);
+  if (lane == 0) res.stats(a, r, p, t, xt);
+  if (TOP && lane < a.k) res.alternative(a, r, lane, v, i);
 }
 
 // The token asked for (0-based; -1 none; others outside the row) and its logit.
+__device__ __forceinline__ int64_t asked_token(const LogprobArgs &a, int64_t r) {
+  return a.logprob ? load_index(a.tokens, a.wide_token, r) - (a.one_based ? 1 : 0) : -1;
+}
 template <typename T, typename A>
-__device__ __forceinline__ void asked_token(const LogprobArgs &a, int64_t r, const T *x, int64_t &t, A &xt) {
-  t = -1;
-  xt = A(0);
-  if (a.logprob) {
-    t = load_index(a.tokens, a.wide_token, r) - (a.one_based ? 1 : 0);
-    if (t >= 0 && t < a.s.D) xt = to_acc(x[t * a.x.sd]);
-  }
+__device__ __forceinline__ A asked_logit(const LogprobArgs &a, int64_t t, const T *x) {
+  return t >= 0 && t < a.s.D ? to_acc(x[t * a.x.sd]) : A(0);
 }
 
 // ---------------------------------------------------------------------------
@@ -291,47 +414,70 @@ __device__ __forceinline__ void asked_token(const LogprobArgs &a, int64_t r, con
 template <typename T, int V>
 struct BatchU { static constexpr int value = V == 1 ? 8 : 4; };
 
-// A warp reads batches `from`, `from + step`, ... of the row up to `to`.
-template <typename T, int V, bool TOP, typename State>
-__device__ __forceinline__ void read_batches(const T *x, int64_t sd, int D, int shift, int from, int step, int to,
-                                             typename AccOf<T>::type c, int k, State &st,
-                                             volatile typename AccOf<T>::type *floor) {
-  using A = typename AccOf<T>::type;
-  constexpr int U = BatchU<T, V>::value;
-  const int lane = threadIdx.x & 31;
-  for (int b = from; b < to; b += step) {
-    const int base = b * (U * V * 32) - shift;
-    A xs[U * V];
+// A lane's pieces of batch b, -Inf beyond the row's ends.
+template <typename T, int V, int U>
+__device__ __forceinline__ void load_batch(const T *x, int64_t sd, int D, int shift, int b, Piece<T, V> (&out)[U]) {
+  const int lane = threadIdx.x & 31, base = b * (U * V * 32) - shift;
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_piece<T, A, V>(x, sd, base + (u * 32 + lane) * V, D, A(-INFINITY), xs + u * V);
-    st.batch(xs, base, D, c, k, TOP && floor ? *floor : A(-INFINITY));
-    // any warp's entry k - 1 will do as floor: the value decides how much is
-    // looked at, never the result
-    if (TOP && floor && lane == 0 && st.top.ki != kNone && st.top.kv > *floor) *floor = st.top.kv;
+  for (int u = 0; u < U; ++u) {
+    const int first = base + (u * 32 + lane) * V;
+    if (V == 1) {
+      out[u].set(0, first < D ? x[first * sd] : (T)(-INFINITY));
+    } else if (first >= 0 && first + V <= D) {
+      out[u] = *reinterpret_cast<const Piece<T, V> *>(x + first);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[u].set(j, first + j >= 0 && first + j < D ? x[first + j] : (T)(-INFINITY));
+    }
   }
 }
 
-// One warp a row.
+template <typename T, int V>
+__device__ __forceinline__ int row_batches(int D, int shift) {
+  constexpr int N = BatchU<T, V>::value * V * 32;
+  return (int)(((int64_t)shift + D + N - 1) / N);
+}
+
+// One warp a row.  The next batch, of this row or of the next one, is on its
+// way while one is worked on; so is the next row's token.
 template <typename T, int V, bool TOP>
-__global__ void __launch_bounds__(256) k_logprob_warp(LogprobArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 2 : TOP ? 3 : 4) k_logprob_warp(LogprobArgs a) {
   using A = typename AccOf<T>::type;
   constexpr int U = BatchU<T, V>::value;
+  __shared__ __align__(16) A sh_spread[TOP ? 8 : 1][TOP ? U * V * 32 : 1];
+  A *spread = sh_spread[TOP ? threadIdx.x >> 5 : 0];
   const A c = LpMath<A>::factor(a.scale);
   const int D = (int)a.s.D;
-  const int64_t rows = a.s.rows();
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
-    const T *x = row_ptr<T>(a.x, r, a.s.L);
-    int64_t t;
-    A xt;
-    asked_token<T, A>(a, r, x, t, xt);
-    const int shift = row_shift<T, V>(x);
-    const int batches = (int)(((int64_t)shift + D + U * V * 32 - 1) / (U * V * 32));
-    RowState<A, U, V, TOP> st;
+  const int64_t rows = a.s.rows(), step = (int64_t)gridDim.x * 8;
+  int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const T *x = row_ptr<T>(a.x, r, a.s.L);
+  Piece<T, V> cur[U], next[U];
+  load_batch<T, V, U>(x, a.x.sd, D, row_shift<T, V>(x), 0, cur);
+  int64_t t = asked_token(a, r);
+  while (true) {
+    const bool more = r + step < rows;
+    const T *xn = more ? row_ptr<T>(a.x, r + step, a.s.L) : x;
+    const int64_t tn = more ? asked_token(a, r + step) : -1;
+    const A xt = asked_logit<T, A>(a, t, x);
+    const int shift = row_shift<T, V>(x), batches = row_batches<T, V>(D, shift);
+    RowState<T, U, V, TOP> st;
     st.init();
-    read_batches<T, V, TOP>(x, a.x.sd, D, shift, 0, 1, batches, c, a.k, st,
-                            static_cast<volatile A *>(nullptr));
+    for (int b = 0; b < batches; ++b) {
+      if (b + 1 < batches)
+        load_batch<T, V, U>(x, a.x.sd, D, shift, b + 1, next);
+      else if (more)
+        load_batch<T, V, U>(xn, a.x.sd, D, row_shift<T, V>(xn), 0, next);
+      st.batch(cur, b * (U * V * 32) - shift, D, c, a.k, A(-INFINITY), spread);
+#pragma unroll
+      for (int u = 0; u < U; ++u) cur[u] = next[u];
+    }
     st.p.warp_merge(c);
     finish_row<A, TOP>(a, r, st.p, st.top.v, st.top.i, t, xt);
+    if (!more) return;
+    r += step;
+    x = xn;
+    t = tn;
   }
 }
 
@@ -339,13 +485,14 @@ __global__ void __launch_bounds__(256) k_logprob_warp(LogprobArgs a) {
 // warps' sums and lists are joined in each block, the blocks' in the first one
 // through distributed shared memory, always in the same order.
 template <typename T, int V, bool TOP, int NW>
-__global__ void __launch_bounds__(NW * 32) k_logprob_cta(LogprobArgs a) {
+__global__ void __launch_bounds__(NW * 32, sizeof(T) == 8 ? 2 : TOP ? 3 : 4) k_logprob_cta(LogprobArgs a) {
   using A = typename AccOf<T>::type;
   constexpr int U = BatchU<T, V>::value;
   __shared__ Part<A> sh_p[NW];
   __shared__ A sh_v[NW][32];
   __shared__ int sh_i[NW][32];
   __shared__ A sh_floor;
+  __shared__ __align__(16) A sh_spread[TOP ? NW : 1][TOP ? U * V * 32 : 1];
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -353,17 +500,26 @@ __global__ void __launch_bounds__(NW * 32) k_logprob_cta(LogprobArgs a) {
   const int D = (int)a.s.D;
   const int64_t r = blockIdx.x / C;
   const T *x = row_ptr<T>(a.x, r, a.s.L);
-  int64_t t;
-  A xt;
-  asked_token<T, A>(a, r, x, t, xt);
+  const int shift = row_shift<T, V>(x), batches = row_batches<T, V>(D, shift), step = C * NW;
+  Piece<T, V> cur[U], next[U];
+  int b = rank * NW + warp;
+  if (b < batches) load_batch<T, V, U>(x, a.x.sd, D, shift, b, cur);
+  int64_t t = asked_token(a, r);
   if (threadIdx.x == 0) sh_floor = A(-INFINITY);
   if (TOP) __syncthreads();
-  const int shift = row_shift<T, V>(x);
-  const int batches = (int)(((int64_t)shift + D + U * V * 32 - 1) / (U * V * 32));
-  RowState<A, U, V, TOP> st;
+  RowState<T, U, V, TOP> st;
   st.init();
-  read_batches<T, V, TOP>(x, a.x.sd, D, shift, rank * NW + warp, C * NW, batches, c, a.k, st,
-                          static_cast<volatile A *>(&sh_floor));
+  volatile A *floor = &sh_floor;
+  for (; b < batches; b += step) {
+    if (b + step < batches) load_batch<T, V, U>(x, a.x.sd, D, shift, b + step, next);
+    st.batch(cur, b * (U * V * 32) - shift, D, c, a.k, TOP ? *floor : A(0), sh_spread[TOP ? warp : 0]);
+    // any warp's entry k - 1 will do as floor: the value decides how much is
+    // looked at, never the result
+    if (TOP && lane == 0 && st.top.ki != kNone && st.top.kv > *floor) *floor = st.top.kv;
+#pragma unroll
+    for (int u = 0; u < U; ++u) cur[u] = next[u];
+  }
+  const A xt = asked_logit<T, A>(a, t, x);
   st.p.warp_merge(c);
   if (lane == 0) sh_p[warp] = st.p;
   if (TOP) {
@@ -372,9 +528,8 @@ __global__ void __launch_bounds__(NW * 32) k_logprob_cta(LogprobArgs a) {
   }
   __syncthreads();
   // lists: halve the number of warps until one is left
-  if (TOP) {
-#pragma unroll
-    for (int n = NW / 2; n; n >>= 1) {
+  auto join_lists = [&](int n) {
+    for (n >>= 1; n; n >>= 1) {
       if (warp < n) {
         st.top.merge_reversed(sh_v[warp + n][31 - lane], sh_i[warp + n][31 - lane]);
         sh_v[warp][lane] = st.top.v;
@@ -382,7 +537,8 @@ __global__ void __launch_bounds__(NW * 32) k_logprob_cta(LogprobArgs a) {
       }
       __syncthreads();
     }
-  }
+  };
+  if (TOP) join_lists(NW);
   if (warp == 0) {
     st.p.init();
     if (lane < NW) st.p = sh_p[lane];
@@ -391,14 +547,26 @@ __global__ void __launch_bounds__(NW * 32) k_logprob_cta(LogprobArgs a) {
   }
   if (C > 1) {
     cluster.sync();
-    if (rank == 0 && warp == 0) {
-      st.p.init();
-      if (lane < C) st.p = cluster.map_shared_rank(sh_p, lane)[0];
-      st.p.warp_merge(c);
-      if (TOP)
-        for (int q = 1; q < C; ++q)
-          st.top.merge_reversed(cluster.map_shared_rank(&sh_v[0][0], q)[31 - lane],
-                                cluster.map_shared_rank(&sh_i[0][0], q)[31 - lane]);
+    if (rank == 0) {
+      // a warp fetches a block's list
+      A v = A(-INFINITY);
+      int i = kNone;
+      if (TOP && warp < C) {
+        v = cluster.map_shared_rank(&sh_v[0][0], warp)[lane];
+        i = cluster.map_shared_rank(&sh_i[0][0], warp)[lane];
+      }
+      if (warp == 0) {
+        st.p.init();
+        if (lane < C) st.p = cluster.map_shared_rank(sh_p, lane)[0];
+        st.p.warp_merge(c);
+      }
+      if (TOP) {
+        __syncthreads();
+        st.top.v = sh_v[warp][lane] = v;
+        st.top.i = sh_i[warp][lane] = i;
+        __syncthreads();
+        join_lists(NW);
+      }
     }
     cluster.sync();  // no block leaves while its shared memory is read
   }
@@ -409,166 +577,256 @@ __global__ void __launch_bounds__(NW * 32) k_logprob_cta(LogprobArgs a) {
 // rows across the lanes
 // ---------------------------------------------------------------------------
 // Column-major logits [tokens, vocabulary]: a row's logits are `sd` apart,
-// neighbouring rows lie side by side.  A block takes LT neighbouring rows
-// (lanes), reads S steps of them along the lanes (full 128-byte lines), turns
-// the tile round in shared memory and has each warp read its four rows along
-// the steps, as the kernels above do.  A word holds PAIR steps of one lane.
-template <typename T>
-struct LaneTile {  // float32, float64
-  static constexpr int LT = 32, NW = 8, PAIR = 1, W = sizeof(T) == 4 ? 128 : 64;
-  using Word = T;
-};
-template <>
-struct LaneTile<__half> {  // lane pairs are read as one word
-  static constexpr int LT = 64, NW = 16, PAIR = 2, W = 128;
-  using Word = uint32_t;
+// neighbouring rows lie side by side.  A thread keeps the sums of V neighbouring
+// rows and walks along the steps: a warp reads 32 * V neighbouring logits at a
+// time and nothing is exchanged but at the end.
+//   m is a reference here, not the maximum: sums are scaled anew only when a
+// logit is 8 bits above it, which after the first steps it hardly ever is.
+//   For the alternatives a thread also leaves the largest logit of each segment
+// of its steps (1/seg of the bytes that it reads).  k_logprob_join, a warp a
+// row, has each lane take the largest of its share of the row's segment maxima;
+// the k-th largest of these is a floor that k logits reach, so the k best lie in
+// the segments whose maximum reaches it.  It reads those few segments again.
+//   (Lists kept while reading cost far more: with tiles turned round in shared
+// memory 65536 x 4096 float32 took 462 us with five alternatives, with
+// candidates gathered by atomics 643 us.)
+template <typename A, int V>
+struct LaneShape {
+  static constexpr int UN = (sizeof(A) == 8 ? 8 : 16) / V;  // steps a thread and tile
+  static constexpr int ROWS = 32 * V, STEPS = 8 * UN;
 };
 
 struct LaneArgs {
   LogprobArgs a;
-  int64_t lblocks;  // blocks of LT lanes
-  int chunk;        // steps a block of the cluster takes, a multiple of the tile's
-  bool pairs;       // float16: lane pairs are 4-byte aligned in every step
+  int64_t lblocks;  // blocks of 32 * V rows
+  int chunk;        // steps a block takes, a multiple of a segment's tiles
+  int chunks;       // blocks a row
+  void *parts;      // [chunk][row], null: the block writes the results
+  void *segs;       // [tile group][warp][row]: maxima of `group` tiles' steps of a thread
+  int nsegs;        // segments a row
+  int group;        // tiles a segment
+  int un_log2, group_log2, len_log2;  // steps a thread and tile, tiles and logits a segment
 };
+constexpr int kSegList = 128;  // segments of a row that are looked into one by one
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(LaneTile<T>::NW * 32, LaneTile<T>::NW == 16 ? 2 : 3) k_logprob_lanes(LaneArgs la) {
+template <typename T, int V, bool TOP>
+__global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
   using A = typename AccOf<T>::type;
-  using Tile = LaneTile<T>;
-  using Word = typename Tile::Word;
-  constexpr int LT = Tile::LT, NW = Tile::NW, PAIR = Tile::PAIR, W = Tile::W, S = W * PAIR;
-  constexpr int ITER = W / NW, R = LT / NW, U = W / 32;
-  static_assert(R == 4, "four rows a warp");
-  constexpr size_t kTile = sizeof(Word) * LT * (W + 1);
-  constexpr size_t kJoin = (sizeof(Part<A>) + 32 * (sizeof(A) + sizeof(int))) * LT;
-  __shared__ __align__(16) unsigned char raw[kTile > kJoin ? kTile : kJoin];
-  Word(*tile)[W + 1] = reinterpret_cast<Word(*)[W + 1]>(raw);
+  using S = LaneShape<A, V>;
+  constexpr int UN = S::UN, ROWS = S::ROWS, STEPS = S::STEPS;
+  __shared__ Part<A> parts[8][ROWS];
   const LogprobArgs &a = la.a;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t group = blockIdx.x / C, o = group / la.lblocks, l0 = (group - o * la.lblocks) * LT;
-  const int64_t L = a.s.L, sd = a.x.sd;
+  const int64_t blk = blockIdx.x / la.chunks, o = blk / la.lblocks, l0 = (blk - o * la.lblocks) * ROWS;
+  const int chunk = (int)(blockIdx.x - blk * la.chunks);
+  const int64_t L = a.s.L, sd = a.x.sd, l = l0 + lane * V;
+  const bool active = l < L;  // V divides L
   const int D = (int)a.s.D;
-  const T *x = static_cast<const T *>(a.x.p) + o * a.x.so + l0;
-  const int left = L - l0 < LT ? (int)(L - l0) : LT;  // lanes of this block
+  const T *x = static_cast<const T *>(a.x.p) + o * a.x.so + (active ? l : 0);
   const A c = LpMath<A>::factor(a.scale);
-  const int s0 = rank * la.chunk, s1 = D < s0 + la.chunk ? D : s0 + la.chunk;
-  // row q of the tile is lane q (float16: even lanes, then odd ones)
-  auto lane_of = [](int q) { return PAIR == 1 ? q : (q < 32 ? 2 * q : 2 * (q - 32) + 1); };
-  // the tokens asked for: lane q of a warp holds its row q's
-  int64_t tok = -1;
-  A tok_x = A(0);
-  if (lane < R && lane_of(warp * R + lane) < left)
-    asked_token<T, A>(a, o * L + l0 + lane_of(warp * R + lane), x + lane_of(warp * R + lane), tok, tok_x);
-
-  Word reg[ITER * PAIR];
-  auto load = [&](int s) {
+  const int s0 = chunk * la.chunk, s1 = D - s0 < la.chunk ? D : s0 + la.chunk;
+  Piece<T, V> cur[UN], next[UN];
+  auto load = [&](int s, Piece<T, V> (&out)[UN]) {
+    if (active && s + STEPS <= s1) {
+      const T *p = x + (int64_t)(s + warp) * sd;
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      const int step = s + (i * NW + warp) * PAIR;
-      if constexpr (PAIR == 1) {
-        reg[i] = lane < left && step < s1 ? x[step * sd + lane] : (T)(-INFINITY);
-      } else {
+      for (int u = 0; u < UN; ++u, p += 8 * sd) out[u] = *reinterpret_cast<const Piece<T, V> *>(p);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t w = 0xFC00FC00u;  // -Inf, -Inf
-          if (step + j < s1) {
-            const T *p = x + (step + j) * sd + 2 * lane;
-            if (la.pairs && 2 * lane + 1 < left)
-              w = *reinterpret_cast<const uint32_t *>(p);
-            else {
-              const unsigned short *h = reinterpret_cast<const unsigned short *>(p);
-              if (2 * lane < left) w = (w & 0xFFFF0000u) | h[0];
-              if (2 * lane + 1 < left) w = (w & 0xFFFFu) | ((uint32_t)h[1] << 16);
-            }
-          }
-          reg[2 * i + j] = w;
+      for (int u = 0; u < UN; ++u) {
+        const int step = s + u * 8 + warp;
+        if (active && step < s1) {
+          out[u] = *reinterpret_cast<const Piece<T, V> *>(x + step * sd);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) out[u].set(j, (T)(-INFINITY));
         }
       }
     }
   };
-
-  RowState<A, U, PAIR, TOP> st[R];
+  Part<A> p[V];
+  A limit[V], sm[V];  // scale anew above `limit`; the segment's maximum
 #pragma unroll
-  for (int q = 0; q < R; ++q) st[q].init();
-  if (s0 < s1) load(s0);
-  for (int s = s0; s < s1; s += S) {
-    __syncthreads();  // the tile before has been read
+  for (int j = 0; j < V; ++j) {
+    p[j].init();
+    limit[j] = LpMath<A>::lowest();
+    sm[j] = A(-INFINITY);
+  }
+  int tiles = 0;  // of the segment
+  A *seg = static_cast<A *>(la.segs);
+  if (TOP) seg += ((int64_t)(s0 / (STEPS * la.group)) * 8 + warp) * a.s.rows() + o * L + l;
+  if (s0 < s1) load(s0, cur);
+  for (int s = s0; s < s1; s += STEPS) {
+    if (s + STEPS < s1) load(s + STEPS, next);
+    A f[UN][V];
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      if constexpr (PAIR == 1) {
-        tile[lane][i * NW + warp] = reg[i];
-      } else {
-        tile[lane][i * NW + warp] = __byte_perm(reg[2 * i], reg[2 * i + 1], 0x5410);
-        tile[32 + lane][i * NW + warp] = __byte_perm(reg[2 * i], reg[2 * i + 1], 0x7632);
-      }
+    for (int u = 0; u < UN; ++u) cur[u].widen(f[u]);
+    bool grown = false;
+    A bm[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      bm[j] = LpMath<A>::max2(f[0][j], A(-INFINITY));
+#pragma unroll
+      for (int u = 1; u < UN; ++u) bm[j] = LpMath<A>::max2(bm[j], f[u][j]);
+      grown |= bm[j] > limit[j];
+      if (TOP) sm[j] = LpMath<A>::max2(sm[j], bm[j]);
     }
-    __syncthreads();
-    if (s + S < s1) load(s + S);  // in flight while this tile is worked on
+    if (__any_sync(~0u, grown)) {
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      A xs[U * PAIR];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Word w = tile[warp * R + q][u * 32 + lane];
-        if constexpr (PAIR == 1) {
-          xs[u] = w;
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-          xs[2 * u] = f.x;
-          xs[2 * u + 1] = f.y;
+      for (int j = 0; j < V; ++j)
+        if (bm[j] > limit[j]) {
+          p[j].rescale(bm[j], c);
+          limit[j] = bm[j] + A(8) / c;
         }
-      }
-      st[q].batch(xs, s, D, c, a.k, A(-INFINITY));
     }
+    if constexpr (std::is_same<A, float>::value && V % 2 == 0) {
+      const uint64_t cc = pack2(c, c);
+#pragma unroll
+      for (int j = 0; j < V; j += 2) {
+        const uint64_t nm = pack2(-p[j].m, -p[j + 1].m);
+        uint64_t s2 = pack2(p[j].s, p[j + 1].s), t2 = pack2(p[j].t, p[j + 1].t);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          float z0, z1;
+          unpack2(mul2(add2(pack2(f[u][j], f[u][j + 1]), nm), cc), z0, z1);
+          z0 = LpMath<A>::floor_z(z0);
+          z1 = LpMath<A>::floor_z(z1);
+          const uint64_t e = pack2(LpMath<A>::ex(z0), LpMath<A>::ex(z1));
+          s2 = add2(s2, e);
+          t2 = fma2(e, pack2(z0, z1), t2);
+        }
+        unpack2(s2, p[j].s, p[j + 1].s);
+        unpack2(t2, p[j].t, p[j + 1].t);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        A col[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) col[u] = f[u][j];
+        p[j].sum(col, c);
+      }
+    }
+    if (TOP && (++tiles == la.group || s + STEPS >= s1)) {
+      tiles = 0;
+      Vec<A, V> w;
+#pragma unroll
+      for (int j = 0; j < V; ++j) w.v[j] = sm[j];
+      if (active) *reinterpret_cast<Vec<A, V> *>(seg) = w;
+      seg += 8 * a.s.rows();
+#pragma unroll
+      for (int j = 0; j < V; ++j) sm[j] = A(-INFINITY);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) cur[u] = next[u];
   }
 #pragma unroll
-  for (int q = 0; q < R; ++q) st[q].p.warp_merge(c);
-
-  if (C == 1) {
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const int l = lane_of(warp * R + q);
-      const int64_t t = __shfl_sync(~0u, tok, q);
-      const A xt = __shfl_sync(~0u, tok_x, q);
-      if (l < left) finish_row<A, TOP>(a, o * L + l0 + l, st[q].p, st[q].top.v, st[q].top.i, t, xt);
-    }
+  for (int j = 0; j < V; ++j) parts[warp][lane * V + j] = p[j];
+  __syncthreads();
+  const int row = threadIdx.x;
+  if (row >= ROWS || l0 + row >= L) return;
+  Part<A> q = parts[0][row];
+  for (int w = 1; w < 8; ++w) q.merge(parts[w][row], c);
+  const int64_t r = o * L + l0 + row;
+  if (la.parts) {
+    static_cast<Part<A> *>(la.parts)[chunk * a.s.rows() + r] = q;
     return;
   }
-  // the blocks' sums and lists: row q of the tile is joined by block q / (LT / C)
-  A *jv = reinterpret_cast<A *>(raw);                       // [LT][32]
-  Part<A> *jp = reinterpret_cast<Part<A> *>(jv + LT * 32);  // [LT]
-  int *ji = reinterpret_cast<int *>(jp + LT);               // [LT][32]
-  __syncthreads();
+  const int64_t t = asked_token(a, r);
+  RowResult<A>(a, q).stats(a, r, q, t, asked_logit<T, A>(a, t, static_cast<const T *>(a.x.p) + o * a.x.so + l0 + row));
+}
+
+// A warp a row: joins the parts of blocks and finds the alternatives.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(256) k_logprob_join(LaneArgs la) {
+  using A = typename AccOf<T>::type;
+  constexpr int U = 8;
+  __shared__ int sh_list[TOP ? 8 : 1][TOP ? kSegList : 1];
+  const LogprobArgs &a = la.a;
+  const int lane = threadIdx.x & 31, k = a.k;
+  const int64_t rows = a.s.rows(), r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const T *x = row_ptr<T>(a.x, r, a.s.L);
+  const int64_t t = asked_token(a, r);
+  const A c = LpMath<A>::factor(a.scale);
+  Part<A> p;
+  p.init();
+  for (int q = lane; q < la.chunks; q += 32) p.merge(static_cast<const Part<A> *>(la.parts)[q * rows + r], c);
+  p.warp_merge(c);
+  const A xt = asked_logit<T, A>(a, t, x);
+  TopList<A> top;
+  top.init();
+  if constexpr (TOP) {
+    const A *segs = static_cast<const A *>(la.segs) + r;
+    const int n = la.nsegs, D = (int)a.s.D;
+    int *list = sh_list[threadIdx.x >> 5];
+    A kept[U], lm = A(-INFINITY);  // the first segments' maxima, and the largest of this lane's
 #pragma unroll
-  for (int q = 0; q < R; ++q) {
-    const int row = warp * R + q;
-    if (lane == 0) jp[row] = st[q].p;
-    if (TOP) {
-      jv[row * 32 + lane] = st[q].top.v;
-      ji[row * 32 + lane] = st[q].top.i;
+    for (int u = 0; u < U; ++u) kept[u] = u * 32 + lane < n ? segs[(int64_t)(u * 32 + lane) * rows] : A(NAN);
+#pragma unroll
+    for (int u = 0; u < U; ++u) lm = LpMath<A>::max2(lm, kept[u]);
+    for (int g = U * 32 + lane; g < n; g += 32) lm = LpMath<A>::max2(lm, segs[(int64_t)g * rows]);
+    const A floor = kth_of_lanes(lm, k);  // k segments, so k logits, are at least this large
+    // the segments that reach the floor; with `above` those over it
+    auto gather = [&](bool above) {
+      int count = 0;
+      auto add = [&](int g, A v) {
+        const bool in = above ? v > floor : v >= floor;
+        const unsigned mask = __ballot_sync(~0u, in);
+        const int at = count + __popc(mask & ((1u << lane) - 1));
+        if (in && at < kSegList) list[at] = g;
+        count += __popc(mask);
+      };
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(u * 32 + lane, kept[u]);
+      for (int b = U * 32; b < n; b += 32) add(b + lane, b + lane < n ? segs[(int64_t)(b + lane) * rows] : A(NAN));
+      __syncwarp();
+      return count;
+    };
+    // logit e of segment g: tile g / 8 of groups, step within it
+    auto look = [&](int to, bool above) {
+      constexpr int M = 4;  // batches in flight
+      for (int e = 0; e < to; e += 32 * M) {
+        A v[M];
+        int step[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const int at = e + m * 32 + lane;
+          step[m] = D;
+          if (at < to) {
+            const int g = list[at >> la.len_log2], i = at & ((1 << la.len_log2) - 1);
+            step[m] = ((((g >> 3) << la.group_log2) + (i >> la.un_log2)) << (la.un_log2 + 3)) +
+                      ((i & ((1 << la.un_log2) - 1)) << 3) + (g & 7);
+          }
+          v[m] = step[m] < D ? to_acc(x[step[m] * a.x.sd]) : A(NAN);
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m) top.offer(v[m], step[m], above ? v[m] > floor : v[m] >= floor, floor, k);
+      }
+    };
+    int count = gather(false);
+    if (count <= kSegList && floor > A(-INFINITY)) {
+      look(count << la.len_log2, false);
+    } else {
+      // Many logits equal to the floor: those over it from their segments (less
+      // than k lanes have one), the others from the row's beginning, where
+      // enough of them are soon found.
+      count = gather(true);
+      if (count <= kSegList) {
+        look(count << la.len_log2, true);
+      } else {
+        for (int s = 0; s < D; s += 32) {
+          const A v = s + lane < D ? to_acc(x[(s + lane) * a.x.sd]) : A(NAN);
+          top.offer(v, s + lane, v > floor, floor, k);
+        }
+      }
+      for (int s = 0; s < D && top.ki == kNone; s += 32) {
+        const A v = s + lane < D ? to_acc(x[(s + lane) * a.x.sd]) : A(NAN);
+        top.offer(v, s + lane, v == floor, floor, k);
+      }
     }
   }
-  cluster.sync();
-  const int per = LT / C;
-  for (int row = rank * per + warp; row < (rank + 1) * per; row += NW) {
-    const int l = lane_of(row);
-    if (l >= left) continue;
-    RowState<A, U, PAIR, TOP> z;
-    z.init();
-    if (lane < C) z.p = cluster.map_shared_rank(jp, lane)[row];
-    z.p.warp_merge(c);
-    if (TOP)
-      for (int q = 0; q < C; ++q)
-        z.top.merge_reversed(cluster.map_shared_rank(jv, q)[row * 32 + 31 - lane],
-                             cluster.map_shared_rank(ji, q)[row * 32 + 31 - lane]);
-    int64_t t;
-    A xt;
-    asked_token<T, A>(a, o * L + l0 + l, x + l, t, xt);
-    finish_row<A, TOP>(a, o * L + l0 + l, z.p, z.top.v, z.top.i, t, xt);
-  }
-  cluster.sync();  // no block leaves while its shared memory is read
+  finish_row<A, TOP>(a, r, p, top.v, top.i, t, xt);
 }
 
 struct LogprobGradArgs {
@@ -754,20 +1012,57 @@ static acd_status launch_clusters(K kernel, const Args &a, int64_t blocks, int t
   return ACD_OK;
 }
 
-template <typename T, bool TOP>
+template <typename T, int V, bool TOP>
 static acd_status launch_lanes(acd_ctx *ctx, const LogprobArgs &a, cudaStream_t s) {
-  using Tile = LaneTile<T>;
-  constexpr int S = Tile::W * Tile::PAIR;
+  using A = typename AccOf<T>::type;
+  using S = LaneShape<A, V>;
   LaneArgs la{};
   la.a = a;
-  la.lblocks = (a.s.L + Tile::LT - 1) / Tile::LT;
-  const int64_t groups = la.lblocks * a.s.O, tiles = (a.s.D + S - 1) / S;
-  int C = 1;
-  while (C < 8 && groups * C < ctx->sm_count && tiles >= C * 2) C *= 2;
-  la.chunk = (int)((tiles + C - 1) / C * S);
-  la.pairs = sizeof(T) == 2 && aligned_to<char>(a.x.p, 4) && a.x.sd % 2 == 0 && a.x.so % 2 == 0;
-  if (groups * C > INT32_MAX) return fail(ACD_ERR_UNSUPPORTED, "acd_token_logprob: too many rows");
-  return launch_clusters(k_logprob_lanes<T, TOP>, la, groups * C, Tile::NW * 32, C, s);
+  la.lblocks = (a.s.L + S::ROWS - 1) / S::ROWS;
+  const int64_t blocks = la.lblocks * a.s.O, tiles = (a.s.D + S::STEPS - 1) / S::STEPS;
+  la.group = 1;
+  while (1 << la.un_log2 < S::UN) ++la.un_log2;
+  if (TOP)  // segments written and read, against k of them read again in 32-byte sectors
+    while (4 * la.group * S::UN * la.group * S::UN * a.k < a.s.D) {
+      la.group *= 2;
+      ++la.group_log2;
+    }
+  la.len_log2 = la.un_log2 + la.group_log2;
+  // rows are divided while there is room for blocks, eight tiles each at least
+  int64_t chunks = (int64_t)ctx->sm_count * 3 / blocks;
+  if (chunks > tiles / 8) chunks = tiles / 8;
+  if (chunks < 1) chunks = 1;
+  const int64_t groups = (tiles + la.group - 1) / la.group, per = (groups + chunks - 1) / chunks;
+  la.chunk = (int)(per * la.group * S::STEPS);
+  la.chunks = (int)((groups + per - 1) / per);
+  la.nsegs = (int)(groups * 8);
+  if (blocks * la.chunks > INT32_MAX) return fail(ACD_ERR_UNSUPPORTED, "acd_token_logprob: too many rows");
+  const bool join = TOP || la.chunks > 1;
+  if (join) {
+    const size_t np = (size_t)la.chunks * a.s.rows(), ns = TOP ? (size_t)la.nsegs * a.s.rows() : 0;
+    void *scratch;
+    ACD_TRY(get_scratch(ctx, ns * sizeof(A) + np * sizeof(Part<A>), s, &scratch));
+    la.segs = scratch;  // 16-byte pieces: rows are a multiple of V
+    la.parts = static_cast<A *>(scratch) + ns;
+  }
+  k_logprob_lanes<T, V, TOP><<<(unsigned)(blocks * la.chunks), 256, 0, s>>>(la);
+  if (join) k_logprob_join<T, TOP><<<(unsigned)((a.s.rows() + 7) / 8), 256, 0, s>>>(la);
+  return ACD_OK;
+}
+
+// Rows a thread: as many as a 16-byte (float16: 8-byte) load holds, if they are
+// aligned alike in every step and there are rows for more than half a warp.
+template <typename T, bool TOP>
+static acd_status launch_lanes_any(acd_ctx *ctx, const LogprobArgs &a, cudaStream_t s) {
+  auto fits = [&](int v) {
+    return a.s.L % v == 0 && a.s.L > 16 * v && aligned_to<char>(a.x.p, v * (int)sizeof(T)) && a.x.sd % v == 0 &&
+           a.x.so % v == 0;
+  };
+  if constexpr (sizeof(T) < 8) {
+    if (fits(4)) return launch_lanes<T, 4, TOP>(ctx, a, s);
+  }
+  if (fits(2)) return launch_lanes<T, 2, TOP>(ctx, a, s);
+  return launch_lanes<T, 1, TOP>(ctx, a, s);
 }
 
 template <typename T, int V, bool TOP>
@@ -791,7 +1086,7 @@ static acd_status launch_logprob(acd_ctx *ctx, const LogprobArgs &a, cudaStream_
   constexpr int V = 16 / sizeof(T);
   // eight lanes fill a 32-byte sector of float32 (half of one of float16)
   if (a.x.sd != 1 && a.x.sl == 1 && a.s.L >= 8)
-    return a.k ? launch_lanes<T, true>(ctx, a, s) : launch_lanes<T, false>(ctx, a, s);
+    return a.k ? launch_lanes_any<T, true>(ctx, a, s) : launch_lanes_any<T, false>(ctx, a, s);
   if (a.x.sd == 1) return a.k ? launch_rows<T, V, true>(ctx, a, s) : launch_rows<T, V, false>(ctx, a, s);
   return a.k ? launch_rows<T, 1, true>(ctx, a, s) : launch_rows<T, 1, false>(ctx, a, s);
 }

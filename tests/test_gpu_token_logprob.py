@@ -144,6 +144,29 @@ def test_masks_ties_and_odd_values(acd, dtype, axis, V):
     check_grad(acd, xs, dtype, axis, tokens[keep], 1.0)
 
 
+@pytest.mark.parametrize("dtype", ["float", "float16"])
+@pytest.mark.parametrize("axis", [1, 2])
+@pytest.mark.parametrize("V", [700, 5000, 40000])
+def test_ties_of_coarse_logits(acd, dtype, axis, V):
+    """Logits of few values: the alternatives hold a few above many equal ones,
+    of which the first count, wherever they stand."""
+    rng = np.random.default_rng(11)
+    x = np.rint(rng.standard_normal((40, V)) * 1.3).astype(NP[dtype])
+    x[0] = 0
+    x[1] = -np.inf
+    x[1, ::7] = 1
+    x[2, V // 2:] = 9
+    x[3, -3:] = 50
+    x[4] = np.arange(V) % 5
+    x[5] = np.minimum(np.arange(V), 2000) if dtype == "float" else np.minimum(np.arange(V) // 4, 500)
+    x[6] = x[5, ::-1]
+    if axis == 1:
+        x = np.asfortranarray(x.T)
+    tokens = make_tokens(rng, 40, V)
+    for top in (1, 7, 20, 32):
+        check_forward(acd, x, dtype, axis, tokens, 1.0, top)
+
+
 def test_nan_row_has_nan_gradient_and_leaves_its_neighbours(acd):
     x = np.random.default_rng(0).standard_normal((100, 3)).astype(np.float32)
     x[7, 1] = np.nan
