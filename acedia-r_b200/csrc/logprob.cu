@@ -55,6 +55,7 @@ struct LpMath<float> {
   }
   static __device__ __forceinline__ float lowest() { return -FLT_MAX; }
   static __device__ __forceinline__ float max2(float a, float b) { return fmaxf(a, b); }
+  static __device__ __forceinline__ float min2(float a, float b) { return fminf(a, b); }
 };
 // Two float32 values in one register pair: one instruction for both.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -89,6 +90,7 @@ struct LpMath<double> {
   static __device__ __forceinline__ double floor_z(double z) { return z < -1000.0 ? -1000.0 : z; }  // e^-1000 = 0
   static __device__ __forceinline__ double lowest() { return -DBL_MAX; }
   static __device__ __forceinline__ double max2(double a, double b) { return fmax(a, b); }
+  static __device__ __forceinline__ double min2(double a, double b) { return fmin(a, b); }
 };
 
 // V neighbouring logits as they lie in memory; float16 pairs as words, so that
@@ -582,14 +584,16 @@ __global__ void __launch_bounds__(NW * 32, sizeof(T) == 8 ? 2 : TOP ? 3 : 4) k_l
 // time and nothing is exchanged but at the end.
 //   m is a reference here, not the maximum: sums are scaled anew only when a
 // logit is 8 bits above it, which after the first steps it hardly ever is.
-//   For the alternatives a thread also leaves the largest logit of each segment
-// of its steps (1/seg of the bytes that it reads).  k_logprob_join, a warp a
-// row, has each lane take the largest of its share of the row's segment maxima;
-// the k-th largest of these is a floor that k logits reach, so the k best lie in
-// the segments whose maximum reaches it.  It reads those few segments again.
-//   (Lists kept while reading cost far more: with tiles turned round in shared
-// memory 65536 x 4096 float32 took 462 us with five alternatives, with
-// candidates gathered by atomics 643 us.)
+//   For the alternatives a thread also leaves the two largest logits of each
+// segment of its steps, and where the largest is (9 bytes a segment).  k
+// segments' largest logits set a bound that the k best logits reach, so each of
+// these is the largest of its segment, or stands in a segment whose second
+// largest reaches the bound too: of those, a few in a hundred, all logits are
+// read again.
+//   (Lists kept while reading cost far more: 65536 x 4096 float32 with five
+// alternatives took 462 us with tiles turned round in shared memory, 643 us with
+// candidates gathered by atomics; reading the best segments again without
+// knowing where in them took 336 us.)
 template <typename A, int V>
 struct LaneShape {
   static constexpr int UN = (sizeof(A) == 8 ? 8 : 16) / V;  // steps a thread and tile
@@ -602,7 +606,9 @@ struct LaneArgs {
   int chunk;        // steps a block takes, a multiple of a segment's tiles
   int chunks;       // blocks a row
   void *parts;      // [chunk][row], null: the block writes the results
-  void *segs;       // [tile group][warp][row]: maxima of `group` tiles' steps of a thread
+  void *segs;       // [tile group][warp][row]: largest logit of `group` tiles' steps of a thread,
+  void *seconds;    //   the next largest (or the same again),
+  uint8_t *places;  //   and which of the segment's logits the largest is (the first such)
   int nsegs;        // segments a row
   int group;        // tiles a segment
   int un_log2, group_log2, len_log2;  // steps a thread and tile, tiles and logits a segment
@@ -645,16 +651,17 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
     }
   };
   Part<A> p[V];
-  A limit[V], sm[V];  // scale anew above `limit`; the segment's maximum
+  A limit[V], s1st[V], s2nd[V];  // scale anew above `limit`; the segment's two largest
+  int place[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     p[j].init();
     limit[j] = LpMath<A>::lowest();
-    sm[j] = A(-INFINITY);
+    s1st[j] = s2nd[j] = A(-INFINITY);
+    place[j] = 0;
   }
-  int tiles = 0;  // of the segment
-  A *seg = static_cast<A *>(la.segs);
-  if (TOP) seg += ((int64_t)(s0 / (STEPS * la.group)) * 8 + warp) * a.s.rows() + o * L + l;
+  int at = 0;  // logits of the segment so far
+  int64_t seg = ((int64_t)(s0 / (STEPS * la.group)) * 8 + warp) * a.s.rows() + o * L + l;
   if (s0 < s1) load(s0, cur);
   for (int s = s0; s < s1; s += STEPS) {
     if (s + STEPS < s1) load(s + STEPS, next);
@@ -669,7 +676,17 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
 #pragma unroll
       for (int u = 1; u < UN; ++u) bm[j] = LpMath<A>::max2(bm[j], f[u][j]);
       grown |= bm[j] > limit[j];
-      if (TOP) sm[j] = LpMath<A>::max2(sm[j], bm[j]);
+    }
+    if (TOP) {
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          place[j] = f[u][j] > s1st[j] ? at + u : place[j];
+          s2nd[j] = LpMath<A>::max2(s2nd[j], LpMath<A>::min2(f[u][j], s1st[j]));
+          s1st[j] = LpMath<A>::max2(s1st[j], f[u][j]);
+        }
+      at += UN;
     }
     if (__any_sync(~0u, grown)) {
 #pragma unroll
@@ -707,15 +724,24 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
         p[j].sum(col, c);
       }
     }
-    if (TOP && (++tiles == la.group || s + STEPS >= s1)) {
-      tiles = 0;
-      Vec<A, V> w;
+    if (TOP && (at == 1 << la.len_log2 || s + STEPS >= s1)) {
+      Vec<A, V> w1, w2;
+      Vec<uint8_t, V> wp;
 #pragma unroll
-      for (int j = 0; j < V; ++j) w.v[j] = sm[j];
-      if (active) *reinterpret_cast<Vec<A, V> *>(seg) = w;
+      for (int j = 0; j < V; ++j) {
+        w1.v[j] = s1st[j];
+        w2.v[j] = s2nd[j];
+        wp.v[j] = (uint8_t)place[j];
+        s1st[j] = s2nd[j] = A(-INFINITY);
+        place[j] = 0;
+      }
+      at = 0;
+      if (active) {
+        *reinterpret_cast<Vec<A, V> *>(static_cast<A *>(la.segs) + seg) = w1;
+        *reinterpret_cast<Vec<A, V> *>(static_cast<A *>(la.seconds) + seg) = w2;
+        *reinterpret_cast<Vec<uint8_t, V> *>(la.places + seg) = wp;
+      }
       seg += 8 * a.s.rows();
-#pragma unroll
-      for (int j = 0; j < V; ++j) sm[j] = A(-INFINITY);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) cur[u] = next[u];
@@ -736,14 +762,117 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
   RowResult<A>(a, q).stats(a, r, q, t, asked_logit<T, A>(a, t, static_cast<const T *>(a.x.p) + o * a.x.so + l0 + row));
 }
 
-// A warp a row: joins the parts of blocks and finds the alternatives.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(256) k_logprob_join(LaneArgs la) {
+// Where logit i of segment g lies in the row: tile g / 8 of groups, step within it.
+__device__ __forceinline__ int segment_step(const LaneArgs &la, int g, int i) {
+  return ((((g >> 3) << la.group_log2) + (i >> la.un_log2)) << (la.un_log2 + 3)) +
+         ((i & ((1 << la.un_log2) - 1)) << 3) + (g & 7);
+}
+
+// The k best logits of row r, found by a warp.
+template <typename T>
+__device__ __forceinline__ TopList<typename AccOf<T>::type> row_alternatives(const LaneArgs &la, int64_t r, int *list) {
   using A = typename AccOf<T>::type;
   constexpr int U = 8;
-  __shared__ int sh_list[TOP ? 8 : 1][TOP ? kSegList : 1];
   const LogprobArgs &a = la.a;
   const int lane = threadIdx.x & 31, k = a.k;
+  const int64_t rows = a.s.rows();
+  const T *x = row_ptr<T>(a.x, r, a.s.L);
+  TopList<A> top;
+  top.init();
+  const A *segs = static_cast<const A *>(la.segs) + r;
+  const int n = la.nsegs, D = (int)a.s.D;
+  A kept[U], lm = A(-INFINITY);  // the first segments' maxima, and the largest of this lane's
+#pragma unroll
+  for (int u = 0; u < U; ++u) kept[u] = u * 32 + lane < n ? segs[(int64_t)(u * 32 + lane) * rows] : A(NAN);
+#pragma unroll
+  for (int u = 0; u < U; ++u) lm = LpMath<A>::max2(lm, kept[u]);
+  for (int g = U * 32 + lane; g < n; g += 32) lm = LpMath<A>::max2(lm, segs[(int64_t)g * rows]);
+  const A floor = kth_of_lanes(lm, k);  // k segments, so k logits, are at least this large
+  // the segments that reach the floor; with `above` those over it
+  auto gather = [&](bool above) {
+    int count = 0;
+    auto add = [&](int g, A v) {
+      const bool in = above ? v > floor : v >= floor;
+      const unsigned mask = __ballot_sync(~0u, in);
+      const int at = count + __popc(mask & ((1u << lane) - 1));
+      if (in && at < kSegList) list[at] = g;
+      count += __popc(mask);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(u * 32 + lane, kept[u]);
+    for (int b = U * 32; b < n; b += 32) add(b + lane, b + lane < n ? segs[(int64_t)(b + lane) * rows] : A(NAN));
+    __syncwarp();
+    return count;
+  };
+  auto look = [&](int to, bool above) {
+    constexpr int M = 4;  // batches in flight
+    for (int e = 0; e < to; e += 32 * M) {
+      A v[M];
+      int step[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const int at = e + m * 32 + lane;
+        step[m] = D;
+        if (at < to) {
+          const int g = list[at >> la.len_log2], i = at & ((1 << la.len_log2) - 1);
+          step[m] = segment_step(la, g, i);
+        }
+        v[m] = step[m] < D ? to_acc(x[step[m] * a.x.sd]) : A(NAN);
+      }
+#pragma unroll
+      for (int m = 0; m < M; ++m) top.offer(v[m], step[m], above ? v[m] > floor : v[m] >= floor, floor, k);
+    }
+  };
+  int count = gather(false);
+  if (count <= kSegList && floor > A(-INFINITY)) {
+    for (int e = 0; e < count; e += 32) {
+      const bool ok = e + lane < count;
+      const int64_t g = ok ? list[e + lane] : 0;
+      top.offer(ok ? segs[g * rows] : A(0), ok ? segment_step(la, (int)g, la.places[g * rows + r]) : 0, ok, floor, k);
+    }
+    const A bound = top.kv;  // no less than the floor
+    for (int e = 0; e < count; e += 32) {
+      const int64_t g = e + lane < count ? list[e + lane] : 0;
+      unsigned mask = __ballot_sync(~0u, e + lane < count && static_cast<const A *>(la.seconds)[g * rows + r] >= bound);
+      while (mask) {
+        const int64_t gs = __shfl_sync(~0u, g, __ffs(mask) - 1);
+        mask &= mask - 1;
+        const int place = la.places[gs * rows + r];
+        for (int i = 0; i < 1 << la.len_log2; i += 32) {
+          const int step = segment_step(la, (int)gs, i + lane);
+          const bool ok = i + lane < 1 << la.len_log2 && i + lane != place && step < D;
+          top.offer(ok ? to_acc(x[step * a.x.sd]) : A(0), step, ok, bound, k);
+        }
+      }
+    }
+  } else {
+    // Many logits equal to the floor: those over it from their segments (less
+    // than k lanes have one), the others from the row's beginning, where
+    // enough of them are soon found.
+    count = gather(true);
+    if (count <= kSegList) {
+      look(count << la.len_log2, true);
+    } else {
+      for (int s = 0; s < D; s += 32) {
+        const A v = s + lane < D ? to_acc(x[(s + lane) * a.x.sd]) : A(NAN);
+        top.offer(v, s + lane, v > floor, floor, k);
+      }
+    }
+    for (int s = 0; s < D && top.ki == kNone; s += 32) {
+      const A v = s + lane < D ? to_acc(x[(s + lane) * a.x.sd]) : A(NAN);
+      top.offer(v, s + lane, v == floor, floor, k);
+    }
+  }
+  return top;
+}
+
+// A warp a row: joins the parts of blocks and finds the alternatives.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 3 : 5) k_logprob_join(const __grid_constant__ LaneArgs la) {
+  using A = typename AccOf<T>::type;
+  __shared__ int sh_list[TOP ? 8 : 1][TOP ? kSegList : 1];
+  const LogprobArgs &a = la.a;
+  const int lane = threadIdx.x & 31;
   const int64_t rows = a.s.rows(), r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (r >= rows) return;
   const T *x = row_ptr<T>(a.x, r, a.s.L);
@@ -756,77 +885,114 @@ __global__ void __launch_bounds__(256) k_logprob_join(LaneArgs la) {
   const A xt = asked_logit<T, A>(a, t, x);
   TopList<A> top;
   top.init();
-  if constexpr (TOP) {
-    const A *segs = static_cast<const A *>(la.segs) + r;
-    const int n = la.nsegs, D = (int)a.s.D;
-    int *list = sh_list[threadIdx.x >> 5];
-    A kept[U], lm = A(-INFINITY);  // the first segments' maxima, and the largest of this lane's
+  if constexpr (TOP) top = row_alternatives<T>(la, r, sh_list[threadIdx.x >> 5]);
+  finish_row<A, TOP>(a, r, p, top.v, top.i, t, xt);
+}
+
+template <typename T>
+__device__ __noinline__ TopList<typename AccOf<T>::type> row_alternatives_apart(const LaneArgs &la, int64_t r, int *list) {
+  return row_alternatives<T>(la, r, list);
+}
+
+// Few alternatives of many rows: a thread a row, its list in registers, so that
+// the segments are read along the rows and a row costs a tenth of a warp's
+// instructions.  A segment that has to be read again, and a row with fewer than
+// K logits above -Inf, is looked at by the whole warp.
+template <typename T, int K>
+__global__ void __launch_bounds__(128) k_logprob_pick(const __grid_constant__ LaneArgs la) {
+  using A = typename AccOf<T>::type;
+  constexpr int U = 8;
+  __shared__ int sh_list[4][kSegList];
+  const LogprobArgs &a = la.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = a.s.rows(), row = (int64_t)blockIdx.x * 128 + threadIdx.x;
+  const bool active = row < rows;
+  const int64_t r = active ? row : rows - 1;
+  const T *x = row_ptr<T>(a.x, r, a.s.L);
+  const int64_t t = asked_token(a, r);
+  const A *segs = static_cast<const A *>(la.segs) + r, *seconds = static_cast<const A *>(la.seconds) + r;
+  const uint8_t *places = la.places + r;
+  const int n = la.nsegs, D = (int)a.s.D, len = 1 << la.len_log2;
+  A v[K];
+  int at[K], g[K];  // logit, its place in the row, its segment
 #pragma unroll
-    for (int u = 0; u < U; ++u) kept[u] = u * 32 + lane < n ? segs[(int64_t)(u * 32 + lane) * rows] : A(NAN);
+  for (int j = 0; j < K; ++j) {
+    v[j] = A(-INFINITY);
+    at[j] = kNone;
+    g[j] = 0;
+  }
+  auto insert = [&](A y, int i, int from) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) lm = LpMath<A>::max2(lm, kept[u]);
-    for (int g = U * 32 + lane; g < n; g += 32) lm = LpMath<A>::max2(lm, segs[(int64_t)g * rows]);
-    const A floor = kth_of_lanes(lm, k);  // k segments, so k logits, are at least this large
-    // the segments that reach the floor; with `above` those over it
-    auto gather = [&](bool above) {
-      int count = 0;
-      auto add = [&](int g, A v) {
-        const bool in = above ? v > floor : v >= floor;
-        const unsigned mask = __ballot_sync(~0u, in);
-        const int at = count + __popc(mask & ((1u << lane) - 1));
-        if (in && at < kSegList) list[at] = g;
-        count += __popc(mask);
-      };
-#pragma unroll
-      for (int u = 0; u < U; ++u) add(u * 32 + lane, kept[u]);
-      for (int b = U * 32; b < n; b += 32) add(b + lane, b + lane < n ? segs[(int64_t)(b + lane) * rows] : A(NAN));
-      __syncwarp();
-      return count;
-    };
-    // logit e of segment g: tile g / 8 of groups, step within it
-    auto look = [&](int to, bool above) {
-      constexpr int M = 4;  // batches in flight
-      for (int e = 0; e < to; e += 32 * M) {
-        A v[M];
-        int step[M];
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-          const int at = e + m * 32 + lane;
-          step[m] = D;
-          if (at < to) {
-            const int g = list[at >> la.len_log2], i = at & ((1 << la.len_log2) - 1);
-            step[m] = ((((g >> 3) << la.group_log2) + (i >> la.un_log2)) << (la.un_log2 + 3)) +
-                      ((i & ((1 << la.un_log2) - 1)) << 3) + (g & 7);
-          }
-          v[m] = step[m] < D ? to_acc(x[step[m] * a.x.sd]) : A(NAN);
-        }
-#pragma unroll
-        for (int m = 0; m < M; ++m) top.offer(v[m], step[m], above ? v[m] > floor : v[m] >= floor, floor, k);
+    for (int j = K - 1; j >= 0; --j) {
+      const int q = j > 0 ? j - 1 : 0;
+      const bool here = better(y, i, v[j], at[j]), above = j > 0 && better(y, i, v[q], at[q]);
+      if (here) {
+        v[j] = above ? v[q] : y;
+        at[j] = above ? at[q] : i;
+        g[j] = above ? g[q] : from;
       }
-    };
-    int count = gather(false);
-    if (count <= kSegList && floor > A(-INFINITY)) {
-      look(count << la.len_log2, false);
-    } else {
-      // Many logits equal to the floor: those over it from their segments (less
-      // than k lanes have one), the others from the row's beginning, where
-      // enough of them are soon found.
-      count = gather(true);
-      if (count <= kSegList) {
-        look(count << la.len_log2, true);
-      } else {
-        for (int s = 0; s < D; s += 32) {
-          const A v = s + lane < D ? to_acc(x[(s + lane) * a.x.sd]) : A(NAN);
-          top.offer(v, s + lane, v > floor, floor, k);
+    }
+  };
+  for (int b = 0; b < n; b += U) {
+    A s[U];
+    int w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = (int64_t)(b + u < n ? b + u : 0) * rows;
+      s[u] = b + u < n ? segs[i] : A(-INFINITY);
+      w[u] = places[i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s[u] >= v[K - 1] && s[u] > A(-INFINITY)) insert(s[u], segment_step(la, b + u, w[u]), b + u);
+  }
+  const A bound = v[K - 1];
+  bool again[K];
+  int seg[K], first[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    seg[j] = g[j];
+    first[j] = at[j];
+    again[j] = active && bound > A(-INFINITY) && seconds[(int64_t)g[j] * rows] >= bound;
+  }
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    for (unsigned mask = __ballot_sync(~0u, again[j]); mask; mask &= mask - 1) {
+      const int src = __ffs(mask) - 1, gs = __shfl_sync(~0u, seg[j], src), fs = __shfl_sync(~0u, first[j], src);
+      const A lim = __shfl_sync(~0u, bound, src);
+      const T *xs = row_ptr<T>(a.x, __shfl_sync(~0u, r, src), a.s.L);
+      for (int i = 0; i < len; i += 32) {
+        const int step = segment_step(la, gs, i + lane);
+        const bool ok = i + lane < len && step < D && step != fs;
+        const A y = ok ? to_acc(xs[step * a.x.sd]) : A(0);
+        for (unsigned in = __ballot_sync(~0u, ok && y >= lim); in; in &= in - 1) {
+          const A z = __shfl_sync(~0u, y, __ffs(in) - 1);
+          const int zi = __shfl_sync(~0u, step, __ffs(in) - 1);
+          if (lane == src) insert(z, zi, 0);
         }
       }
-      for (int s = 0; s < D && top.ki == kNone; s += 32) {
-        const A v = s + lane < D ? to_acc(x[(s + lane) * a.x.sd]) : A(NAN);
-        top.offer(v, s + lane, v == floor, floor, k);
+    }
+  for (unsigned mask = __ballot_sync(~0u, active && !(bound > A(-INFINITY))); mask; mask &= mask - 1) {
+    const int src = __ffs(mask) - 1;
+    const TopList<A> top = row_alternatives_apart<T>(la, __shfl_sync(~0u, r, src), sh_list[threadIdx.x >> 5]);
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      const A tv = __shfl_sync(~0u, top.v, j);
+      const int ti = __shfl_sync(~0u, top.i, j);
+      if (lane == src) {
+        v[j] = tv;
+        at[j] = ti;
       }
     }
   }
-  finish_row<A, TOP>(a, r, p, top.v, top.i, t, xt);
+  if (!active) return;
+  const A c = LpMath<A>::factor(a.scale);
+  Part<A> p = static_cast<const Part<A> *>(la.parts)[r];
+  for (int q = 1; q < la.chunks; ++q) p.merge(static_cast<const Part<A> *>(la.parts)[q * rows + r], c);
+  const RowResult<A> res(a, p);
+  res.stats(a, r, p, t, asked_logit<T, A>(a, t, x));
+#pragma unroll
+  for (int j = 0; j < K; ++j) res.alternative(a, r, j, v[j], at[j]);
 }
 
 struct LogprobGradArgs {
@@ -1022,11 +1188,16 @@ static acd_status launch_lanes(acd_ctx *ctx, const LogprobArgs &a, cudaStream_t 
   const int64_t blocks = la.lblocks * a.s.O, tiles = (a.s.D + S::STEPS - 1) / S::STEPS;
   la.group = 1;
   while (1 << la.un_log2 < S::UN) ++la.un_log2;
-  if (TOP)  // segments written and read, against k of them read again in 32-byte sectors
-    while (4 * la.group * S::UN * la.group * S::UN * a.k < a.s.D) {
+  if (TOP) {
+    // a segment of n logits costs 18 bytes written and read, and k^2 / 2 in the
+    // row's V / n segments are read again, 64 bytes a logit: least at n^3 = 0.28
+    // (V / k)^2 (places are bytes: at most 256)
+    auto enough = [&](double m) { return m * m * m * a.k * a.k > 0.28 * (double)a.s.D * (double)a.s.D; };
+    while (la.group * S::UN < 256 && !enough(1.5 * la.group * S::UN)) {
       la.group *= 2;
       ++la.group_log2;
     }
+  }
   la.len_log2 = la.un_log2 + la.group_log2;
   // rows are divided while there is room for blocks, eight tiles each at least
   int64_t chunks = (int64_t)ctx->sm_count * 3 / blocks;
@@ -1041,12 +1212,33 @@ static acd_status launch_lanes(acd_ctx *ctx, const LogprobArgs &a, cudaStream_t 
   if (join) {
     const size_t np = (size_t)la.chunks * a.s.rows(), ns = TOP ? (size_t)la.nsegs * a.s.rows() : 0;
     void *scratch;
-    ACD_TRY(get_scratch(ctx, ns * sizeof(A) + np * sizeof(Part<A>), s, &scratch));
-    la.segs = scratch;  // 16-byte pieces: rows are a multiple of V
-    la.parts = static_cast<A *>(scratch) + ns;
+    ACD_TRY(get_scratch(ctx, ns * (2 * sizeof(A) + 1) + np * sizeof(Part<A>), s, &scratch));
+    la.segs = scratch;  // written V rows at a time: rows are a multiple of V
+    la.seconds = static_cast<A *>(scratch) + ns;
+    la.parts = static_cast<A *>(scratch) + 2 * ns;
+    la.places = reinterpret_cast<uint8_t *>(static_cast<Part<A> *>(la.parts) + np);
   }
   k_logprob_lanes<T, V, TOP><<<(unsigned)(blocks * la.chunks), 256, 0, s>>>(la);
-  if (join) k_logprob_join<T, TOP><<<(unsigned)((a.s.rows() + 7) / 8), 256, 0, s>>>(la);
+  if (!join) return ACD_OK;
+  if constexpr (TOP && sizeof(T) < 8) {
+    // a thread a row from four warps an SM on (65536 rows of 4096 float32, five
+    // alternatives: the warp kernel takes 190 us for this part)
+    if (a.k <= 8 && a.s.rows() >= (int64_t)ctx->sm_count * 128) {
+      const unsigned grid = (unsigned)((a.s.rows() + 127) / 128);
+      switch (a.k) {
+        case 1: k_logprob_pick<T, 1><<<grid, 128, 0, s>>>(la); break;
+        case 2: k_logprob_pick<T, 2><<<grid, 128, 0, s>>>(la); break;
+        case 3: k_logprob_pick<T, 3><<<grid, 128, 0, s>>>(la); break;
+        case 4: k_logprob_pick<T, 4><<<grid, 128, 0, s>>>(la); break;
+        case 5: k_logprob_pick<T, 5><<<grid, 128, 0, s>>>(la); break;
+        case 6: k_logprob_pick<T, 6><<<grid, 128, 0, s>>>(la); break;
+        case 7: k_logprob_pick<T, 7><<<grid, 128, 0, s>>>(la); break;
+        default: k_logprob_pick<T, 8><<<grid, 128, 0, s>>>(la); break;
+      }
+      return ACD_OK;
+    }
+  }
+  k_logprob_join<T, TOP><<<(unsigned)((a.s.rows() + 7) / 8), 256, 0, s>>>(la);
   return ACD_OK;
 }
 

@@ -167,6 +167,23 @@ def test_ties_of_coarse_logits(acd, dtype, axis, V):
         check_forward(acd, x, dtype, axis, tokens, 1.0, top)
 
 
+@pytest.mark.parametrize("dtype", ["float", "float16"])
+@pytest.mark.parametrize("top", [1, 3, 5, 8, 9])
+def test_many_rows_across_the_lanes(acd, dtype, top):
+    """Rows enough for a thread each: smooth, coarse (ties at the last
+    alternative), masked to fewer tokens than alternatives, empty, with NaN."""
+    rng = np.random.default_rng(top)
+    rows, V = 19001, 270
+    x = (rng.standard_normal((rows, V)) * 3).astype(NP[dtype])
+    x[:6000] = np.rint(x[:6000])
+    x[100:200] = -np.inf
+    x[150:200, 17] = 1
+    x[160:200, 3] = 1
+    x[200:220, ::5] = np.nan
+    x[220:240] = 2
+    check_forward(acd, x, dtype, 2, make_tokens(rng, rows, V), 1.0, top)
+
+
 def test_nan_row_has_nan_gradient_and_leaves_its_neighbours(acd):
     x = np.random.default_rng(0).standard_normal((100, 3)).astype(np.float32)
     x[7, 1] = np.nan
