@@ -584,16 +584,18 @@ __global__ void __launch_bounds__(NW * 32, sizeof(T) == 8 ? 2 : TOP ? 3 : 4) k_l
 // time and nothing is exchanged but at the end.
 //   m is a reference here, not the maximum: sums are scaled anew only when a
 // logit is 8 bits above it, which after the first steps it hardly ever is.
-//   For the alternatives a thread also leaves the two largest logits of each
-// segment of its steps, and where the largest is (9 bytes a segment).  k
-// segments' largest logits set a bound that the k best logits reach, so each of
-// these is the largest of its segment, or stands in a segment whose second
-// largest reaches the bound too: of those, a few in a hundred, all logits are
-// read again.
+//   For the alternatives a thread takes the maximum of every four of its logits
+// (a unit), and for each segment of its steps leaves the two largest of these
+// and where the largest is (9 bytes a segment).  k segments' largest logits set
+// a bound that the k best logits reach, so each of these stands in the best unit
+// of a segment, or in a segment whose second value reaches the bound too: of
+// those, a few in a hundred, all logits are read again.
 //   (Lists kept while reading cost far more: 65536 x 4096 float32 with five
 // alternatives took 462 us with tiles turned round in shared memory, 643 us with
 // candidates gathered by atomics; reading the best segments again without
-// knowing where in them took 336 us.)
+// knowing where in them took 336 us, tracking single logits 311 us; 264 us now.)
+constexpr int kUnit = 4;  // logits of which one maximum is taken
+
 template <typename A, int V>
 struct LaneShape {
   static constexpr int UN = (sizeof(A) == 8 ? 8 : 16) / V;  // steps a thread and tile
@@ -607,8 +609,8 @@ struct LaneArgs {
   int chunks;       // blocks a row
   void *parts;      // [chunk][row], null: the block writes the results
   void *segs;       // [tile group][warp][row]: largest logit of `group` tiles' steps of a thread,
-  void *seconds;    //   the next largest (or the same again),
-  uint8_t *places;  //   and which of the segment's logits the largest is (the first such)
+  void *seconds;    //   the largest outside its unit,
+  uint8_t *places;  //   and which unit that is
   int nsegs;        // segments a row
   int group;        // tiles a segment
   int un_log2, group_log2, len_log2;  // steps a thread and tile, tiles and logits a segment
@@ -660,11 +662,17 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
     s1st[j] = s2nd[j] = A(-INFINITY);
     place[j] = 0;
   }
-  int at = 0;  // logits of the segment so far
+  int unit = 0;  // units of the segment so far
   int64_t seg = ((int64_t)(s0 / (STEPS * la.group)) * 8 + warp) * a.s.rows() + o * L + l;
   if (s0 < s1) load(s0, cur);
   for (int s = s0; s < s1; s += STEPS) {
-    if (s + STEPS < s1) load(s + STEPS, next);
+    // the next tile is under way meanwhile; with the segments' values there are
+    // no registers for it at four blocks an SM, which are worth more
+    if (TOP) {
+      if (s > s0) load(s, cur);
+    } else if (s + STEPS < s1) {
+      load(s + STEPS, next);
+    }
     A f[UN][V];
 #pragma unroll
     for (int u = 0; u < UN; ++u) cur[u].widen(f[u]);
@@ -672,22 +680,22 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
     A bm[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      bm[j] = LpMath<A>::max2(f[0][j], A(-INFINITY));
+      bm[j] = A(-INFINITY);
 #pragma unroll
-      for (int u = 1; u < UN; ++u) bm[j] = LpMath<A>::max2(bm[j], f[u][j]);
+      for (int q = 0; q < UN / kUnit; ++q) {
+        A um = f[q * kUnit][j];
+#pragma unroll
+        for (int u = 1; u < kUnit; ++u) um = LpMath<A>::max2(um, f[q * kUnit + u][j]);
+        if (TOP) {
+          place[j] = um > s1st[j] ? unit + q : place[j];
+          s2nd[j] = LpMath<A>::max2(s2nd[j], LpMath<A>::min2(um, s1st[j]));
+          s1st[j] = LpMath<A>::max2(s1st[j], um);
+        }
+        bm[j] = LpMath<A>::max2(bm[j], um);
+      }
       grown |= bm[j] > limit[j];
     }
-    if (TOP) {
-#pragma unroll
-      for (int u = 0; u < UN; ++u)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          place[j] = f[u][j] > s1st[j] ? at + u : place[j];
-          s2nd[j] = LpMath<A>::max2(s2nd[j], LpMath<A>::min2(f[u][j], s1st[j]));
-          s1st[j] = LpMath<A>::max2(s1st[j], f[u][j]);
-        }
-      at += UN;
-    }
+    unit += UN / kUnit;
     if (__any_sync(~0u, grown)) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
@@ -724,7 +732,7 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
         p[j].sum(col, c);
       }
     }
-    if (TOP && (at == 1 << la.len_log2 || s + STEPS >= s1)) {
+    if (TOP && (unit * kUnit == 1 << la.len_log2 || s + STEPS >= s1)) {
       Vec<A, V> w1, w2;
       Vec<uint8_t, V> wp;
 #pragma unroll
@@ -735,7 +743,7 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
         s1st[j] = s2nd[j] = A(-INFINITY);
         place[j] = 0;
       }
-      at = 0;
+      unit = 0;
       if (active) {
         *reinterpret_cast<Vec<A, V> *>(static_cast<A *>(la.segs) + seg) = w1;
         *reinterpret_cast<Vec<A, V> *>(static_cast<A *>(la.seconds) + seg) = w2;
@@ -743,8 +751,10 @@ __global__ void __launch_bounds__(256, 4) k_logprob_lanes(LaneArgs la) {
       }
       seg += 8 * a.s.rows();
     }
+    if (!TOP) {
 #pragma unroll
-    for (int u = 0; u < UN; ++u) cur[u] = next[u];
+      for (int u = 0; u < UN; ++u) cur[u] = next[u];
+    }
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) parts[warp][lane * V + j] = p[j];
@@ -825,10 +835,15 @@ __device__ __forceinline__ TopList<typename AccOf<T>::type> row_alternatives(con
   };
   int count = gather(false);
   if (count <= kSegList && floor > A(-INFINITY)) {
-    for (int e = 0; e < count; e += 32) {
-      const bool ok = e + lane < count;
-      const int64_t g = ok ? list[e + lane] : 0;
-      top.offer(ok ? segs[g * rows] : A(0), ok ? segment_step(la, (int)g, la.places[g * rows + r]) : 0, ok, floor, k);
+    for (int e = 0; e < count * kUnit; e += 32) {
+      const int at = e + lane;
+      int step = D;
+      if (at < count * kUnit) {
+        const int g = list[at / kUnit];
+        step = segment_step(la, g, la.places[(int64_t)g * rows + r] * kUnit + at % kUnit);
+      }
+      const A v = step < D ? to_acc(x[step * a.x.sd]) : A(NAN);
+      top.offer(v, step, v >= floor, floor, k);
     }
     const A bound = top.kv;  // no less than the floor
     for (int e = 0; e < count; e += 32) {
@@ -840,7 +855,7 @@ __device__ __forceinline__ TopList<typename AccOf<T>::type> row_alternatives(con
         const int place = la.places[gs * rows + r];
         for (int i = 0; i < 1 << la.len_log2; i += 32) {
           const int step = segment_step(la, (int)gs, i + lane);
-          const bool ok = i + lane < 1 << la.len_log2 && i + lane != place && step < D;
+          const bool ok = i + lane < 1 << la.len_log2 && (i + lane) / kUnit != place && step < D;
           top.offer(ok ? to_acc(x[step * a.x.sd]) : A(0), step, ok, bound, k);
         }
       }
@@ -894,14 +909,15 @@ __device__ __noinline__ TopList<typename AccOf<T>::type> row_alternatives_apart(
   return row_alternatives<T>(la, r, list);
 }
 
-// Few alternatives of many rows: a thread a row, its list in registers, so that
+// Few alternatives of many rows: a thread a row, its lists in registers, so that
 // the segments are read along the rows and a row costs a tenth of a warp's
-// instructions.  A segment that has to be read again, and a row with fewer than
-// K logits above -Inf, is looked at by the whole warp.
+// instructions.  three segments more than K are kept for those that tie with
+// the K-th; a row with more ties, or with fewer than K logits above -Inf, and a
+// segment that has to be read again are looked at by the whole warp.
 template <typename T, int K>
 __global__ void __launch_bounds__(128) k_logprob_pick(const __grid_constant__ LaneArgs la) {
   using A = typename AccOf<T>::type;
-  constexpr int U = 8;
+  constexpr int U = 8, N = K + 3;
   __shared__ int sh_list[4][kSegList];
   const LogprobArgs &a = la.a;
   const int lane = threadIdx.x & 31;
@@ -913,66 +929,92 @@ __global__ void __launch_bounds__(128) k_logprob_pick(const __grid_constant__ La
   const A *segs = static_cast<const A *>(la.segs) + r, *seconds = static_cast<const A *>(la.seconds) + r;
   const uint8_t *places = la.places + r;
   const int n = la.nsegs, D = (int)a.s.D, len = 1 << la.len_log2;
-  A v[K];
-  int at[K], g[K];  // logit, its place in the row, its segment
+  A v[N], lost = A(-INFINITY);  // segments by their largest logit; the largest left out
+  int g[N];
 #pragma unroll
-  for (int j = 0; j < K; ++j) {
+  for (int j = 0; j < N; ++j) {
     v[j] = A(-INFINITY);
-    at[j] = kNone;
     g[j] = 0;
   }
-  auto insert = [&](A y, int i, int from) {
+  for (int b = 0; b < n; b += U) {
+    A s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = b + u < n ? segs[(int64_t)(b + u) * rows] : A(-INFINITY);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      lost = LpMath<A>::max2(lost, LpMath<A>::min2(s[u], v[N - 1]));
+      if (s[u] > v[N - 1]) {
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j) {
+          const int q = j > 0 ? j - 1 : 0;
+          const bool here = s[u] > v[j], above = j > 0 && s[u] > v[q];
+          if (here) {
+            v[j] = above ? v[q] : s[u];
+            g[j] = above ? g[q] : b + u;
+          }
+        }
+      }
+    }
+  }
+  const A bound = v[K - 1];
+  const bool plain = bound > A(-INFINITY) && lost < bound;
+  A w[K];  // the logits
+  int at[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    w[j] = A(-INFINITY);
+    at[j] = kNone;
+  }
+  auto insert = [&](A y, int i) {
 #pragma unroll
     for (int j = K - 1; j >= 0; --j) {
       const int q = j > 0 ? j - 1 : 0;
-      const bool here = better(y, i, v[j], at[j]), above = j > 0 && better(y, i, v[q], at[q]);
+      const bool here = better(y, i, w[j], at[j]), above = j > 0 && better(y, i, w[q], at[q]);
       if (here) {
-        v[j] = above ? v[q] : y;
+        w[j] = above ? w[q] : y;
         at[j] = above ? at[q] : i;
-        g[j] = above ? g[q] : from;
       }
     }
   };
-  for (int b = 0; b < n; b += U) {
-    A s[U];
-    int w[U];
+  int place[N];
+  bool again[N];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t i = (int64_t)(b + u < n ? b + u : 0) * rows;
-      s[u] = b + u < n ? segs[i] : A(-INFINITY);
-      w[u] = places[i];
+  for (int j = 0; j < N; ++j) {
+    const bool in = active && plain && v[j] >= bound;
+    place[j] = in ? places[(int64_t)g[j] * rows] : -1;
+    again[j] = in && seconds[(int64_t)g[j] * rows] >= bound;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    A y[kUnit];
+    int step[kUnit];
+#pragma unroll
+    for (int u = 0; u < kUnit; ++u) {
+      step[u] = segment_step(la, g[j], place[j] * kUnit + u);
+      y[u] = place[j] >= 0 && step[u] < D ? to_acc(x[step[u] * a.x.sd]) : A(NAN);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s[u] >= v[K - 1] && s[u] > A(-INFINITY)) insert(s[u], segment_step(la, b + u, w[u]), b + u);
-  }
-  const A bound = v[K - 1];
-  bool again[K];
-  int seg[K], first[K];
-#pragma unroll
-  for (int j = 0; j < K; ++j) {
-    seg[j] = g[j];
-    first[j] = at[j];
-    again[j] = active && bound > A(-INFINITY) && seconds[(int64_t)g[j] * rows] >= bound;
+    for (int u = 0; u < kUnit; ++u)
+      if (y[u] >= bound) insert(y[u], step[u]);
   }
 #pragma unroll
-  for (int j = 0; j < K; ++j)
+  for (int j = 0; j < N; ++j)
     for (unsigned mask = __ballot_sync(~0u, again[j]); mask; mask &= mask - 1) {
-      const int src = __ffs(mask) - 1, gs = __shfl_sync(~0u, seg[j], src), fs = __shfl_sync(~0u, first[j], src);
+      const int src = __ffs(mask) - 1, gs = __shfl_sync(~0u, g[j], src), ps = __shfl_sync(~0u, place[j], src);
       const A lim = __shfl_sync(~0u, bound, src);
       const T *xs = row_ptr<T>(a.x, __shfl_sync(~0u, r, src), a.s.L);
       for (int i = 0; i < len; i += 32) {
         const int step = segment_step(la, gs, i + lane);
-        const bool ok = i + lane < len && step < D && step != fs;
+        const bool ok = i + lane < len && step < D && (i + lane) / kUnit != ps;
         const A y = ok ? to_acc(xs[step * a.x.sd]) : A(0);
         for (unsigned in = __ballot_sync(~0u, ok && y >= lim); in; in &= in - 1) {
           const A z = __shfl_sync(~0u, y, __ffs(in) - 1);
           const int zi = __shfl_sync(~0u, step, __ffs(in) - 1);
-          if (lane == src) insert(z, zi, 0);
+          if (lane == src) insert(z, zi);
         }
       }
     }
-  for (unsigned mask = __ballot_sync(~0u, active && !(bound > A(-INFINITY))); mask; mask &= mask - 1) {
+  for (unsigned mask = __ballot_sync(~0u, active && !plain); mask; mask &= mask - 1) {
     const int src = __ffs(mask) - 1;
     const TopList<A> top = row_alternatives_apart<T>(la, __shfl_sync(~0u, r, src), sh_list[threadIdx.x >> 5]);
 #pragma unroll
@@ -980,7 +1022,7 @@ __global__ void __launch_bounds__(128) k_logprob_pick(const __grid_constant__ La
       const A tv = __shfl_sync(~0u, top.v, j);
       const int ti = __shfl_sync(~0u, top.i, j);
       if (lane == src) {
-        v[j] = tv;
+        w[j] = tv;
         at[j] = ti;
       }
     }
@@ -992,7 +1034,7 @@ __global__ void __launch_bounds__(128) k_logprob_pick(const __grid_constant__ La
   const RowResult<A> res(a, p);
   res.stats(a, r, p, t, asked_logit<T, A>(a, t, x));
 #pragma unroll
-  for (int j = 0; j < K; ++j) res.alternative(a, r, j, v[j], at[j]);
+  for (int j = 0; j < K; ++j) res.alternative(a, r, j, w[j], at[j]);
 }
 
 struct LogprobGradArgs {
