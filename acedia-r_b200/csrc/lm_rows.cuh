@@ -30,6 +30,61 @@ __device__ __forceinline__ __half from_acc<__half, float>(float x) { return __fl
 __device__ __forceinline__ float fma_a(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_a(double a, double b, double c) { return fma(a, b, c); }
 
+// Two float32 values in one register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// As many accumulator values as one instruction takes: two float32, one float64.
+template <typename A>
+struct Pk;
+template <>
+struct Pk<float> {
+  static constexpr int N = 2;
+  uint64_t v;
+  static __device__ __forceinline__ Pk from(const float *f) { return {pack2(f[0], f[1])}; }
+  static __device__ __forceinline__ Pk all(float x) { return {pack2(x, x)}; }
+  __device__ __forceinline__ void to(float *f) const { unpack2(v, f[0], f[1]); }
+  __device__ __forceinline__ float sum() const {
+    float a, b;
+    unpack2(v, a, b);
+    return a + b;
+  }
+};
+__device__ __forceinline__ Pk<float> pmul(Pk<float> a, Pk<float> b) { return {mul2(a.v, b.v)}; }
+__device__ __forceinline__ Pk<float> pfma(Pk<float> a, Pk<float> b, Pk<float> c) { return {fma2(a.v, b.v, c.v)}; }
+template <>
+struct Pk<double> {
+  static constexpr int N = 1;
+  double v;
+  static __device__ __forceinline__ Pk from(const double *f) { return {f[0]}; }
+  static __device__ __forceinline__ Pk all(double x) { return {x}; }
+  __device__ __forceinline__ void to(double *f) const { f[0] = v; }
+  __device__ __forceinline__ double sum() const { return v; }
+};
+__device__ __forceinline__ Pk<double> pmul(Pk<double> a, Pk<double> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Pk<double> pfma(Pk<double> a, Pk<double> b, Pk<double> c) { return {fma(a.v, b.v, c.v)}; }
+
 // A tensor as rows: element d of row r = l + L*o lies at p + l*sl + d*sd + o*so.
 struct Rows {
   void *p = nullptr;

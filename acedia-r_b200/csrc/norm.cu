@@ -6,7 +6,12 @@
 //   t = dh + rs_h (dy w_pre - hn mean(dy w_pre hn)),  dr = alpha t,
 //   u = t gate,  db = rs_b (u w_post - bn mean(u w_post bn)),
 //   dw_pre = sum dy hn,  dw_post = sum u bn,  dgate = sum t b'.
+#include <cooperative_groups.h>
+
 #include "lm_rows.cuh"
+#include "tma.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace acd {
 
@@ -378,139 +383,371 @@ __device__ __forceinline__ void unit_rows(const GradPlan &p, int64_t u, int64_t 
   r1 = g * p.per + (part + 1) * p.per / p.parts;
 }
 
-// One piece of a row's gradient, in two steps around the row's sums.  With
-//   q = d_h + rs_h d_y w_pre,  hn = h rs_h,  bn = b rs_b,  e = gate w_post bn
-// t = q - rs_h hn m1, so that mean(u w_post bn) = mean(q e) - m1 mean(rs_h hn e)
-// comes from the same pass as m1 = mean(d_y w_pre hn): one reduction a row.
-template <typename T, typename A, int V, int TPR, bool WHOLE>
-struct GradPiece {
-  A dh[V], dy[V], h[V], b[V];
-  __device__ __forceinline__ void load(const NormGradArgs &a, int64_t row, int tid, int D) {
-    if (a.dh.p) {
-      load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dh, row, a.s.L), a.dh.sd, tid, 0, D, dh);
-    } else {
+// V columns of a row's gradient, in two steps around the row's sums.  With
+//   q = d_h + rs_h d_y w_pre,  hn = h rs_h,  bn = b rs_b,  f = gate w_post
+// t = q - rs_h hn m1, so that mean(u w_post bn) = mean(q f bn) - m1 rs_h
+// mean(hn f bn) comes from the same pass as m1 = mean(d_y w_pre hn): one
+// reduction a row.  sum t bn is what the gradients of the gate (times w_post)
+// and of w_post (times gate) have in common while the gate row stays the same.
+template <typename A, int V>
+struct GradCols {
+  using P = Pk<A>;
+  static constexpr int M = V / P::N;
+  P q[M], hn[M], bn[M], dy[M];
+  __device__ __forceinline__ void begin(const A (&dh)[V], const A (&dyv)[V], const A (&h)[V], const A (&b)[V],
+                                        const P (&wp)[M], const P (&f)[M], A rh, A rb, A (&s)[3]) {
+    const P prh = P::all(rh), prb = P::all(rb);
+    P s0 = P::all(A(0)), s1 = s0, s2 = s0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) dh[j] = A(0);
+    for (int j = 0; j < M; ++j) {
+      dy[j] = P::from(dyv + j * P::N);
+      hn[j] = pmul(P::from(h + j * P::N), prh);
+      bn[j] = pmul(P::from(b + j * P::N), prb);
+      const P u = pmul(dy[j], wp[j]), e = pmul(f[j], bn[j]);
+      q[j] = pfma(prh, u, P::from(dh + j * P::N));
+      s0 = pfma(u, hn[j], s0);
+      s1 = pfma(q[j], e, s1);
+      s2 = pfma(hn[j], e, s2);
     }
-    load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dy, row, a.s.L), a.dy.sd, tid, 0, D, dy);
-    load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.h, row, a.s.L), a.h.sd, tid, 0, D, h);
-    load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.b, row, a.s.L), a.b.sd, tid, 0, D, b);
+    s[0] = s0.sum();
+    s[1] = s1.sum();
+    s[2] = s2.sum();
   }
-  __device__ __forceinline__ void sums(const A *wp, const A *wo, const A *g, A rh, A rb, A (&s)[3]) const {
+  // s: the row's sums; adds to pre and tb, leaves the gradients in dr and db.
+  __device__ __forceinline__ void end(const A (&s)[3], A inv, A rh, A rb, A alpha, bool post, const P (&f)[M], P (&pre)[M],
+                                      P (&tb)[M], A (&dr)[V], A (&db)[V]) {
+    const A m1 = s[0] * inv * rh;
+    const P nm1 = P::all(-m1), nm2 = P::all(post ? -(s[1] - m1 * s[2]) * inv : A(0)), prb = P::all(rb), pal = P::all(alpha);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const A hn = h[j] * rh, u = dy[j] * wp[j], e = g[j] * wo[j] * (b[j] * rb);
-      s[0] = fma_a(u, hn, s[0]);
-      s[1] = fma_a(fma_a(rh, u, dh[j]), e, s[1]);
-      s[2] = fma_a(rh * hn, e, s[2]);
-    }
-  }
-  // Leaves alpha t in dh and the block's gradient in dy; adds to the sums.
-  __device__ __forceinline__ void finish(const A *wp, const A *wo, const A *g, A rh, A rb, A m1, A m2, A alpha,
-                                         bool post, A *pre, A *pst, A *gte) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const A hn = h[j] * rh, bn = b[j] * rb;
-      const A t = fma_a(rh, fma_a(dy[j], wp[j], -(hn * m1)), dh[j]);
-      const A u = t * g[j];
-      pre[j] = fma_a(dy[j], hn, pre[j]);
-      pst[j] = fma_a(u, bn, pst[j]);
-      gte[j] = fma_a(t, bn * wo[j], gte[j]);
-      dh[j] = alpha * t;
-      dy[j] = post ? rb * fma_a(u, wo[j], -(bn * m2)) : u;
+    for (int j = 0; j < M; ++j) {
+      const P t = pfma(hn[j], nm1, q[j]);
+      pre[j] = pfma(dy[j], hn[j], pre[j]);
+      tb[j] = pfma(t, bn[j], tb[j]);
+      pmul(pal, t).to(dr + j * P::N);
+      P x = pmul(t, f[j]);
+      if (post) x = pmul(pfma(bn[j], nm2, x), prb);
+      x.to(db + j * P::N);
     }
   }
 };
 
-template <typename A, int V>
-__device__ __forceinline__ void ones(A *v) {
+// The operands that stay while the gate row does: w_pre, and f = gate w_post.
+template <typename T, typename A, int V, int TPR, bool WHOLE>
+__device__ __forceinline__ void load_operands(const NormGradArgs &a, int64_t row, int tid, int D, A (&wo)[V], A (&g)[V],
+                                              Pk<A> (&f)[V / Pk<A>::N]) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = A(1);
+  for (int j = 0; j < V; ++j) wo[j] = g[j] = A(1);
+  if (a.w_post) load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.w_post), 1, tid, 0, D, wo);
+  if (a.gate)
+    load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + row / a.per * a.gate_sg, a.gate_sd, tid, 0, D, g);
+#pragma unroll
+  for (int j = 0; j < V / Pk<A>::N; ++j)
+    f[j] = pmul(Pk<A>::from(wo + j * Pk<A>::N), Pk<A>::from(g + j * Pk<A>::N));
 }
 
-// One piece a thread, TPR threads a row; the column sums stay in registers.
+// Adds the RPB sub-blocks' columns into the first one's, in order.
+template <typename A, int V, int TPR, int RPB>
+__device__ __forceinline__ void add_subs(A (&acc)[V], A (*join)[V]) {
+  if (RPB == 1) return;
+  const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < V; ++j) join[threadIdx.x][j] = acc[j];
+  __syncthreads();
+  if (sub == 0)
+    for (int q = 1; q < RPB; ++q)
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += join[q * TPR + tid][j];
+}
+
+template <typename A, int V, int TPR, bool WHOLE>
+__device__ __forceinline__ void store_sums(A *dst, int64_t sd, int tid, int D, const A (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int d = column<V, TPR, WHOLE>(tid, 0, j);
+    if (d < D) dst[d * sd] = v[j];
+  }
+}
+
+// V columns a thread, TPR threads a row; the column sums stay in registers.
 template <typename T, int TPR, bool WHOLE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_grad_vec(NormGradArgs a, GradPlan plan) {
   using A = typename AccOf<T>::type;
-  constexpr int V = 16 / sizeof(T), BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
+  using P = Pk<A>;
+  constexpr int V = 16 / sizeof(T), BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR, M = V / P::N;
   __shared__ A sh[2][BLOCK / 32 * 3];
   __shared__ A join[RPB > 1 ? BLOCK : 1][V];
   const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int D = (int)a.s.D;
-  const T *w_pre = static_cast<const T *>(a.w_pre), *w_post = static_cast<const T *>(a.w_post);
+  const bool post = a.w_post != nullptr;
   const A alpha = (A)a.alpha, inv = A(1) / (A)a.s.D;
-  A pre[V] = {}, pst[V] = {};
+  P wp[M], f[M], pre[M], pst[M];
+  A wo[V], g[V], c[V];
+  load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.w_pre), 1, tid, 0, D, c);
+#pragma unroll
+  for (int j = 0; j < M; ++j) {
+    wp[j] = P::from(c + j * P::N);
+    pre[j] = pst[j] = P::all(A(0));
+  }
   int flip = 0;
   for (int64_t u = blockIdx.x; u < plan.groups * plan.parts; u += gridDim.x) {
     int64_t r0, r1;
     unit_rows(plan, u, r0, r1);
-    A gte[V] = {};
+    load_operands<T, A, V, TPR, WHOLE>(a, r0, tid, D, wo, g, f);
+    P tb[M];
+#pragma unroll
+    for (int j = 0; j < M; ++j) tb[j] = P::all(A(0));
     for (int64_t rr = r0; rr < r1; rr += RPB) {
-      const int64_t row = rr + sub;
-      const bool ok = row < r1;
-      GradPiece<T, A, V, TPR, WHOLE> p;
-      p.load(a, ok ? row : r0, tid, ok ? D : 0);
-      A wp[V], wo[V], g[V];
-      load_cols<T, A, V, TPR, WHOLE>(w_pre, 1, tid, 0, D, wp);
-      if (w_post)
-        load_cols<T, A, V, TPR, WHOLE>(w_post, 1, tid, 0, D, wo);
-      else
-        ones<A, V>(wo);
-      if (a.gate)
-        load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + r0 / a.per * a.gate_sg, a.gate_sd, tid, 0, D, g);
-      else
-        ones<A, V>(g);
+      const bool ok = rr + sub < r1;
+      const int64_t row = ok ? rr + sub : r0;
+      const int n = ok ? D : 0;
+      A dh[V], dy[V], h[V], b[V], s[3];
+#pragma unroll
+      for (int j = 0; j < V; ++j) dh[j] = A(0);
+      if (a.dh.p) load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dh, row, a.s.L), a.dh.sd, tid, 0, n, dh);
+      load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dy, row, a.s.L), a.dy.sd, tid, 0, n, dy);
+      load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.h, row, a.s.L), a.h.sd, tid, 0, n, h);
+      load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.b, row, a.s.L), a.b.sd, tid, 0, n, b);
       const A rh = ok ? static_cast<const A *>(a.rstd_h)[row] : A(0);
-      const A rb = w_post && ok ? static_cast<const A *>(a.rstd_b)[row] : A(1);
-      A s[3] = {};
-      p.sums(wp, wo, g, rh, rb, s);
+      const A rb = post && ok ? static_cast<const A *>(a.rstd_b)[row] : A(1);
+      GradCols<A, V> p;
+      p.begin(dh, dy, h, b, wp, f, rh, rb, s);
       row_sum<A, 3, TPR>(s, sh[flip]);
       flip ^= 1;
-      const A m1 = s[0] * inv, m2 = (s[1] - m1 * s[2]) * inv;
-      p.finish(wp, wo, g, rh, rb, m1, m2, alpha, w_post != nullptr, pre, pst, gte);
-      if (ok) {
-        store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dr, row, a.s.L), a.dr.sd, tid, 0, D, p.dh);
-        store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.db, row, a.s.L), a.db.sd, tid, 0, D, p.dy);
-      }
+      p.end(s, inv, rh, rb, alpha, post, f, pre, tb, dh, dy);
+      store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dr, row, a.s.L), a.dr.sd, tid, 0, n, dh);
+      store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.db, row, a.s.L), a.db.sd, tid, 0, n, dy);
+    }
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      pst[j] = pfma(P::from(g + j * P::N), tb[j], pst[j]);
+      pmul(P::from(wo + j * P::N), tb[j]).to(c + j * P::N);
     }
     if (plan.gate) {
-      if (RPB > 1) {
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < V; ++j) join[threadIdx.x][j] = gte[j];
-        __syncthreads();
-        if (sub == 0)
-          for (int q = 1; q < RPB; ++q)
-#pragma unroll
-            for (int j = 0; j < V; ++j) gte[j] += join[q * TPR + tid][j];
-      }
-      if (sub == 0)
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (column<V, TPR, WHOLE>(tid, 0, j) < D)
-            static_cast<A *>(plan.gate)[u * plan.gate_su + column<V, TPR, WHOLE>(tid, 0, j) * plan.gate_sd] = gte[j];
+      add_subs<A, V, TPR, RPB>(c, join);
+      if (sub == 0) store_sums<A, V, TPR, WHOLE>(static_cast<A *>(plan.gate) + u * plan.gate_su, plan.gate_sd, tid, D, c);
     }
   }
+#pragma unroll
   for (int w = 0; w < 2; ++w) {
     A *dst = static_cast<A *>(w ? plan.post : plan.pre);
-    A *acc = w ? pst : pre;
     if (!dst) continue;
-    if (RPB > 1) {
-      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < V; ++j) join[threadIdx.x][j] = acc[j];
-      __syncthreads();
-      if (sub == 0)
-        for (int q = 1; q < RPB; ++q)
-#pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] += join[q * TPR + tid][j];
-    }
-    if (sub == 0)
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (column<V, TPR, WHOLE>(tid, 0, j) < D)
-          dst[(int64_t)blockIdx.x * D + column<V, TPR, WHOLE>(tid, 0, j)] = acc[j];
+    for (int j = 0; j < M; ++j) (w ? pst[j] : pre[j]).to(c + j * P::N);
+    add_subs<A, V, TPR, RPB>(c, join);
+    if (sub == 0) store_sums<A, V, TPR, WHOLE>(dst + (int64_t)blockIdx.x * D, 1, tid, D, c);
   }
+}
+
+// The same with rows brought in by bulk copies through a ring of stages, so that
+// several rows are under way while one is worked on (without it the loads of a
+// row waited for its two halves: 470 us on 16384 x 4096 float16).  A cluster of
+// CL blocks divides the columns of wider rows, each block of TPR compute threads
+// and a warp that issues the copies; the rows' sums then go to the other blocks
+// by asynchronous stores that count on a barrier there.
+constexpr uint64_t kRingWaitNs = 1000000000ull;  // 1 s
+constexpr int kRingWaitCode = 6;
+constexpr int kRingMost = 8;  // stages, blocks of a cluster
+
+template <typename A>
+struct RingShared {
+  uint64_t full[kRingMost], empty[kRingMost], joined[2];
+  A part[2][32][4];             // the warps' sums
+  A other[2][kRingMost][4];     // the blocks' sums
+  int abort;
+};
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_addr(dst)),
+               "l"(src), "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
+}
+
+// 16 bytes to the same place of block `rank` of the cluster, counted on its barrier.
+__device__ __forceinline__ void send16(const void *at, const uint64_t *bar, int rank, uint64_t lo, uint64_t hi) {
+  uint32_t d, m;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(at)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"(smem_addr(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(d), "l"(lo),
+               "l"(hi), "r"(m)
+               : "memory");
+}
+
+template <typename T, int TPR>
+__global__ void __launch_bounds__(TPR + 32, TPR <= 256 ? 2 : 1) k_norm_grad_ring(NormGradArgs a, GradPlan plan, int stages, Control *control) {
+  using A = typename AccOf<T>::type;
+  using P = Pk<A>;
+  constexpr int V = 16 / sizeof(T), M = V / P::N, NW = TPR / 32;
+  extern __shared__ __align__(128) unsigned char ring[];  // [stage][dy, h, b, dh][TPR * 16 bytes]
+  __shared__ RingShared<A> sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t cid = blockIdx.x / CL, nclusters = gridDim.x / CL;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
+  const int c0 = rank * TPR * V;  // this block's columns
+  const int D = (int)a.s.D - c0 < TPR * V ? (int)a.s.D - c0 : TPR * V;
+  const int64_t units = plan.groups * plan.parts;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], NW);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.joined[i], 1);
+    sh.abort = 0;
+    mbar_init_fence();
+  }
+  if (CL > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  if (warp == NW) {
+    if (lane == 0) {
+      const uint32_t bytes = D * (uint32_t)sizeof(T);
+      int n = 0, slot = 0;
+      uint32_t phase = 1;
+      bool go = true;
+      for (int64_t u = cid; go && u < units; u += nclusters) {
+        int64_t r0, r1;
+        unit_rows(plan, u, r0, r1);
+        for (int64_t row = r0; row < r1; ++row, ++n) {
+          if (n >= stages &&
+              !mbar_wait_thread(&sh.empty[slot], phase, &sh.abort, control, kRingWaitCode, kRingWaitNs)) {
+            go = false;
+            break;
+          }
+          unsigned char *st = ring + (size_t)slot * 4 * TPR * 16;
+          mbar_arrive_expect_tx(&sh.full[slot], bytes * (a.dh.p ? 4 : 3));
+          bulk_load(st, row_ptr<T>(a.dy, row, a.s.L) + c0, bytes, &sh.full[slot]);
+          bulk_load(st + TPR * 16, row_ptr<T>(a.h, row, a.s.L) + c0, bytes, &sh.full[slot]);
+          bulk_load(st + 2 * TPR * 16, row_ptr<T>(a.b, row, a.s.L) + c0, bytes, &sh.full[slot]);
+          if (a.dh.p) bulk_load(st + 3 * TPR * 16, row_ptr<T>(a.dh, row, a.s.L) + c0, bytes, &sh.full[slot]);
+          if (++slot == stages) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // given up: the copies in flight land before the block may end
+      if (*reinterpret_cast<volatile int *>(&sh.abort))
+        for (int q = n > stages ? n - stages : 0; q < n; ++q)
+          mbar_wait_bounded(&sh.full[q % stages], (uint32_t)(q / stages) & 1u, kRingWaitNs);
+    }
+  } else {
+    const bool post = a.w_post != nullptr;
+    const A alpha = (A)a.alpha, inv = A(1) / (A)a.s.D;
+    const bool mine = tid * V < D;
+    NormGradArgs slice = a;  // operands from this block's first column on
+    slice.w_pre = static_cast<const T *>(a.w_pre) + c0;
+    if (a.w_post) slice.w_post = static_cast<const T *>(a.w_post) + c0;
+    if (a.gate) slice.gate = static_cast<const T *>(a.gate) + c0;
+    P wp[M], f[M], pre[M], pst[M];
+    A c[V];
+    load_cols<T, A, V, TPR, true>(static_cast<const T *>(slice.w_pre), 1, tid, 0, D, c);
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      wp[j] = P::from(c + j * P::N);
+      pre[j] = pst[j] = P::all(A(0));
+    }
+    int slot = 0, flip = 0;
+    uint32_t phase = 0, joined = 0;
+    bool dead = false;
+    for (int64_t u = cid; u < units; u += nclusters) {
+      int64_t r0, r1;
+      unit_rows(plan, u, r0, r1);
+      A wo[V], g[V];
+      load_operands<T, A, V, TPR, true>(slice, r0, tid, D, wo, g, f);
+      P tb[M];
+#pragma unroll
+      for (int j = 0; j < M; ++j) tb[j] = P::all(A(0));
+      A rh_next = r0 < r1 ? static_cast<const A *>(a.rstd_h)[r0] : A(0);
+      A rb_next = r0 < r1 && post ? static_cast<const A *>(a.rstd_b)[r0] : A(1);
+      for (int64_t row = r0; row < r1; ++row) {
+        const A rh = rh_next, rb = rb_next;
+        if (row + 1 < r1) {
+          rh_next = static_cast<const A *>(a.rstd_h)[row + 1];
+          if (post) rb_next = static_cast<const A *>(a.rstd_b)[row + 1];
+        }
+        // once given up, the warps go on without waiting: all of them reach the barriers
+        dead = dead || !mbar_wait_warp(&sh.full[slot], phase, &sh.abort, control, kRingWaitCode, kRingWaitNs);
+        const unsigned char *st = ring + (size_t)slot * 4 * TPR * 16;
+        A dh[V], dy[V], h[V], b[V], s[3];
+#pragma unroll
+        for (int j = 0; j < V; ++j) dh[j] = A(0);
+        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st), 1, tid, 0, D, dy);
+        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + TPR * 16), 1, tid, 0, D, h);
+        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + 2 * TPR * 16), 1, tid, 0, D, b);
+        if (a.dh.p) load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + 3 * TPR * 16), 1, tid, 0, D, dh);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[slot]);
+        if (++slot == stages) {
+          slot = 0;
+          phase ^= 1u;
+        }
+        GradCols<A, V> p;
+        p.begin(dh, dy, h, b, wp, f, rh, rb, s);
+#pragma unroll
+        for (int q = 16; q; q >>= 1)
+#pragma unroll
+          for (int j = 0; j < 3; ++j) s[j] += __shfl_xor_sync(~0u, s[j], q);
+        if (lane == 0)
+#pragma unroll
+          for (int j = 0; j < 3; ++j) sh.part[flip][warp][j] = s[j];
+        asm volatile("bar.sync 1, %0;" ::"n"(TPR) : "memory");
+#pragma unroll
+        for (int j = 0; j < 3; ++j) s[j] = lane < NW ? sh.part[flip][lane][j] : A(0);
+#pragma unroll
+        for (int q = NW / 2; q; q >>= 1)
+#pragma unroll
+          for (int j = 0; j < 3; ++j) s[j] += __shfl_xor_sync(~0u, s[j], q);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) s[j] = __shfl_sync(~0u, s[j], 0);
+        if (CL > 1) {
+          if (warp == 0 && lane < CL) {
+            if (lane == 0) mbar_arrive_expect_tx(&sh.joined[flip], CL * 4 * (uint32_t)sizeof(A));
+            // the block's sums to every block, its own included
+            if constexpr (sizeof(A) == 4) {
+              send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, pack2(s[0], s[1]), pack2(s[2], 0.0f));
+            } else {
+              send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, __double_as_longlong(s[0]),
+                     __double_as_longlong(s[1]));
+              send16(&sh.other[flip][rank][2], &sh.joined[flip], lane, __double_as_longlong(s[2]), 0);
+            }
+          }
+          dead = dead || !mbar_wait_warp(&sh.joined[flip], joined, &sh.abort, control, kRingWaitCode, kRingWaitNs);
+#pragma unroll
+          for (int j = 0; j < 3; ++j) {
+            s[j] = A(0);
+            for (int q = 0; q < CL; ++q) s[j] += sh.other[flip][q][j];
+          }
+          joined ^= (uint32_t)flip;  // both barriers have had a phase
+        }
+        flip ^= 1;
+        p.end(s, inv, rh, rb, alpha, post, f, pre, tb, dh, dy);
+        if (mine) {
+          store_cols<T, A, V, TPR, true>(row_ptr<T>(a.dr, row, a.s.L) + c0, 1, tid, 0, D, dh);
+          store_cols<T, A, V, TPR, true>(row_ptr<T>(a.db, row, a.s.L) + c0, 1, tid, 0, D, dy);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < M; ++j) {
+        pst[j] = pfma(P::from(g + j * P::N), tb[j], pst[j]);
+        pmul(P::from(wo + j * P::N), tb[j]).to(c + j * P::N);
+      }
+      if (plan.gate)
+        store_sums<A, V, TPR, true>(static_cast<A *>(plan.gate) + u * plan.gate_su + c0 * plan.gate_sd, plan.gate_sd, tid, D, c);
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      A *dst = static_cast<A *>(w ? plan.post : plan.pre);
+      if (!dst) continue;
+#pragma unroll
+      for (int j = 0; j < M; ++j) (w ? pst[j] : pre[j]).to(c + j * P::N);
+      store_sums<A, V, TPR, true>(dst + cid * a.s.D + c0, 1, tid, D, c);
+    }
+  }
+  __syncwarp();
+  if (CL > 1) cluster.sync();  // no block leaves while another may still write to it
 }
 
 // Column sums of `n` partial rows: 32 columns a block, its 8 warps split the
@@ -591,18 +828,16 @@ static acd_status launch_norm(acd_ctx *ctx, const NormArgs &a, cudaStream_t s) {
   return ACD_OK;
 }
 
-template <typename T, int TPR>
-static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool whole, cudaStream_t s) {
-  using A = typename AccOf<T>::type;
-  constexpr int BLOCK = TPR < 256 ? 256 : TPR;
-  auto kern = whole ? k_norm_grad_vec<T, TPR, true> : k_norm_grad_vec<T, TPR, false>;
+// Deals the rows out to `grid` blocks (or clusters) that take `sub` rows at a
+// time, runs `go` with the plan and joins the column sums.
+template <typename A, typename Go>
+static acd_status run_norm_grad(acd_ctx *ctx, const NormGradArgs &a, int64_t grid, int sub, cudaStream_t s, Go go) {
   const int64_t rows = a.s.rows(), D = a.s.D;
-  int64_t grid = (int64_t)ctx->sm_count * resident_blocks(reinterpret_cast<const void *>(kern), BLOCK, 0);
   GradPlan p{};
   p.per = a.per;
   p.groups = rows / a.per;
   p.parts = grid / p.groups;
-  if (p.parts > (p.per + BLOCK / TPR - 1) / (BLOCK / TPR)) p.parts = (p.per + BLOCK / TPR - 1) / (BLOCK / TPR);
+  if (p.parts > (p.per + sub - 1) / sub) p.parts = (p.per + sub - 1) / sub;
   if (p.parts < 1) p.parts = 1;
   if (grid > p.groups * p.parts) grid = p.groups * p.parts;
   const bool gate_part = a.d_gate && p.parts > 1;
@@ -615,7 +850,7 @@ static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool
   p.gate = a.d_gate ? (gate_part ? gate : a.d_gate) : nullptr;
   p.gate_sd = gate_part ? 1 : a.gate_sd;
   p.gate_su = gate_part ? D : a.gate_sg;
-  kern<<<(unsigned)grid, BLOCK, 0, s>>>(a, p);
+  ACD_TRY(go(grid, p));
   JoinArgs<A> j{};
   j.D = D;
   j.src[0] = pre;
@@ -634,6 +869,45 @@ static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool
   return ACD_OK;
 }
 
+template <typename T, int TPR>
+static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool whole, cudaStream_t s) {
+  constexpr int BLOCK = TPR < 256 ? 256 : TPR;
+  auto kern = whole ? k_norm_grad_vec<T, TPR, true> : k_norm_grad_vec<T, TPR, false>;
+  const int64_t grid = (int64_t)ctx->sm_count * resident_blocks(reinterpret_cast<const void *>(kern), BLOCK, 0);
+  return run_norm_grad<typename AccOf<T>::type>(ctx, a, grid, BLOCK / TPR, s, [&](int64_t blocks, const GradPlan &p) {
+    kern<<<(unsigned)blocks, BLOCK, 0, s>>>(a, p);
+    return ACD_OK;
+  });
+}
+
+template <typename T, int TPR>
+static acd_status launch_norm_grad_ring(acd_ctx *ctx, const NormGradArgs &a, int CL, cudaStream_t s) {
+  auto kern = k_norm_grad_ring<T, TPR>;
+  const int resident = TPR <= 256 ? 2 : 1;
+  // stages: an SM's shared memory, some KB aside for each block
+  int stages = (228 / resident - 6) * 1024 / (4 * TPR * 16);
+  if (stages > kRingMost) stages = kRingMost;
+  const int dyn = stages * 4 * TPR * 16;
+  ACD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn));
+  return run_norm_grad<typename AccOf<T>::type>(
+      ctx, a, (int64_t)ctx->sm_count * resident / CL, 1, s, [&](int64_t clusters, const GradPlan &p) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(clusters * CL), 1, 1);
+        cfg.blockDim = dim3(TPR + 32, 1, 1);
+        cfg.dynamicSmemBytes = dyn;
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = CL;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        ACD_CUDA(cudaLaunchKernelEx(&cfg, kern, a, p, stages, ctx->control));
+        return ACD_OK;
+      });
+}
+
 template <typename T>
 static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStream_t s) {
   using A = typename AccOf<T>::type;
@@ -642,6 +916,11 @@ static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStre
                      (!a.dh.p || whole_rows(a.dh, V)) && whole_rows(a.dy, V) && whole_rows(a.h, V) &&
                      whole_rows(a.b, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
   const int64_t pieces = (a.s.D + V - 1) / V;
+  // rows of 2 KB and more are worth a bulk copy each
+  if (whole && pieces > 128 && pieces <= 512 * kRingMost) {
+    if (pieces <= 256) return launch_norm_grad_ring<T, 256>(ctx, a, 1, s);
+    return launch_norm_grad_ring<T, 512>(ctx, a, (int)((pieces + 511) / 512), s);
+  }
   if (pieces <= 1024) {
     if (pieces <= 32) return launch_norm_grad_vec<T, 32>(ctx, a, whole, s);
     if (pieces <= 128) return launch_norm_grad_vec<T, 128>(ctx, a, whole, s);

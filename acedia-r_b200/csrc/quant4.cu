@@ -494,6 +494,7 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
     }
   }
   if (C == 1) return;
+  __syncwarp();
   // the blocks of a cluster hold sums over different inputs of the same outputs
   cluster.sync();
   const int mb = blockIdx.x / C, r0 = rank * kRowsPerBlock / C, rows = (rank + 1) * kRowsPerBlock / C - r0;

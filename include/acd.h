@@ -166,7 +166,8 @@ acd_status acd_ctx_set_allocator(acd_ctx *ctx, acd_alloc_fn alloc, acd_free_fn f
  * 1 = the scan's look-back wait expired, 2 = a wait of the TMA transpose
  * pipeline expired, 3 = the TMA load wait of the cluster softmax expired,
  * 4 = the row softmax's wait for a lane group's statistics expired, 5 = the
- * 4-bit product's wait for its weights expired. */
+ * 4-bit product's wait for its weights expired, 6 = a wait of the residual
+ * norm's gradient for its rows expired. */
 acd_status acd_ctx_check(acd_ctx *ctx, acd_stream stream, int32_t *code);
 /* Test hook for the bounded look-back wait of the scan: when `tile` >= 0,
  * the scan kernel's tile with that index never publishes its prefix, so the
