@@ -85,6 +85,41 @@ struct Pk<double> {
 __device__ __forceinline__ Pk<double> pmul(Pk<double> a, Pk<double> b) { return {a.v * b.v}; }
 __device__ __forceinline__ Pk<double> pfma(Pk<double> a, Pk<double> b, Pk<double> c) { return {fma(a.v, b.v, c.v)}; }
 
+// V elements as they lie in memory; float16 pairs as words, so that
+// they take no more registers than bytes until they are widened.
+template <typename T, int V>
+struct Piece {
+  Vec<T, V> d;
+  template <typename A>
+  __device__ __forceinline__ void widen(A *f) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = to_acc(d.v[j]);
+  }
+  __device__ __forceinline__ void set(int j, T x) { d.v[j] = x; }
+};
+template <int V>
+struct Half2Piece {
+  Vec<uint32_t, V / 2> d;
+  __device__ __forceinline__ void widen(float *f) const {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&d.v[j / 2]));
+      f[j] = p.x;
+      f[j + 1] = p.y;
+    }
+  }
+  __device__ __forceinline__ void set(int j, __half x) {
+    const uint32_t h = __half_as_ushort(x);
+    d.v[j / 2] = j % 2 ? (d.v[j / 2] & 0xFFFFu) | h << 16 : (d.v[j / 2] & 0xFFFF0000u) | h;
+  }
+};
+template <>
+struct Piece<__half, 2> : Half2Piece<2> {};
+template <>
+struct Piece<__half, 4> : Half2Piece<4> {};
+template <>
+struct Piece<__half, 8> : Half2Piece<8> {};
+
 // A tensor as rows: element d of row r = l + L*o lies at p + l*sl + d*sd + o*so.
 struct Rows {
   void *p = nullptr;

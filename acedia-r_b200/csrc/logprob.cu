@@ -68,41 +68,6 @@ struct LpMath<double> {
   static __device__ __forceinline__ double min2(double a, double b) { return fmin(a, b); }
 };
 
-// V neighbouring logits as they lie in memory; float16 pairs as words, so that
-// they take no more registers than bytes until they are widened.
-template <typename T, int V>
-struct Piece {
-  Vec<T, V> d;
-  template <typename A>
-  __device__ __forceinline__ void widen(A *f) const {
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = to_acc(d.v[j]);
-  }
-  __device__ __forceinline__ void set(int j, T x) { d.v[j] = x; }
-};
-template <int V>
-struct Half2Piece {
-  Vec<uint32_t, V / 2> d;
-  __device__ __forceinline__ void widen(float *f) const {
-#pragma unroll
-    for (int j = 0; j < V; j += 2) {
-      const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&d.v[j / 2]));
-      f[j] = p.x;
-      f[j + 1] = p.y;
-    }
-  }
-  __device__ __forceinline__ void set(int j, __half x) {
-    const uint32_t h = __half_as_ushort(x);
-    d.v[j / 2] = j % 2 ? (d.v[j / 2] & 0xFFFFu) | h << 16 : (d.v[j / 2] & 0xFFFF0000u) | h;
-  }
-};
-template <>
-struct Piece<__half, 2> : Half2Piece<2> {};
-template <>
-struct Piece<__half, 4> : Half2Piece<4> {};
-template <>
-struct Piece<__half, 8> : Half2Piece<8> {};
-
 // m starts at the lowest finite value, so that -Inf - m is -Inf and never NaN:
 // a part of -Inf only keeps S = 0.  floor_z keeps T free of 0 * Inf.  A NaN
 // logit, and +Inf (Inf - Inf), make S NaN; the maximum passes over NaN.

@@ -224,25 +224,24 @@ __device__ __forceinline__ int column(int tid, int n, int j) {
   return WHOLE ? (n * TPR + tid) * V + j : (n * V + j) * TPR + tid;
 }
 
-template <typename T, typename A, int V, int TPR, bool WHOLE>
-__device__ __forceinline__ void load_cols(const T *x, int64_t sd, int tid, int n, int D, A *out) {
-  if (WHOLE) {
-    const int first = column<V, TPR, true>(tid, n, 0);
-    if (first < D) {
-      const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(x + first);
-#pragma unroll
-      for (int j = 0; j < V; ++j) out[j] = to_acc(v.v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) out[j] = A(0);
-    }
-  } else {
+template <typename T, int V, int TPR, bool WHOLE>
+__device__ __forceinline__ Piece<T, V> fetch_cols(const T *x, int64_t sd, int tid, int n, int D) {
+  Piece<T, V> p;
+  if (WHOLE && column<V, TPR, true>(tid, n, 0) < D)
+    p = *reinterpret_cast<const Piece<T, V> *>(x + column<V, TPR, true>(tid, n, 0));
+  if (!WHOLE || column<V, TPR, true>(tid, n, 0) >= D) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int d = column<V, TPR, false>(tid, n, j);
-      out[j] = d < D ? to_acc(x[d * sd]) : A(0);
+      const int d = column<V, TPR, WHOLE>(tid, n, j);
+      p.set(j, !WHOLE && d < D ? x[d * sd] : (T)0.0f);
     }
   }
+  return p;
+}
+
+template <typename T, typename A, int V, int TPR, bool WHOLE>
+__device__ __forceinline__ void load_cols(const T *x, int64_t sd, int tid, int n, int D, A *out) {
+  fetch_cols<T, V, TPR, WHOLE>(x, sd, tid, n, D).widen(out);
 }
 
 template <typename T, typename A, int V, int TPR, bool WHOLE>
@@ -469,9 +468,11 @@ __device__ __forceinline__ void store_sums(A *dst, int64_t sd, int tid, int D, c
   }
 }
 
-// V columns a thread, TPR threads a row; the column sums stay in registers.
+// V columns a thread, TPR threads a row; the column sums stay in registers.  The
+// next row is under way while one is worked on.
 template <typename T, int TPR, bool WHOLE>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_grad_vec(NormGradArgs a, GradPlan plan) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 256 || sizeof(T) == 8 ? 1 : 2)
+    k_norm_grad_vec(NormGradArgs a, GradPlan plan) {
   using A = typename AccOf<T>::type;
   using P = Pk<A>;
   constexpr int V = 16 / sizeof(T), BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR, M = V / P::N;
@@ -497,27 +498,44 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_grad_vec(NormGra
     P tb[M];
 #pragma unroll
     for (int j = 0; j < M; ++j) tb[j] = P::all(A(0));
-    for (int64_t rr = r0; rr < r1; rr += RPB) {
+    struct {
+      Piece<T, V> dh, dy, h, b;
+      A rh, rb;
+    } cur, next;
+    auto fetch = [&](int64_t rr, auto &x) {
       const bool ok = rr + sub < r1;
       const int64_t row = ok ? rr + sub : r0;
       const int n = ok ? D : 0;
+      if (a.dh.p) x.dh = fetch_cols<T, V, TPR, WHOLE>(row_ptr<T>(a.dh, row, a.s.L), a.dh.sd, tid, 0, n);
+      x.dy = fetch_cols<T, V, TPR, WHOLE>(row_ptr<T>(a.dy, row, a.s.L), a.dy.sd, tid, 0, n);
+      x.h = fetch_cols<T, V, TPR, WHOLE>(row_ptr<T>(a.h, row, a.s.L), a.h.sd, tid, 0, n);
+      x.b = fetch_cols<T, V, TPR, WHOLE>(row_ptr<T>(a.b, row, a.s.L), a.b.sd, tid, 0, n);
+      x.rh = ok ? static_cast<const A *>(a.rstd_h)[row] : A(0);
+      x.rb = post && ok ? static_cast<const A *>(a.rstd_b)[row] : A(1);
+    };
+    if (r0 < r1) fetch(r0, cur);
+    for (int64_t rr = r0; rr < r1; rr += RPB) {
+      if (rr + RPB < r1) fetch(rr + RPB, next);
       A dh[V], dy[V], h[V], b[V], s[3];
 #pragma unroll
       for (int j = 0; j < V; ++j) dh[j] = A(0);
-      if (a.dh.p) load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dh, row, a.s.L), a.dh.sd, tid, 0, n, dh);
-      load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dy, row, a.s.L), a.dy.sd, tid, 0, n, dy);
-      load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.h, row, a.s.L), a.h.sd, tid, 0, n, h);
-      load_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.b, row, a.s.L), a.b.sd, tid, 0, n, b);
-      const A rh = ok ? static_cast<const A *>(a.rstd_h)[row] : A(0);
-      const A rb = post && ok ? static_cast<const A *>(a.rstd_b)[row] : A(1);
+      if (a.dh.p) cur.dh.widen(dh);
+      cur.dy.widen(dy);
+      cur.h.widen(h);
+      cur.b.widen(b);
       GradCols<A, V> p;
-      p.begin(dh, dy, h, b, wp, f, rh, rb, s);
+      p.begin(dh, dy, h, b, wp, f, cur.rh, cur.rb, s);
       row_sum<A, 3, TPR>(s, sh[flip]);
       flip ^= 1;
-      p.end(s, inv, rh, rb, alpha, post, f, pre, tb, dh, dy);
-      store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dr, row, a.s.L), a.dr.sd, tid, 0, n, dh);
-      store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.db, row, a.s.L), a.db.sd, tid, 0, n, dy);
+      p.end(s, inv, cur.rh, cur.rb, alpha, post, f, pre, tb, dh, dy);
+      if (rr + sub < r1) {
+        store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dr, rr + sub, a.s.L), a.dr.sd, tid, 0, D, dh);
+        store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.db, rr + sub, a.s.L), a.db.sd, tid, 0, D, dy);
+      }
+      cur = next;
     }
+    // (read again: they are wanted once a unit only)
+    load_operands<T, A, V, TPR, WHOLE>(a, r0, tid, D, wo, g, f);
 #pragma unroll
     for (int j = 0; j < M; ++j) {
       pst[j] = pfma(P::from(g + j * P::N), tb[j], pst[j]);
@@ -923,6 +941,7 @@ static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStre
   }
   if (pieces <= 1024) {
     if (pieces <= 32) return launch_norm_grad_vec<T, 32>(ctx, a, whole, s);
+    if (pieces <= 64) return launch_norm_grad_vec<T, 64>(ctx, a, whole, s);
     if (pieces <= 128) return launch_norm_grad_vec<T, 128>(ctx, a, whole, s);
     if (pieces <= 256) return launch_norm_grad_vec<T, 256>(ctx, a, whole, s);
     if (pieces <= 512) return launch_norm_grad_vec<T, 512>(ctx, a, whole, s);
