@@ -432,13 +432,13 @@ struct GradCols {
 
 // The operands that stay while the gate row does: w_pre, and f = gate w_post.
 template <typename T, typename A, int V, int TPR, bool WHOLE>
-__device__ __forceinline__ void load_operands(const NormGradArgs &a, int64_t row, int tid, int D, A (&wo)[V], A (&g)[V],
+__device__ __forceinline__ void load_operands(const NormGradArgs &a, int64_t row, int tid, int n, int D, A (&wo)[V], A (&g)[V],
                                               Pk<A> (&f)[V / Pk<A>::N]) {
 #pragma unroll
   for (int j = 0; j < V; ++j) wo[j] = g[j] = A(1);
-  if (a.w_post) load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.w_post), 1, tid, 0, D, wo);
+  if (a.w_post) load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.w_post), 1, tid, n, D, wo);
   if (a.gate)
-    load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + row / a.per * a.gate_sg, a.gate_sd, tid, 0, D, g);
+    load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + row / a.per * a.gate_sg, a.gate_sd, tid, n, D, g);
 #pragma unroll
   for (int j = 0; j < V / Pk<A>::N; ++j)
     f[j] = pmul(Pk<A>::from(wo + j * Pk<A>::N), Pk<A>::from(g + j * Pk<A>::N));
@@ -460,10 +460,10 @@ __device__ __forceinline__ void add_subs(A (&acc)[V], A (*join)[V]) {
 }
 
 template <typename A, int V, int TPR, bool WHOLE>
-__device__ __forceinline__ void store_sums(A *dst, int64_t sd, int tid, int D, const A (&v)[V]) {
+__device__ __forceinline__ void store_sums(A *dst, int64_t sd, int tid, int n, int D, const A (&v)[V]) {
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int d = column<V, TPR, WHOLE>(tid, 0, j);
+    const int d = column<V, TPR, WHOLE>(tid, n, j);
     if (d < D) dst[d * sd] = v[j];
   }
 }
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
   for (int64_t u = blockIdx.x; u < plan.groups * plan.parts; u += gridDim.x) {
     int64_t r0, r1;
     unit_rows(plan, u, r0, r1);
-    load_operands<T, A, V, TPR, WHOLE>(a, r0, tid, D, wo, g, f);
+    load_operands<T, A, V, TPR, WHOLE>(a, r0, tid, 0, D, wo, g, f);
     P tb[M];
 #pragma unroll
     for (int j = 0; j < M; ++j) tb[j] = P::all(A(0));
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
       cur = next;
     }
     // (read again: they are wanted once a unit only)
-    load_operands<T, A, V, TPR, WHOLE>(a, r0, tid, D, wo, g, f);
+    load_operands<T, A, V, TPR, WHOLE>(a, r0, tid, 0, D, wo, g, f);
 #pragma unroll
     for (int j = 0; j < M; ++j) {
       pst[j] = pfma(P::from(g + j * P::N), tb[j], pst[j]);
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
     }
     if (plan.gate) {
       add_subs<A, V, TPR, RPB>(c, join);
-      if (sub == 0) store_sums<A, V, TPR, WHOLE>(static_cast<A *>(plan.gate) + u * plan.gate_su, plan.gate_sd, tid, D, c);
+      if (sub == 0) store_sums<A, V, TPR, WHOLE>(static_cast<A *>(plan.gate) + u * plan.gate_su, plan.gate_sd, tid, 0, D, c);
     }
   }
 #pragma unroll
@@ -553,25 +553,29 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
 #pragma unroll
     for (int j = 0; j < M; ++j) (w ? pst[j] : pre[j]).to(c + j * P::N);
     add_subs<A, V, TPR, RPB>(c, join);
-    if (sub == 0) store_sums<A, V, TPR, WHOLE>(dst + (int64_t)blockIdx.x * D, 1, tid, D, c);
+    if (sub == 0) store_sums<A, V, TPR, WHOLE>(dst + (int64_t)blockIdx.x * D, 1, tid, 0, D, c);
   }
 }
 
 // The same with rows brought in by bulk copies through a ring of stages, so that
-// several rows are under way while one is worked on (without it the loads of a
-// row waited for its two halves: 470 us on 16384 x 4096 float16).  A cluster of
-// CL blocks divides the columns of wider rows, each block of TPR compute threads
-// and a warp that issues the copies; the rows' sums then go to the other blocks
-// by asynchronous stores that count on a barrier there.
+// several rows are under way while one is worked on.  A row stays in shared
+// memory: it is read once for its sums and once more for its gradients, which
+// leaves the registers to the column sums of NV pieces a thread and allows two
+// blocks on an SM, whose barriers then overlap (one block of 512 threads with
+// the row in registers: 220 us on 16384 x 4096 float16; two of 512 with 64
+// registers a thread: 369 us).  A cluster of CL blocks divides the columns of wider rows; the rows'
+// sums go to the other blocks by asynchronous stores that count on a barrier
+// there.
 constexpr uint64_t kRingWaitNs = 1000000000ull;  // 1 s
 constexpr int kRingWaitCode = 6;
-constexpr int kRingMost = 8;  // stages, blocks of a cluster
+constexpr int kRingStages = 3;
+constexpr int kRingCluster = 8;
 
 template <typename A>
 struct RingShared {
-  uint64_t full[kRingMost], empty[kRingMost], joined[2];
-  A part[2][32][4];             // the warps' sums
-  A other[2][kRingMost][4];     // the blocks' sums
+  uint64_t full[kRingStages], joined[2];
+  A part[2][32][4];                             // the warps' sums
+  alignas(16) A other[2][kRingCluster][4];      // the blocks' sums, sent 16 bytes at a time
   int abort;
 };
 
@@ -592,25 +596,27 @@ __device__ __forceinline__ void send16(const void *at, const uint64_t *bar, int 
                : "memory");
 }
 
-template <typename T, int TPR>
-__global__ void __launch_bounds__(TPR + 32, TPR <= 256 ? 2 : 1) k_norm_grad_ring(NormGradArgs a, GradPlan plan, int stages, Control *control) {
+constexpr int kRingThreads = 256;
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_ring(NormGradArgs a, GradPlan plan,
+                                                                                  Control *control) {
+  constexpr int TPR = kRingThreads;
   using A = typename AccOf<T>::type;
   using P = Pk<A>;
-  constexpr int V = 16 / sizeof(T), M = V / P::N, NW = TPR / 32;
-  extern __shared__ __align__(128) unsigned char ring[];  // [stage][dy, h, b, dh][TPR * 16 bytes]
+  constexpr int V = 16 / sizeof(T), M = V / P::N, NW = TPR / 32, N = kRingStages;
+  extern __shared__ __align__(128) unsigned char ring[];  // [stage][dy, h, b, dh][NV * TPR * 16 bytes]
   __shared__ RingShared<A> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t cid = blockIdx.x / CL, nclusters = gridDim.x / CL;
+  const int64_t cid = blockIdx.x / CL, nclusters = gridDim.x / CL, units = plan.groups * plan.parts;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
-  const int c0 = rank * TPR * V;  // this block's columns
-  const int D = (int)a.s.D - c0 < TPR * V ? (int)a.s.D - c0 : TPR * V;
-  const int64_t units = plan.groups * plan.parts;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < stages; ++i) {
-      mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], NW);
-    }
+  constexpr int W = NV * TPR * V, ROW = NV * TPR * 16;  // columns of a block, bytes of its part of a row
+  const int c0 = rank * W;
+  const int D = (int)a.s.D - c0 < W ? (int)a.s.D - c0 : W;
+  const bool post = a.w_post != nullptr;
+  if (tid == 0) {
+    for (int i = 0; i < N; ++i) mbar_init(&sh.full[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&sh.joined[i], 1);
     sh.abort = 0;
     mbar_init_fence();
@@ -619,151 +625,178 @@ __global__ void __launch_bounds__(TPR + 32, TPR <= 256 ? 2 : 1) k_norm_grad_ring
     cluster.sync();
   else
     __syncthreads();
-  if (warp == NW) {
-    if (lane == 0) {
-      const uint32_t bytes = D * (uint32_t)sizeof(T);
-      int n = 0, slot = 0;
-      uint32_t phase = 1;
-      bool go = true;
-      for (int64_t u = cid; go && u < units; u += nclusters) {
-        int64_t r0, r1;
-        unit_rows(plan, u, r0, r1);
-        for (int64_t row = r0; row < r1; ++row, ++n) {
-          if (n >= stages &&
-              !mbar_wait_thread(&sh.empty[slot], phase, &sh.abort, control, kRingWaitCode, kRingWaitNs)) {
-            go = false;
-            break;
-          }
-          unsigned char *st = ring + (size_t)slot * 4 * TPR * 16;
-          mbar_arrive_expect_tx(&sh.full[slot], bytes * (a.dh.p ? 4 : 3));
-          bulk_load(st, row_ptr<T>(a.dy, row, a.s.L) + c0, bytes, &sh.full[slot]);
-          bulk_load(st + TPR * 16, row_ptr<T>(a.h, row, a.s.L) + c0, bytes, &sh.full[slot]);
-          bulk_load(st + 2 * TPR * 16, row_ptr<T>(a.b, row, a.s.L) + c0, bytes, &sh.full[slot]);
-          if (a.dh.p) bulk_load(st + 3 * TPR * 16, row_ptr<T>(a.dh, row, a.s.L) + c0, bytes, &sh.full[slot]);
-          if (++slot == stages) {
-            slot = 0;
-            phase ^= 1u;
-          }
-        }
+  // thread 0 walks ahead over the rows of this block's units and issues their copies
+  int64_t fu = cid, frow = 0, fend = 0;
+  int issued = 0;
+  if (fu < units) unit_rows(plan, fu, frow, fend);
+  auto issue = [&]() {
+    while (frow >= fend) {
+      fu += nclusters;
+      if (fu >= units) return;
+      unit_rows(plan, fu, frow, fend);
+    }
+    uint64_t *bar = &sh.full[issued % N];
+    unsigned char *st = ring + (size_t)(issued % N) * 4 * ROW;
+    const uint32_t bytes = D * (uint32_t)sizeof(T);
+    mbar_arrive_expect_tx(bar, bytes * (a.dh.p ? 4 : 3));
+    bulk_load(st, row_ptr<T>(a.dy, frow, a.s.L) + c0, bytes, bar);
+    bulk_load(st + ROW, row_ptr<T>(a.h, frow, a.s.L) + c0, bytes, bar);
+    bulk_load(st + 2 * ROW, row_ptr<T>(a.b, frow, a.s.L) + c0, bytes, bar);
+    if (a.dh.p) bulk_load(st + 3 * ROW, row_ptr<T>(a.dh, frow, a.s.L) + c0, bytes, bar);
+    ++frow;
+    ++issued;
+  };
+  if (tid == 0)
+    for (int i = 0; i < N && fu < units; ++i) issue();
+
+  const A alpha = (A)a.alpha, inv = A(1) / (A)a.s.D;
+  NormGradArgs slice = a;  // operands from this block's first column on
+  slice.w_pre = static_cast<const T *>(a.w_pre) + c0;
+  if (a.w_post) slice.w_post = static_cast<const T *>(a.w_post) + c0;
+  if (a.gate) slice.gate = static_cast<const T *>(a.gate) + c0;
+  Piece<T, V> wraw[NV];
+  P f[NV][M], pre[NV][M], tb[NV][M];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    wraw[v] = fetch_cols<T, V, TPR, true>(static_cast<const T *>(slice.w_pre), 1, tid, v, D);
+#pragma unroll
+    for (int j = 0; j < M; ++j) pre[v][j] = P::all(A(0));
+  }
+  int n = 0, slot = 0, flip = 0;
+  uint32_t phase = 0, joined = 0;
+  bool dead = false, first = true;
+  for (int64_t u = cid; u < units; u += nclusters) {
+    int64_t r0, r1;
+    unit_rows(plan, u, r0, r1);
+    A wo[V], g[V], c[V];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      load_operands<T, A, V, TPR, true>(slice, r0, tid, v, D, wo, g, f[v]);
+#pragma unroll
+      for (int j = 0; j < M; ++j) tb[v][j] = P::all(A(0));
+    }
+    A rh_next = r0 < r1 ? static_cast<const A *>(a.rstd_h)[r0] : A(0);
+    A rb_next = r0 < r1 && post ? static_cast<const A *>(a.rstd_b)[r0] : A(1);
+    for (int64_t row = r0; row < r1; ++row, ++n) {
+      const A rh = rh_next, rb = rb_next;
+      if (row + 1 < r1) {
+        rh_next = static_cast<const A *>(a.rstd_h)[row + 1];
+        if (post) rb_next = static_cast<const A *>(a.rstd_b)[row + 1];
       }
-      // given up: the copies in flight land before the block may end
-      if (*reinterpret_cast<volatile int *>(&sh.abort))
-        for (int q = n > stages ? n - stages : 0; q < n; ++q)
-          mbar_wait_bounded(&sh.full[q % stages], (uint32_t)(q / stages) & 1u, kRingWaitNs);
-    }
-  } else {
-    const bool post = a.w_post != nullptr;
-    const A alpha = (A)a.alpha, inv = A(1) / (A)a.s.D;
-    const bool mine = tid * V < D;
-    NormGradArgs slice = a;  // operands from this block's first column on
-    slice.w_pre = static_cast<const T *>(a.w_pre) + c0;
-    if (a.w_post) slice.w_post = static_cast<const T *>(a.w_post) + c0;
-    if (a.gate) slice.gate = static_cast<const T *>(a.gate) + c0;
-    P wp[M], f[M], pre[M], pst[M];
-    A c[V];
-    load_cols<T, A, V, TPR, true>(static_cast<const T *>(slice.w_pre), 1, tid, 0, D, c);
-#pragma unroll
-    for (int j = 0; j < M; ++j) {
-      wp[j] = P::from(c + j * P::N);
-      pre[j] = pst[j] = P::all(A(0));
-    }
-    int slot = 0, flip = 0;
-    uint32_t phase = 0, joined = 0;
-    bool dead = false;
-    for (int64_t u = cid; u < units; u += nclusters) {
-      int64_t r0, r1;
-      unit_rows(plan, u, r0, r1);
-      A wo[V], g[V];
-      load_operands<T, A, V, TPR, true>(slice, r0, tid, D, wo, g, f);
-      P tb[M];
-#pragma unroll
-      for (int j = 0; j < M; ++j) tb[j] = P::all(A(0));
-      A rh_next = r0 < r1 ? static_cast<const A *>(a.rstd_h)[r0] : A(0);
-      A rb_next = r0 < r1 && post ? static_cast<const A *>(a.rstd_b)[r0] : A(1);
-      for (int64_t row = r0; row < r1; ++row) {
-        const A rh = rh_next, rb = rb_next;
-        if (row + 1 < r1) {
-          rh_next = static_cast<const A *>(a.rstd_h)[row + 1];
-          if (post) rb_next = static_cast<const A *>(a.rstd_b)[row + 1];
-        }
-        // once given up, the warps go on without waiting: all of them reach the barriers
-        dead = dead || !mbar_wait_warp(&sh.full[slot], phase, &sh.abort, control, kRingWaitCode, kRingWaitNs);
-        const unsigned char *st = ring + (size_t)slot * 4 * TPR * 16;
-        A dh[V], dy[V], h[V], b[V], s[3];
+      // once given up, the warps go on without waiting: all of them reach the barriers
+      dead = dead || !mbar_wait_warp(&sh.full[slot], phase, &sh.abort, control, kRingWaitCode, kRingWaitNs);
+      const unsigned char *st = ring + (size_t)slot * 4 * ROW;
+      A s[3] = {A(0), A(0), A(0)};
+      GradCols<A, V> p;
+      auto read = [&](int v, A (&sums)[3]) {
+        A dh[V], dy[V], h[V], b[V];
+        P wp[M];
 #pragma unroll
         for (int j = 0; j < V; ++j) dh[j] = A(0);
-        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st), 1, tid, 0, D, dy);
-        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + TPR * 16), 1, tid, 0, D, h);
-        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + 2 * TPR * 16), 1, tid, 0, D, b);
-        if (a.dh.p) load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + 3 * TPR * 16), 1, tid, 0, D, dh);
+        wraw[v].widen(dy);
+#pragma unroll
+        for (int j = 0; j < M; ++j) wp[j] = P::from(dy + j * P::N);
+        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st), 1, tid, v, D, dy);
+        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + ROW), 1, tid, v, D, h);
+        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + 2 * ROW), 1, tid, v, D, b);
+        if (a.dh.p) load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + 3 * ROW), 1, tid, v, D, dh);
+        p.begin(dh, dy, h, b, wp, f[v], rh, rb, sums);
+      };
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        A part[3];
+        read(v, part);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) s[j] += part[j];
+      }
+#pragma unroll
+      for (int q = 16; q; q >>= 1)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) s[j] += __shfl_xor_sync(~0u, s[j], q);
+      if (lane == 0)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) sh.part[flip][warp][j] = s[j];
+      __syncthreads();
+      // the row before has been read to the end by everyone: its stage is free
+      if (tid == 0 && n > 0 && fu < units && !dead) issue();
+#pragma unroll
+      for (int j = 0; j < 3; ++j) s[j] = lane < NW ? sh.part[flip][lane][j] : A(0);
+#pragma unroll
+      for (int q = NW / 2; q; q >>= 1)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) s[j] += __shfl_xor_sync(~0u, s[j], q);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) s[j] = __shfl_sync(~0u, s[j], 0);
+      if (CL > 1) {
+        if (warp == 0 && lane < CL) {
+          if (lane == 0) mbar_arrive_expect_tx(&sh.joined[flip], CL * 4 * (uint32_t)sizeof(A));
+          // the block's sums to every block, its own included
+          if constexpr (sizeof(A) == 4) {
+            send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, pack2(s[0], s[1]), pack2(s[2], 0.0f));
+          } else {
+            send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, __double_as_longlong(s[0]),
+                   __double_as_longlong(s[1]));
+            send16(&sh.other[flip][rank][2], &sh.joined[flip], lane, __double_as_longlong(s[2]), 0);
+          }
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.empty[slot]);
-        if (++slot == stages) {
-          slot = 0;
-          phase ^= 1u;
+        dead = dead || !mbar_wait_warp(&sh.joined[flip], joined, &sh.abort, control, kRingWaitCode, kRingWaitNs);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          s[j] = A(0);
+          for (int q = 0; q < CL; ++q) s[j] += sh.other[flip][q][j];
         }
-        GradCols<A, V> p;
-        p.begin(dh, dy, h, b, wp, f, rh, rb, s);
-#pragma unroll
-        for (int q = 16; q; q >>= 1)
-#pragma unroll
-          for (int j = 0; j < 3; ++j) s[j] += __shfl_xor_sync(~0u, s[j], q);
-        if (lane == 0)
-#pragma unroll
-          for (int j = 0; j < 3; ++j) sh.part[flip][warp][j] = s[j];
-        asm volatile("bar.sync 1, %0;" ::"n"(TPR) : "memory");
-#pragma unroll
-        for (int j = 0; j < 3; ++j) s[j] = lane < NW ? sh.part[flip][lane][j] : A(0);
-#pragma unroll
-        for (int q = NW / 2; q; q >>= 1)
-#pragma unroll
-          for (int j = 0; j < 3; ++j) s[j] += __shfl_xor_sync(~0u, s[j], q);
-#pragma unroll
-        for (int j = 0; j < 3; ++j) s[j] = __shfl_sync(~0u, s[j], 0);
-        if (CL > 1) {
-          if (warp == 0 && lane < CL) {
-            if (lane == 0) mbar_arrive_expect_tx(&sh.joined[flip], CL * 4 * (uint32_t)sizeof(A));
-            // the block's sums to every block, its own included
-            if constexpr (sizeof(A) == 4) {
-              send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, pack2(s[0], s[1]), pack2(s[2], 0.0f));
-            } else {
-              send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, __double_as_longlong(s[0]),
-                     __double_as_longlong(s[1]));
-              send16(&sh.other[flip][rank][2], &sh.joined[flip], lane, __double_as_longlong(s[2]), 0);
-            }
-          }
-          dead = dead || !mbar_wait_warp(&sh.joined[flip], joined, &sh.abort, control, kRingWaitCode, kRingWaitNs);
-#pragma unroll
-          for (int j = 0; j < 3; ++j) {
-            s[j] = A(0);
-            for (int q = 0; q < CL; ++q) s[j] += sh.other[flip][q][j];
-          }
-          joined ^= (uint32_t)flip;  // both barriers have had a phase
-        }
-        flip ^= 1;
-        p.end(s, inv, rh, rb, alpha, post, f, pre, tb, dh, dy);
-        if (mine) {
-          store_cols<T, A, V, TPR, true>(row_ptr<T>(a.dr, row, a.s.L) + c0, 1, tid, 0, D, dh);
-          store_cols<T, A, V, TPR, true>(row_ptr<T>(a.db, row, a.s.L) + c0, 1, tid, 0, D, dy);
-        }
+        joined ^= (uint32_t)flip;  // both barriers have had a phase
       }
+      flip ^= 1;
+      asm volatile("" ::: "memory");  // read again, not kept
 #pragma unroll
-      for (int j = 0; j < M; ++j) {
-        pst[j] = pfma(P::from(g + j * P::N), tb[j], pst[j]);
-        pmul(P::from(wo + j * P::N), tb[j]).to(c + j * P::N);
+      for (int v = 0; v < NV; ++v) {
+        A again[3], dr[V], db[V];
+        read(v, again);
+        p.end(s, inv, rh, rb, alpha, post, f[v], pre[v], tb[v], dr, db);
+        store_cols<T, A, V, TPR, true>(row_ptr<T>(a.dr, row, a.s.L) + c0, 1, tid, v, D, dr);
+        store_cols<T, A, V, TPR, true>(row_ptr<T>(a.db, row, a.s.L) + c0, 1, tid, v, D, db);
       }
-      if (plan.gate)
-        store_sums<A, V, TPR, true>(static_cast<A *>(plan.gate) + u * plan.gate_su + c0 * plan.gate_sd, plan.gate_sd, tid, D, c);
+      if (++slot == N) {
+        slot = 0;
+        phase ^= 1u;
+      }
     }
+    // (wo and g read again rather than kept over the rows; the sums of w_post go
+    // straight to this block's row of the partial sums)
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      A *dst = static_cast<A *>(w ? plan.post : plan.pre);
-      if (!dst) continue;
+    for (int v = 0; v < NV; ++v) {
+      load_operands<T, A, V, TPR, true>(slice, r0, tid, v, D, wo, g, f[v]);
+      if (plan.post && column<V, TPR, true>(tid, v, 0) < D) {
+        A *dst = static_cast<A *>(plan.post) + cid * a.s.D + c0 + column<V, TPR, true>(tid, v, 0);
 #pragma unroll
-      for (int j = 0; j < M; ++j) (w ? pst[j] : pre[j]).to(c + j * P::N);
-      store_sums<A, V, TPR, true>(dst + cid * a.s.D + c0, 1, tid, D, c);
+        for (int j = 0; j < M; ++j) pmul(P::from(g + j * P::N), tb[v][j]).to(c + j * P::N);
+#pragma unroll
+        for (int j = 0; j < V; ++j) dst[j] = first ? c[j] : dst[j] + c[j];
+      }
+      if (plan.gate) {
+#pragma unroll
+        for (int j = 0; j < M; ++j) pmul(P::from(wo + j * P::N), tb[v][j]).to(c + j * P::N);
+        store_sums<A, V, TPR, true>(static_cast<A *>(plan.gate) + u * plan.gate_su + c0 * plan.gate_sd, plan.gate_sd, tid, v,
+                                    D, c);
+      }
+    }
+    first = false;
+  }
+  if (plan.pre) {
+    A c[V];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int j = 0; j < M; ++j) pre[v][j].to(c + j * P::N);
+      store_sums<A, V, TPR, true>(static_cast<A *>(plan.pre) + cid * a.s.D + c0, 1, tid, v, D, c);
     }
   }
+  // given up: the copies in flight land before the block may end
+  if (dead && tid == 0)
+    for (int q = issued > N ? issued - N : 0; q < issued; ++q)
+      mbar_wait_bounded(&sh.full[q % N], (uint32_t)(q / N) & 1u, kRingWaitNs);
   __syncwarp();
   if (CL > 1) cluster.sync();  // no block leaves while another may still write to it
 }
@@ -898,20 +931,16 @@ static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool
   });
 }
 
-template <typename T, int TPR>
+template <typename T, int NV>
 static acd_status launch_norm_grad_ring(acd_ctx *ctx, const NormGradArgs &a, int CL, cudaStream_t s) {
-  auto kern = k_norm_grad_ring<T, TPR>;
-  const int resident = TPR <= 256 ? 2 : 1;
-  // stages: an SM's shared memory, some KB aside for each block
-  int stages = (228 / resident - 6) * 1024 / (4 * TPR * 16);
-  if (stages > kRingMost) stages = kRingMost;
-  const int dyn = stages * 4 * TPR * 16;
+  auto kern = k_norm_grad_ring<T, NV>;
+  const int dyn = kRingStages * 4 * NV * kRingThreads * 16;
   ACD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn));
   return run_norm_grad<typename AccOf<T>::type>(
-      ctx, a, (int64_t)ctx->sm_count * resident / CL, 1, s, [&](int64_t clusters, const GradPlan &p) {
+      ctx, a, (int64_t)ctx->sm_count * (NV == 1 ? 3 : 2) / CL, 1, s, [&](int64_t clusters, const GradPlan &p) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(clusters * CL), 1, 1);
-        cfg.blockDim = dim3(TPR + 32, 1, 1);
+        cfg.blockDim = dim3(kRingThreads, 1, 1);
         cfg.dynamicSmemBytes = dyn;
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
@@ -921,7 +950,7 @@ static acd_status launch_norm_grad_ring(acd_ctx *ctx, const NormGradArgs &a, int
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        ACD_CUDA(cudaLaunchKernelEx(&cfg, kern, a, p, stages, ctx->control));
+        ACD_CUDA(cudaLaunchKernelEx(&cfg, kern, a, p, ctx->control));
         return ACD_OK;
       });
 }
@@ -935,9 +964,9 @@ static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStre
                      whole_rows(a.b, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
   const int64_t pieces = (a.s.D + V - 1) / V;
   // rows of 2 KB and more are worth a bulk copy each
-  if (whole && pieces > 128 && pieces <= 512 * kRingMost) {
-    if (pieces <= 256) return launch_norm_grad_ring<T, 256>(ctx, a, 1, s);
-    return launch_norm_grad_ring<T, 512>(ctx, a, (int)((pieces + 511) / 512), s);
+  if (whole && pieces > 128 && pieces <= 512 * kRingCluster) {
+    if (pieces <= 256) return launch_norm_grad_ring<T, 1>(ctx, a, 1, s);
+    return launch_norm_grad_ring<T, 2>(ctx, a, (int)((pieces + 511) / 512), s);
   }
   if (pieces <= 1024) {
     if (pieces <= 32) return launch_norm_grad_vec<T, 32>(ctx, a, whole, s);
