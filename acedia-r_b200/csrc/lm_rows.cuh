@@ -96,6 +96,11 @@ struct Piece {
     for (int j = 0; j < V; ++j) f[j] = to_acc(d.v[j]);
   }
   __device__ __forceinline__ void set(int j, T x) { d.v[j] = x; }
+  template <typename A>
+  __device__ __forceinline__ void round(const A *f) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) d.v[j] = from_acc<T, A>(f[j]);
+  }
 };
 template <int V>
 struct Half2Piece {
@@ -106,6 +111,13 @@ struct Half2Piece {
       const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&d.v[j / 2]));
       f[j] = p.x;
       f[j + 1] = p.y;
+    }
+  }
+  __device__ __forceinline__ void round(const float *f) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const __half2 h = __floats2half2_rn(f[j], f[j + 1]);
+      d.v[j / 2] = *reinterpret_cast<const uint32_t *>(&h);
     }
   }
   __device__ __forceinline__ void set(int j, __half x) {
@@ -132,10 +144,17 @@ struct RowShape {
   __host__ __device__ int64_t rows() const { return L * O; }
 };
 
+// (Rows are counted in 31 bits: a 64-bit division is many times a 32-bit one.  The
+// branch keeps the division, some 100 cycles, away from rows that need none.)
 template <typename T>
 __device__ __forceinline__ T *row_ptr(const Rows &v, int64_t r, int64_t L) {
-  const int64_t o = L == 1 ? r : r / L, l = L == 1 ? 0 : r - o * L;
-  return static_cast<T *>(v.p) + l * v.sl + o * v.so;
+  int64_t at = r * v.so;
+  if (L != 1) {
+    asm volatile("" ::: "memory");  // not turned into a selection of both results
+    const uint32_t o = (uint32_t)r / (uint32_t)L, l = (uint32_t)r - o * (uint32_t)L;
+    at = l * v.sl + o * v.so;
+  }
+  return static_cast<T *>(v.p) + at;
 }
 
 // Views `d` around `axis`; the axes before it, and those after it, must each
@@ -216,9 +235,7 @@ __device__ __forceinline__ void load_piece(const T *x, int64_t sd, int first, in
   if (V == 1) {
     out[0] = first < D ? to_acc(x[first * sd]) : fill;
   } else if (first >= 0 && first + V <= D) {
-    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(x + first);
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = to_acc(v.v[j]);
+    reinterpret_cast<const Piece<T, V> *>(x + first)->widen(out);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) out[j] = first + j >= 0 && first + j < D ? to_acc(x[first + j]) : fill;
@@ -228,10 +245,9 @@ __device__ __forceinline__ void load_piece(const T *x, int64_t sd, int first, in
 template <typename T, typename A, int V>
 __device__ __forceinline__ void store_piece(T *x, int64_t sd, int first, int D, const A *v) {
   if (V > 1 && first >= 0 && first + V <= D) {
-    Vec<T, V> w;
-#pragma unroll
-    for (int j = 0; j < V; ++j) w.v[j] = from_acc<T, A>(v[j]);
-    *reinterpret_cast<Vec<T, V> *>(x + first) = w;
+    Piece<T, V> w;
+    w.round(v);
+    *reinterpret_cast<Piece<T, V> *>(x + first) = w;
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)

@@ -322,7 +322,7 @@ struct RowResult {
     }
   }
   __device__ __forceinline__ void alternative(const LogprobArgs &a, int64_t r, int j, A v, int i) const {
-    const int64_t o = a.s.L == 1 ? r : r / a.s.L, l = r - o * a.s.L;
+    const int64_t o = (uint32_t)r / (uint32_t)a.s.L, l = r - o * a.s.L;
     const int64_t at = l + a.s.L * (j + a.k * o);
     const bool none = i == kNone;
     store_index(a.top_index, a.wide_index, at,

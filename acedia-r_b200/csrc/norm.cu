@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) k_norm_rows(NormArgs a) {
   for (int64_t row = blockIdx.x; row < a.s.rows(); row += gridDim.x) {
     const T *r = row_ptr<T>(a.r, row, a.s.L), *b = row_ptr<T>(a.b, row, a.s.L);
     T *h = row_ptr<T>(a.h, row, a.s.L), *y = row_ptr<T>(a.y, row, a.s.L);
-    const T *gate = a.gate ? static_cast<const T *>(a.gate) + row / a.per * a.gate_sg : nullptr;
+    const T *gate = a.gate ? static_cast<const T *>(a.gate) + (int64_t)((uint32_t)row / (uint32_t)a.per) * a.gate_sg : nullptr;
     A rb = 1;
     if (w_post) {
       A q = 0;
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) k_norm_grad_rows(NormGradArgs a) {
     T *dr = row_ptr<T>(a.dr, row, a.s.L), *db = row_ptr<T>(a.db, row, a.s.L);
     const T *dh = a.dh.p ? row_ptr<T>(a.dh, row, a.s.L) : nullptr, *dy = row_ptr<T>(a.dy, row, a.s.L);
     const T *h = row_ptr<T>(a.h, row, a.s.L), *b = row_ptr<T>(a.b, row, a.s.L);
-    const T *gate = a.gate ? static_cast<const T *>(a.gate) + row / a.per * a.gate_sg : nullptr;
+    const T *gate = a.gate ? static_cast<const T *>(a.gate) + (int64_t)((uint32_t)row / (uint32_t)a.per) * a.gate_sg : nullptr;
     const A rh = static_cast<const A *>(a.rstd_h)[row];
     const A rb = w_post ? static_cast<const A *>(a.rstd_b)[row] : A(1);
     A m1 = 0, m2 = 0;
@@ -249,10 +249,9 @@ __device__ __forceinline__ void store_cols(T *x, int64_t sd, int tid, int n, int
   if (WHOLE) {
     const int first = column<V, TPR, true>(tid, n, 0);
     if (first < D) {
-      Vec<T, V> w;
-#pragma unroll
-      for (int j = 0; j < V; ++j) w.v[j] = from_acc<T, A>(v[j]);
-      *reinterpret_cast<Vec<T, V> *>(x + first) = w;
+      Piece<T, V> w;
+      w.round(v);
+      *reinterpret_cast<Piece<T, V> *>(x + first) = w;
     }
   } else {
 #pragma unroll
@@ -293,12 +292,13 @@ __device__ __forceinline__ void row_sum(A (&v)[N], A *sh) {
   }
 }
 
-// TPR threads a row, NV pieces of V columns a thread; the row stays in registers between
-// the two sums.
+// TPR threads a row, NV pieces of V columns a thread; the row stays in registers
+// between the two sums.
 template <typename T, int TPR, int NV, bool WHOLE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) {
   using A = typename AccOf<T>::type;
-  constexpr int V = 16 / sizeof(T), BLOCK = TPR < 256 ? 256 : TPR;
+  using P = Pk<A>;
+  constexpr int V = 16 / sizeof(T), BLOCK = TPR < 256 ? 256 : TPR, M = V / P::N;
   __shared__ A sh[2][BLOCK / 32];
   const int64_t row = (int64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
   const bool ok = row < a.s.rows();  // whole warps: a row has at least one
@@ -307,55 +307,70 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) 
   const int D = ok ? (int)a.s.D : 0;
   const T *r = row_ptr<T>(a.r, rr, a.s.L), *b = row_ptr<T>(a.b, rr, a.s.L);
   const T *w_pre = static_cast<const T *>(a.w_pre), *w_post = static_cast<const T *>(a.w_post);
-  const A alpha = (A)a.alpha, eps = (A)a.eps, inv = A(1) / (A)a.s.D;
-  A bv[NV][V], rv[NV][V];
+  const A eps = (A)a.eps, inv = A(1) / (A)a.s.D;
+  Piece<T, V> br[NV], rr_[NV];
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    load_cols<T, A, V, TPR, WHOLE>(b, a.b.sd, tid, n, D, bv[n]);
-    load_cols<T, A, V, TPR, WHOLE>(r, a.r.sd, tid, n, D, rv[n]);
+    br[n] = fetch_cols<T, V, TPR, WHOLE>(b, a.b.sd, tid, n, D);
+    rr_[n] = fetch_cols<T, V, TPR, WHOLE>(r, a.r.sd, tid, n, D);
   }
-  A rb = 1;
-  if (w_post) {
-    A q[1] = {A(0)};
+  P h[NV][M];
+  A f[V];
+  auto sum_of_squares = [&]() {
+    P q = P::all(A(0));
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
-      for (int j = 0; j < V; ++j) q[0] = fma_a(bv[n][j], bv[n][j], q[0]);
-    row_sum<A, 1, TPR>(q, sh[0]);
-    rb = rsqrt_a(q[0] * inv + eps);
-  }
-  A q[1] = {A(0)};
+      for (int j = 0; j < M; ++j) q = pfma(h[n][j], h[n][j], q);
+    return q.sum();
+  };
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    A w[V];
-    if (w_post) {
-      load_cols<T, A, V, TPR, WHOLE>(w_post, 1, tid, n, D, w);
+    br[n].widen(f);
 #pragma unroll
-      for (int j = 0; j < V; ++j) bv[n][j] *= rb * w[j];
-    }
-    if (a.gate) {
-      load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + rr / a.per * a.gate_sg, a.gate_sd, tid, n, D, w);
+    for (int j = 0; j < M; ++j) h[n][j] = P::from(f + j * P::N);
+  }
+  A rb = 1;
+  if (w_post) {
+    A q[1] = {sum_of_squares()};
+    row_sum<A, 1, TPR>(q, sh[0]);
+    rb = rsqrt_a(q[0] * inv + eps);
+    const P prb = P::all(rb);
 #pragma unroll
-      for (int j = 0; j < V; ++j) bv[n][j] *= w[j];
-    }
+    for (int n = 0; n < NV; ++n) {
+      load_cols<T, A, V, TPR, WHOLE>(w_post, 1, tid, n, D, f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      bv[n][j] = fma_a(alpha, rv[n][j], bv[n][j]);
-      q[0] = fma_a(bv[n][j], bv[n][j], q[0]);
+      for (int j = 0; j < M; ++j) h[n][j] = pmul(pmul(h[n][j], prb), P::from(f + j * P::N));
     }
   }
+  const P alpha = P::all((A)a.alpha);
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    if (a.gate) {
+      load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + (int64_t)((uint32_t)rr / (uint32_t)a.per) * a.gate_sg, a.gate_sd, tid, n, D, f);
+#pragma unroll
+      for (int j = 0; j < M; ++j) h[n][j] = pmul(h[n][j], P::from(f + j * P::N));
+    }
+    rr_[n].widen(f);
+#pragma unroll
+    for (int j = 0; j < M; ++j) h[n][j] = pfma(alpha, P::from(f + j * P::N), h[n][j]);
+  }
+  A q[1] = {sum_of_squares()};
   row_sum<A, 1, TPR>(q, sh[1]);
   const A rh = rsqrt_a(q[0] * inv + eps);
   if (!ok) return;
-  T *h = row_ptr<T>(a.h, rr, a.s.L), *y = row_ptr<T>(a.y, rr, a.s.L);
+  const P prh = P::all(rh);
+  T *ho = row_ptr<T>(a.h, rr, a.s.L), *yo = row_ptr<T>(a.y, rr, a.s.L);
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    A w[V];
-    load_cols<T, A, V, TPR, WHOLE>(w_pre, 1, tid, n, D, w);
-    store_cols<T, A, V, TPR, WHOLE>(h, a.h.sd, tid, n, D, bv[n]);
+    A y[V];
+    load_cols<T, A, V, TPR, WHOLE>(w_pre, 1, tid, n, D, f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[j] *= bv[n][j] * rh;
-    store_cols<T, A, V, TPR, WHOLE>(y, a.y.sd, tid, n, D, w);
+    for (int j = 0; j < M; ++j) pmul(pmul(h[n][j], prh), P::from(f + j * P::N)).to(y + j * P::N);
+    store_cols<T, A, V, TPR, WHOLE>(yo, a.y.sd, tid, n, D, y);
+#pragma unroll
+    for (int j = 0; j < M; ++j) h[n][j].to(f + j * P::N);
+    store_cols<T, A, V, TPR, WHOLE>(ho, a.h.sd, tid, n, D, f);
   }
   if (tid == 0) {
     if (a.rstd_h) static_cast<A *>(a.rstd_h)[row] = rh;
@@ -383,48 +398,55 @@ __device__ __forceinline__ void unit_rows(const GradPlan &p, int64_t u, int64_t 
 }
 
 // V columns of a row's gradient, in two steps around the row's sums.  With
-//   q = d_h + rs_h d_y w_pre,  hn = h rs_h,  bn = b rs_b,  f = gate w_post
-// t = q - rs_h hn m1, so that mean(u w_post bn) = mean(q f bn) - m1 rs_h
-// mean(hn f bn) comes from the same pass as m1 = mean(d_y w_pre hn): one
-// reduction a row.  sum t bn is what the gradients of the gate (times w_post)
-// and of w_post (times gate) have in common while the gate row stays the same.
+//   u = d_y w_pre,  q = d_h + rs_h u,  f = gate w_post,  e = f b
+// and the sums s0 = sum u h, s1 = sum q e, s2 = sum h e over the row,
+//   m1 = mean(d_y w_pre hn) = rs_h s0 / D,  t = q - rs_h^2 m1 h / rs_h,
+//   mean(u w_post bn) = rs_b (s1 - rs_h m1 s2) / D:
+// one reduction a row.  sum t bn is what the gradients of the gate (times
+// w_post) and of w_post (times gate) have in common while the gate row stays.
 template <typename A, int V>
 struct GradCols {
   using P = Pk<A>;
   static constexpr int M = V / P::N;
-  P q[M], hn[M], bn[M], dy[M];
-  __device__ __forceinline__ void begin(const A (&dh)[V], const A (&dyv)[V], const A (&h)[V], const A (&b)[V],
-                                        const P (&wp)[M], const P (&f)[M], A rh, A rb, A (&s)[3]) {
-    const P prh = P::all(rh), prb = P::all(rb);
-    P s0 = P::all(A(0)), s1 = s0, s2 = s0;
+  P q[M], h[M], b[M], dy[M];
+  __device__ __forceinline__ void take(const A (&dhv)[V], const A (&dyv)[V], const A (&hv)[V], const A (&bv)[V],
+                                       const P (&wp)[M], A rh) {
+    const P prh = P::all(rh);
 #pragma unroll
     for (int j = 0; j < M; ++j) {
       dy[j] = P::from(dyv + j * P::N);
-      hn[j] = pmul(P::from(h + j * P::N), prh);
-      bn[j] = pmul(P::from(b + j * P::N), prb);
-      const P u = pmul(dy[j], wp[j]), e = pmul(f[j], bn[j]);
-      q[j] = pfma(prh, u, P::from(dh + j * P::N));
-      s0 = pfma(u, hn[j], s0);
+      h[j] = P::from(hv + j * P::N);
+      b[j] = P::from(bv + j * P::N);
+      q[j] = pfma(prh, pmul(dy[j], wp[j]), P::from(dhv + j * P::N));
+    }
+  }
+  __device__ __forceinline__ void sums(const P (&wp)[M], const P (&f)[M], A (&s)[3]) const {
+    P s0 = P::all(A(0)), s1 = s0, s2 = s0;
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const P e = pmul(f[j], b[j]);
+      s0 = pfma(pmul(dy[j], wp[j]), h[j], s0);
       s1 = pfma(q[j], e, s1);
-      s2 = pfma(hn[j], e, s2);
+      s2 = pfma(h[j], e, s2);
     }
     s[0] = s0.sum();
     s[1] = s1.sum();
     s[2] = s2.sum();
   }
   // s: the row's sums; adds to pre and tb, leaves the gradients in dr and db.
-  __device__ __forceinline__ void end(const A (&s)[3], A inv, A rh, A rb, A alpha, bool post, const P (&f)[M], P (&pre)[M],
-                                      P (&tb)[M], A (&dr)[V], A (&db)[V]) {
-    const A m1 = s[0] * inv * rh;
-    const P nm1 = P::all(-m1), nm2 = P::all(post ? -(s[1] - m1 * s[2]) * inv : A(0)), prb = P::all(rb), pal = P::all(alpha);
+  __device__ __forceinline__ void finish(const A (&s)[3], A inv, A rh, A rb, A alpha, bool post, const P (&f)[M],
+                                         P (&pre)[M], P (&tb)[M], A (&dr)[V], A (&db)[V]) const {
+    const A m1 = rh * (s[0] * inv) * rh;  // times rs_h once more: t = q - (rs_h m1) h
+    const P nm1 = P::all(-m1 * rh), prh = P::all(rh), prb = P::all(rb), pal = P::all(alpha);
+    const P nm2 = P::all(post ? -(rb * inv) * (s[1] - m1 * rh * s[2]) : A(0));
 #pragma unroll
     for (int j = 0; j < M; ++j) {
-      const P t = pfma(hn[j], nm1, q[j]);
-      pre[j] = pfma(dy[j], hn[j], pre[j]);
-      tb[j] = pfma(t, bn[j], tb[j]);
+      const P t = pfma(h[j], nm1, q[j]), bn = pmul(b[j], prb);
+      pre[j] = pfma(dy[j], pmul(h[j], prh), pre[j]);
+      tb[j] = pfma(t, bn, tb[j]);
       pmul(pal, t).to(dr + j * P::N);
       P x = pmul(t, f[j]);
-      if (post) x = pmul(pfma(bn[j], nm2, x), prb);
+      if (post) x = pmul(pfma(bn, nm2, x), prb);
       x.to(db + j * P::N);
     }
   }
@@ -438,7 +460,7 @@ __device__ __forceinline__ void load_operands(const NormGradArgs &a, int64_t row
   for (int j = 0; j < V; ++j) wo[j] = g[j] = A(1);
   if (a.w_post) load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.w_post), 1, tid, n, D, wo);
   if (a.gate)
-    load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + row / a.per * a.gate_sg, a.gate_sd, tid, n, D, g);
+    load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + (int64_t)((uint32_t)row / (uint32_t)a.per) * a.gate_sg, a.gate_sd, tid, n, D, g);
 #pragma unroll
   for (int j = 0; j < V / Pk<A>::N; ++j)
     f[j] = pmul(Pk<A>::from(wo + j * Pk<A>::N), Pk<A>::from(g + j * Pk<A>::N));
@@ -524,10 +546,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
       cur.h.widen(h);
       cur.b.widen(b);
       GradCols<A, V> p;
-      p.begin(dh, dy, h, b, wp, f, cur.rh, cur.rb, s);
+      p.take(dh, dy, h, b, wp, cur.rh);
+      p.sums(wp, f, s);
       row_sum<A, 3, TPR>(s, sh[flip]);
       flip ^= 1;
-      p.end(s, inv, cur.rh, cur.rb, alpha, post, f, pre, tb, dh, dy);
+      p.finish(s, inv, cur.rh, cur.rb, alpha, post, f, pre, tb, dh, dy);
       if (rr + sub < r1) {
         store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dr, rr + sub, a.s.L), a.dr.sd, tid, 0, D, dh);
         store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.db, rr + sub, a.s.L), a.db.sd, tid, 0, D, dy);
@@ -621,6 +644,9 @@ __global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_rin
     sh.abort = 0;
     mbar_init_fence();
   }
+  // what no copy writes
+  for (int i = tid; i < N * 4 * NV * TPR; i += TPR)
+    if (i % (NV * TPR) * V >= D) reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0, 0, 0, 0);
   if (CL > 1)
     cluster.sync();
   else
@@ -688,24 +714,27 @@ __global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_rin
       const unsigned char *st = ring + (size_t)slot * 4 * ROW;
       A s[3] = {A(0), A(0), A(0)};
       GradCols<A, V> p;
-      auto read = [&](int v, A (&sums)[3]) {
+      P wp[M];
+      auto read = [&](int v) {
         A dh[V], dy[V], h[V], b[V];
-        P wp[M];
 #pragma unroll
         for (int j = 0; j < V; ++j) dh[j] = A(0);
         wraw[v].widen(dy);
 #pragma unroll
         for (int j = 0; j < M; ++j) wp[j] = P::from(dy + j * P::N);
-        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st), 1, tid, v, D, dy);
-        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + ROW), 1, tid, v, D, h);
-        load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + 2 * ROW), 1, tid, v, D, b);
-        if (a.dh.p) load_cols<T, A, V, TPR, true>(reinterpret_cast<const T *>(st + 3 * ROW), 1, tid, v, D, dh);
-        p.begin(dh, dy, h, b, wp, f[v], rh, rb, sums);
+        // (beyond the row's end a stage holds zeros)
+        const Piece<T, V> *at = reinterpret_cast<const Piece<T, V> *>(st) + v * TPR + tid;
+        at[0].widen(dy);
+        at[NV * TPR].widen(h);
+        at[2 * NV * TPR].widen(b);
+        if (a.dh.p) at[3 * NV * TPR].widen(dh);
+        p.take(dh, dy, h, b, wp, rh);
       };
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         A part[3];
-        read(v, part);
+        read(v);
+        p.sums(wp, f[v], part);
 #pragma unroll
         for (int j = 0; j < 3; ++j) s[j] += part[j];
       }
@@ -752,9 +781,9 @@ __global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_rin
       asm volatile("" ::: "memory");  // read again, not kept
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        A again[3], dr[V], db[V];
-        read(v, again);
-        p.end(s, inv, rh, rb, alpha, post, f[v], pre[v], tb[v], dr, db);
+        A dr[V], db[V];
+        read(v);
+        p.finish(s, inv, rh, rb, alpha, post, f[v], pre[v], tb[v], dr, db);
         store_cols<T, A, V, TPR, true>(row_ptr<T>(a.dr, row, a.s.L) + c0, 1, tid, v, D, dr);
         store_cols<T, A, V, TPR, true>(row_ptr<T>(a.db, row, a.s.L) + c0, 1, tid, v, D, db);
       }
@@ -801,8 +830,8 @@ __global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_rin
   if (CL > 1) cluster.sync();  // no block leaves while another may still write to it
 }
 
-// Column sums of `n` partial rows: 32 columns a block, its 8 warps split the
-// rows and are added in order.
+// Column sums of `n` partial rows: a block takes 32 W columns, its 8 warps split
+// the rows and are added in order.
 template <typename A>
 struct JoinArgs {
   const A *src[3];
@@ -811,27 +840,41 @@ struct JoinArgs {
   int64_t D;
 };
 
-template <typename A>
+template <typename A, int W>
 __global__ void __launch_bounds__(256) k_norm_grad_join(JoinArgs<A> a) {
-  __shared__ A sh[8][32];
+  __shared__ Vec<A, W> sh[8][32];
   // blockIdx.y: 0 pre, 1 post, 2 + g gate row g
   const int w = blockIdx.y < 2 ? blockIdx.y : 2;
   const int64_t g = w == 2 ? blockIdx.y - 2 : 0;
   if (!a.dst[w]) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t d = (int64_t)blockIdx.x * 32 + lane, n = a.n[w];
-  A s = 0;
-  if (d < a.D) {
+  const int64_t d = ((int64_t)blockIdx.x * 32 + lane) * W, n = a.n[w];
+  Vec<A, W> s;
+#pragma unroll
+  for (int j = 0; j < W; ++j) s.v[j] = A(0);
+  if (d < a.D) {  // W divides D
     const A *p = a.src[w] + g * n * a.D + d;
-#pragma unroll 8
-    for (int64_t i = warp; i < n; i += 8) s += p[i * a.D];
+    constexpr int U = 12;  // rows in flight
+    for (int64_t i = warp; i < n; i += 8 * U) {
+      Vec<A, W> x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + 8 * u < n) x[u] = *reinterpret_cast<const Vec<A, W> *>(p + (i + 8 * u) * a.D);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + 8 * u < n)
+#pragma unroll
+          for (int j = 0; j < W; ++j) s.v[j] += x[u].v[j];
+    }
   }
   sh[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && d < a.D) {
-    for (int q = 1; q < 8; ++q) s += sh[q][lane];
-    a.dst[w][d * a.sd[w] + g * a.sg[w]] = s;
-  }
+  if (warp == 0 && d < a.D)
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      for (int q = 1; q < 8; ++q) s.v[j] += sh[q][lane].v[j];
+      a.dst[w][(d + j) * a.sd[w] + g * a.sg[w]] = s.v[j];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -866,12 +909,18 @@ static acd_status launch_norm(acd_ctx *ctx, const NormArgs &a, cudaStream_t s) {
                      whole_rows(a.y, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
   const int64_t pieces = (a.s.D + V - 1) / V;
   if (pieces <= 4096) {
+    // a warp a row up to four pieces a lane, then two to four pieces a thread
     if (pieces <= 32) return launch_norm_vec<T, 32, 1>(a, whole, s);
     if (pieces <= 64) return launch_norm_vec<T, 32, 2>(a, whole, s);
+    if (pieces <= 96) return launch_norm_vec<T, 32, 3>(a, whole, s);
+    if (pieces <= 128) return launch_norm_vec<T, 32, 4>(a, whole, s);
     if (pieces <= 256) return launch_norm_vec<T, 128, 2>(a, whole, s);
+    if (pieces <= 384) return launch_norm_vec<T, 128, 3>(a, whole, s);
     if (pieces <= 512) return launch_norm_vec<T, 256, 2>(a, whole, s);
+    if (pieces <= 768) return launch_norm_vec<T, 256, 3>(a, whole, s);
     if (pieces <= 1024) return launch_norm_vec<T, 512, 2>(a, whole, s);
-    if (pieces <= 2048) return launch_norm_vec<T, 1024, 2>(a, whole, s);
+    if (pieces <= 1536) return launch_norm_vec<T, 512, 3>(a, whole, s);
+    if (pieces <= 2048) return launch_norm_vec<T, 512, 4>(a, whole, s);
     return launch_norm_vec<T, 1024, 4>(a, whole, s);
   }
   const int grid = persistent_grid(ctx, k_norm_rows<T>, 256, 0, a.s.rows());
@@ -915,8 +964,13 @@ static acd_status run_norm_grad(acd_ctx *ctx, const NormGradArgs &a, int64_t gri
   j.sd[0] = j.sd[1] = 1;
   j.sd[2] = a.gate_sd;
   j.sg[2] = a.gate_sg;
-  if (j.dst[0] || j.dst[1] || j.dst[2])
-    k_norm_grad_join<A><<<dim3((unsigned)((D + 31) / 32), (unsigned)(2 + (gate_part ? p.groups : 0))), 256, 0, s>>>(j);
+  if (j.dst[0] || j.dst[1] || j.dst[2]) {
+    const unsigned rows_y = (unsigned)(2 + (gate_part ? p.groups : 0));
+    if (D % 2 == 0)
+      k_norm_grad_join<A, 2><<<dim3((unsigned)((D / 2 + 31) / 32), rows_y), 256, 0, s>>>(j);
+    else
+      k_norm_grad_join<A, 1><<<dim3((unsigned)((D + 31) / 32), rows_y), 256, 0, s>>>(j);
+  }
   return ACD_OK;
 }
 
