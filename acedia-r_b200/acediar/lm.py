@@ -6,7 +6,9 @@ computation is a call into libacediar_b200.so on the current torch stream.  The
 formulas and every rule on masked, missing and empty values stand beside the C
 functions in include/acd.h.  The reference has none of these operators.
 """
+import ctypes
 import numbers
+import struct
 from collections import namedtuple
 
 import torch
@@ -35,8 +37,31 @@ def _new(shape, dtype, device):
     return t
 
 
+_pack_desc = struct.Struct("Pq%dq%dqii" % (L.MAX_DIMS, L.MAX_DIMS)).pack  # the layout of acd_desc
+assert struct.calcsize("Pq%dq%dqii" % (L.MAX_DIMS, L.MAX_DIMS)) == ctypes.sizeof(L.Desc)
+_pad = [(0,) * (L.MAX_DIMS - n) for n in range(L.MAX_DIMS + 1)]
+_functions = {}
+
+
+def _call(name):
+    """The C function, taking descriptors as bytes: these calls have up to 14 of
+    them, and a ctypes structure costs three times as much to make."""
+    f = _functions.get(name)
+    if f is None:
+        lib = L.lib()
+        f = lib[name]  # a function object of its own
+        f.argtypes = [ctypes.c_char_p if t is ctypes.POINTER(L.Desc) else t for t in getattr(lib, name).argtypes]
+        f.restype = ctypes.c_int32
+        _functions[name] = f
+    return f
+
+
 def _desc(t):
-    return None if t is None else t.desc()
+    if t is None:
+        return None
+    n = len(t.shape)
+    pad = _pad[n]
+    return _pack_desc(t.storage.data_ptr(), t.offset, *t.shape, *pad, *t.strides, *pad, n, L.DTYPE_CODES[t.dtype])
 
 
 def _dense(t):
@@ -46,6 +71,8 @@ def _dense(t):
 
 
 def _axis0(x, axis):
+    if type(axis) is int and 1 <= axis <= len(x.shape):
+        return axis - 1
     if not isinstance(axis, numbers.Number) or axis != int(axis) or axis < 1 or axis > x.ndims:
         raise ValueError("axis must be a single positive integer within tensor dimensions")
     return int(axis) - 1
@@ -86,13 +113,13 @@ def token_logprob(logits, tokens=None, axis=1, scale=1.0, top=0):
     if top:
         tshape = logits.shape[:a] + (int(top),) + logits.shape[a + 1:]
         index, top_logprob = _new(tshape, "int64", dev), _new(tshape, st, dev)
-    f, c, s = L.lib().acd_token_logprob, context(), _stream()
+    f, c, s = _call("acd_token_logprob"), context(), _stream()
     out = [_desc(t) for t in (logprob, entropy, lse, index, top_logprob)]
     tokens = _dense(tokens)
-    r = f(c, *out, logits.desc(), _desc(tokens), a, scale, 1, s)
+    r = f(c, *out, _desc(logits), _desc(tokens), a, scale, 1, s)
     if r == _UNSUPPORTED and not logits.is_contiguous():
         logits = contiguous(logits)
-        r = f(c, *out, logits.desc(), _desc(tokens), a, scale, 1, s)
+        r = f(c, *out, _desc(logits), _desc(tokens), a, scale, 1, s)
     L.check(r, "token_logprob")
     return TokenLogprob(logprob, entropy, lse, index, top_logprob)
 
@@ -104,14 +131,14 @@ def token_logprob_grad(logits, tokens, logsumexp, entropy=None, d_logprob=None, 
     gradients with respect to its outputs (None: none).  inplace=True writes
     the gradient over the logits."""
     a = _axis0(logits, axis)
-    f, c, s = L.lib().acd_token_logprob_grad, context(), _stream()
+    f, c, s = _call("acd_token_logprob_grad"), context(), _stream()
     grad = logits if inplace else _new(logits.shape, logits.dtype, logits.device)
     rest = [_dense(t) for t in (logsumexp, entropy, d_logprob, d_entropy, d_logsumexp)]
     tokens = _dense(tokens)
-    r = f(c, grad.desc(), logits.desc(), _desc(tokens), a, scale, *[_desc(t) for t in rest], 1, s)
+    r = f(c, _desc(grad), _desc(logits), _desc(tokens), a, scale, *[_desc(t) for t in rest], 1, s)
     if r == _UNSUPPORTED and not inplace and not logits.is_contiguous():
         logits = contiguous(logits)
-        r = f(c, grad.desc(), logits.desc(), _desc(tokens), a, scale, *[_desc(t) for t in rest], 1, s)
+        r = f(c, _desc(grad), _desc(logits), _desc(tokens), a, scale, *[_desc(t) for t in rest], 1, s)
     L.check(r, "token_logprob_grad")
     return grad
 
@@ -136,9 +163,9 @@ def residual_norm(residual, block, w_pre, w_post=None, gate=None, axis=1, alpha=
     y = block if inplace else _new(block.shape, block.dtype, dev)
     rh = _new(shape, st, dev)
     rb = _new(shape, st, dev) if w_post is not None else None
-    L.check(L.lib().acd_residual_norm(context(), h.desc(), y.desc(), rh.desc(), _desc(rb), residual.desc(),
-                                      block.desc(), w_pre.desc(), _desc(w_post), _desc(gate), a, alpha, eps, _stream()),
-            "residual_norm")
+    L.check(_call("acd_residual_norm")(context(), _desc(h), _desc(y), _desc(rh), _desc(rb), _desc(residual),
+                                       _desc(block), _desc(w_pre), _desc(w_post), _desc(gate), a, alpha, eps,
+                                       _stream()), "residual_norm")
     return ResidualNorm(h, y, rh, rb)
 
 
@@ -155,9 +182,9 @@ def residual_norm_grad(d_h, d_y, h, block, rstd_h, rstd_block, w_pre, w_post=Non
     dr, db = _new(block.shape, block.dtype, dev), _new(block.shape, block.dtype, dev)
     like = lambda t: None if t is None else _new(t.shape, st, dev)  # noqa: E731
     dpre, dpost, dgate = like(w_pre), like(w_post), like(gate)
-    L.check(L.lib().acd_residual_norm_grad(
-        context(), dr.desc(), db.desc(), dpre.desc(), _desc(dpost), _desc(dgate), _desc(d_h), d_y.desc(), h.desc(),
-        block.desc(), rstd_h.desc(), _desc(rstd_block), w_pre.desc(), _desc(w_post), _desc(gate), a, alpha,
+    L.check(_call("acd_residual_norm_grad")(
+        context(), _desc(dr), _desc(db), _desc(dpre), _desc(dpost), _desc(dgate), _desc(d_h), _desc(d_y), _desc(h),
+        _desc(block), _desc(rstd_h), _desc(rstd_block), _desc(w_pre), _desc(w_post), _desc(gate), a, alpha,
         _stream()), "residual_norm_grad")
     return ResidualNormGrad(dr, db, dpre, dpost, dgate)
 
@@ -176,7 +203,7 @@ def quant4_encode(w, group=128, zeros=False, scale_dtype="float16"):
     q = _new((16 * -(-inner // 32), out), "int8", w.device)
     s = _new((-(-inner // group), out), sd, w.device)
     z = _new(s.shape, sd, w.device) if zeros else None
-    L.check(L.lib().acd_quant4_encode(context(), q.desc(), s.desc(), _desc(z), w.desc(), int(group), _stream()),
+    L.check(_call("acd_quant4_encode")(context(), _desc(q), _desc(s), _desc(z), _desc(w), int(group), _stream()),
             "quant4_encode")
     return Quant4(q, s, z)
 
@@ -192,6 +219,6 @@ def quant4_matvec(weights, scales, x, group=128, zeros=None, out_dtype=None):
     odt = x.dtype if out_dtype is None else _norm_dtype(out_dtype)
     weights, scales, zeros = _dense(weights), _dense(scales), _dense(zeros)
     out = _new((weights.shape[1],) + x.shape[1:], odt, x.device)
-    L.check(L.lib().acd_quant4_matvec(context(), out.desc(), weights.desc(), scales.desc(), _desc(zeros), x.desc(),
+    L.check(_call("acd_quant4_matvec")(context(), _desc(out), _desc(weights), _desc(scales), _desc(zeros), _desc(x),
                                       int(group), _stream()), "quant4_matvec")
     return out

@@ -277,6 +277,10 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 // shared memory (occupancy API, cached per kernel and launch shape).
 int resident_blocks(const void *kernel, int threads, size_t smem);
 
+// Lets `kernel` have `bytes` of dynamic shared memory on the context's device
+// (the driver is asked once for a kernel, device and size).
+acd_status allow_smem(const acd_ctx *ctx, const void *kernel, size_t bytes);
+
 // Persistent grid: as many blocks as are resident at once (a multiple of the
 // SM count), or fewer when there is less work.  A larger grid would run as a
 // second, partly filled wave.

@@ -126,6 +126,29 @@ int resident_blocks(const void *kernel, int threads, size_t smem) {
   return nb;
 }
 
+acd_status allow_smem(const acd_ctx *ctx, const void *kernel, size_t bytes) {
+  struct Entry {
+    const void *k;
+    int device;
+    size_t bytes;
+  };
+  static std::mutex mu;
+  static Entry entries[256];
+  static int used = 0;
+  std::lock_guard<std::mutex> lk(mu);
+  Entry *e = nullptr;
+  for (int i = 0; i < used; ++i)
+    if (entries[i].k == kernel && entries[i].device == ctx->device) e = &entries[i];
+  if (e && e->bytes >= bytes) return ACD_OK;
+  ACD_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (!e && used < 256) {
+    e = &entries[used++];
+    *e = Entry{kernel, ctx->device, 0};
+  }
+  if (e) e->bytes = bytes;
+  return ACD_OK;
+}
+
 acd_status get_counters(acd_ctx *ctx, size_t n, cudaStream_t stream, unsigned int **out) {
   ACD_TRY(get_zeroed(ctx, &ctx->counters, &ctx->counters_n, n, stream, "counter"));
   *out = ctx->counters;

@@ -989,7 +989,7 @@ template <typename T, int NV>
 static acd_status launch_norm_grad_ring(acd_ctx *ctx, const NormGradArgs &a, int CL, cudaStream_t s) {
   auto kern = k_norm_grad_ring<T, NV>;
   const int dyn = kRingStages * 4 * NV * kRingThreads * 16;
-  ACD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn));
+  ACD_TRY(allow_smem(ctx, reinterpret_cast<const void *>(kern), dyn));
   return run_norm_grad<typename AccOf<T>::type>(
       ctx, a, (int64_t)ctx->sm_count * (NV == 1 ? 3 : 2) / CL, 1, s, [&](int64_t clusters, const GradPlan &p) {
         cudaLaunchConfig_t cfg = {};
