@@ -1024,25 +1024,39 @@ __device__ __forceinline__ GradRow<A> grad_row(const LogprobGradArgs &a, int64_t
   return g;
 }
 
-template <typename A>
-__device__ __forceinline__ A grad_value(const GradRow<A> &g, A x, A c);
-template <>
-__device__ __forceinline__ float grad_value<float>(const GradRow<float> &g, float x, float c) {
-  using M = LpMath<float>;
-  const float d = M::floor_z(fmaf(c, x, -g.lse));  // p = 0 where d is below the floor: 0 log 0 = 0
-  return M::ex(d * 1.44269504088896341f) * fmaf(-g.a1, d, g.a0);
-}
-template <>
-__device__ __forceinline__ double grad_value<double>(const GradRow<double> &g, double x, double c) {
-  const double d = LpMath<double>::floor_z(fma(c, x, -g.lse));
-  return exp(d) * fma(-g.a1, d, g.a0);
+// N logits of one row (or, with G = N, of N rows side by side).
+template <typename A, int N, int G>
+__device__ __forceinline__ void grad_values(const GradRow<A> (&g)[G], A (&x)[N], A c) {
+  using M = LpMath<A>;
+  if constexpr (std::is_same<A, float>::value && N % 2 == 0) {
+    const uint64_t cc = pack2(c, c), l2e = pack2(1.44269504088896341f, 1.44269504088896341f);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const GradRow<A> &p = g[G == 1 ? 0 : j], &q = g[G == 1 ? 0 : j + 1];
+      float d0, d1, z0, z1;
+      unpack2(fma2(cc, pack2(x[j], x[j + 1]), pack2(-p.lse, -q.lse)), d0, d1);
+      d0 = M::floor_z(d0);  // p = 0 where d is below the floor: 0 log 0 = 0
+      d1 = M::floor_z(d1);
+      const uint64_t d = pack2(d0, d1);
+      unpack2(mul2(d, l2e), z0, z1);
+      unpack2(mul2(pack2(M::ex(z0), M::ex(z1)), fma2(pack2(-p.a1, -q.a1), d, pack2(p.a0, q.a0))), x[j], x[j + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const GradRow<A> &p = g[G == 1 ? 0 : j];
+      const A d = M::floor_z(fma_a(c, x[j], -p.lse));
+      const A e = std::is_same<A, float>::value ? M::ex(d * A(1.44269504088896341)) : M::ex(d);
+      x[j] = e * fma_a(-p.a1, d, p.a0);
+    }
+  }
 }
 
 // Rows along the axis: a warp takes U pieces a lane of one row, 16 bytes each
 // (V logits; the row may start and end inside a piece), reads them all and
 // then writes.  V = 1: any strides.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) k_logprob_grad_rows(LogprobGradArgs a, uint32_t segs, uint32_t tasks) {
+__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 2 : 5) k_logprob_grad_rows(LogprobGradArgs a, uint32_t segs, uint32_t tasks) {
   using A = typename AccOf<T>::type;
   constexpr int U = BatchU<T, V>::value;
   const int lane = threadIdx.x & 31;
@@ -1052,21 +1066,20 @@ __global__ void __launch_bounds__(256) k_logprob_grad_rows(LogprobGradArgs a, ui
     const uint32_t r = task / segs, seg = task - r * segs;
     const T *x = row_ptr<T>(a.x, r, a.s.L);
     T *out = row_ptr<T>(a.g, r, a.s.L);
-    const int base = (int)seg * (U * V * 32) - row_shift<T, V>(x);
-    A xs[U * V];
-#pragma unroll
-    for (int u = 0; u < U; ++u) load_piece<T, A, V>(x, a.x.sd, base + (u * 32 + lane) * V, D, A(-INFINITY), xs + u * V);
-    const GradRow<A> g = grad_row<A>(a, r);
+    const int shift = row_shift<T, V>(x), base = (int)seg * (U * V * 32) - shift;
+    Piece<T, V> raw[U];
+    load_batch<T, V, U>(x, a.x.sd, D, shift, (int)seg, raw);
+    const GradRow<A> g[1] = {grad_row<A>(a, r)};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int first = base + (u * 32 + lane) * V;
       A v[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = grad_value<A>(g, xs[u * V + j], c);
-      if (g.t >= first && g.t < first + V) {
+      raw[u].widen(v);
+      grad_values<A, V, 1>(g, v, c);
+      if (g[0].t >= first && g[0].t < first + V) {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (first + j == g.t) v[j] += g.gt;
+          if (first + j == g[0].t) v[j] += g[0].gt;
       }
       store_piece<T, A, V>(out, a.g.sd, first, D, v);
     }
@@ -1095,20 +1108,21 @@ __global__ void __launch_bounds__(256) k_logprob_grad_lanes(LogprobGradArgs a, i
   int64_t s = blockIdx.y * chunk;
   const int64_t s1 = s + chunk < a.s.D ? s + chunk : a.s.D;
   for (s += threadIdx.x >> bx_log2; s < s1; s += UN * by) {
-    Vec<T, V> w[UN];
+    Piece<T, V> w[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (s + u * by < s1) w[u] = *reinterpret_cast<const Vec<T, V> *>(x + (s + u * by) * a.x.sd);
+      if (s + u * by < s1) w[u] = *reinterpret_cast<const Piece<T, V> *>(x + (s + u * by) * a.x.sd);
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       if (s + u * by >= s1) break;
+      A v[V];
+      w[u].widen(v);
+      grad_values<A, V, V>(g, v, c);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        A v = grad_value<A>(g[j], to_acc(w[u].v[j]), c);
-        if (g[j].t == (int)(s + u * by)) v += g[j].gt;
-        w[u].v[j] = from_acc<T, A>(v);
-      }
-      *reinterpret_cast<Vec<T, V> *>(out + (s + u * by) * a.g.sd) = w[u];
+      for (int j = 0; j < V; ++j)
+        if (g[j].t == (int)(s + u * by)) v[j] += g[j].gt;
+      w[u].round(v);
+      *reinterpret_cast<Piece<T, V> *>(out + (s + u * by) * a.g.sd) = w[u];
     }
   }
 }
