@@ -55,7 +55,10 @@ __device__ __forceinline__ void store_f(void *p, bool half, int64_t i, float v) 
 //   y = sum_groups s sum (n - 8) x  +  sum_groups s (8 - z) sum x,
 // the second term from sums of x that are made once.  float32 activations are
 // split into three bfloat16 parts that hold all 24 bits, which go in as three
-// columns.
+// columns.  One instruction's columns (NT = 1) are prepared by each block for
+// itself, a segment of the inputs at a time; more columns would cost the blocks
+// more than their weights do (64 us of 10007 x 8200 with six float32 columns),
+// so a kernel of its own prepares those once and they come in with the weights.
 constexpr int kRowsPerBlock = 64;
 constexpr int kTileBytes = 128;                       // of one output: 256 inputs, 8 chunks of 32
 constexpr int kBoxBytes = kRowsPerBlock * kTileBytes;
@@ -66,7 +69,9 @@ constexpr int kQWaitCode = 5;
 struct Quant4Plan {
   int mblocks;         // blocks of 64 outputs
   int ktiles, tper;    // tiles of 256 inputs: in all, a block of a cluster (even, or all)
-  int seg;             // tiles whose activations are in shared memory at once
+  int stages;          // of the ring
+  int seg;             // tiles whose activations are in shared memory at once (NT = 1)
+  int xtile;           // bytes of a tile's activations and sums as k_quant4_x leaves them (NT > 1)
   int vectors;         // columns of x a block (gridDim.y blocks of them)
   int cols;            // matrix columns: vectors, or three for each
   int xcols;           // places for them: 2 more than a multiple of 4, whose 16-byte reads meet no bank twice
@@ -75,9 +80,7 @@ struct Quant4Plan {
   bool wide;           // a tile's scales are one aligned load
 };
 
-// Stages of the ring: with more columns their activations want the room.
-template <int NT>
-struct Q4Stages { static constexpr int value = NT == 1 ? 4 : 3; };
+constexpr int kMaxStages = 4;
 
 // Columns of x that 8 NT matrix columns hold.
 template <bool X16, int NT>
@@ -187,9 +190,8 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
   return r;
 }
 
-template <int STAGES>
 struct Quant4Shared {
-  uint64_t full[STAGES], empty[STAGES];
+  uint64_t full[kMaxStages], empty[kMaxStages];
   int abort;
 };
 
@@ -272,16 +274,27 @@ __device__ __forceinline__ float row_value(const float *red, int v) {
   return ZEROS ? y + red[8 * NT + v] : y;
 }
 
+// The activations of a tile and of a block's columns, as stage_x lays them out.
+template <bool X16, int NT, int SUB, bool ZEROS>
+__global__ void __launch_bounds__(256) k_quant4_x(Quant4Args a, Quant4Plan p, unsigned char *out) {
+  unsigned char *at = out + ((int64_t)blockIdx.y * p.ktiles + blockIdx.x) * p.xtile;
+  stage_x<X16, SUB, Q4Vectors<X16, NT>::value, ZEROS>(a, p, blockIdx.x, 1, blockIdx.y * p.vectors,
+                                                      reinterpret_cast<uint4 *>(at),
+                                                      reinterpret_cast<float *>(at + 512 * p.xcols));
+}
+
 template <bool X16, int NT, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ CUtensorMap map, Quant4Args a,
-                                                       Quant4Plan p, Control *control) {
+                                                       Quant4Plan p, const unsigned char *xpre, Control *control) {
+  constexpr bool PRE = NT > 1;
   constexpr int VS = Q4Vectors<X16, NT>::value, RED = SumsStride<8 * NT + (ZEROS ? VS : 0)>::value, SLOTS = 8 / SUB;
-  constexpr int kStages = Q4Stages<NT>::value;
   extern __shared__ unsigned char smem[];
-  __shared__ Quant4Shared<kStages> sh;
+  __shared__ Quant4Shared sh;
   // the swizzle goes by the address: stages start on 1024 bytes
   unsigned char *stages = smem + ((1024u - (smem_addr(smem) & 1023u)) & 1023u);
-  float *red = reinterpret_cast<float *>(stages + kStages * kStageBytes);  // [64][RED]
+  const int kStages = p.stages;
+  const uint32_t stride = PRE ? (uint32_t)(kStageBytes + 2 * p.xtile + 1023) & ~1023u : (uint32_t)kStageBytes;
+  float *red = reinterpret_cast<float *>(stages + kStages * stride);  // [64][RED]
   uint4 *xf = reinterpret_cast<uint4 *>(red + kRowsPerBlock * RED);
   float *sx = reinterpret_cast<float *>(xf + p.seg * 32 * p.xcols);
   cg::cluster_group cluster = cg::this_cluster();
@@ -316,8 +329,16 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
             break;
           }
           const bool two = 2 * i + 1 < nt;  // a tile past the range is not loaded
-          unsigned char *st = stages + slot * kStageBytes;
-          mbar_arrive_expect_tx(&sh.full[slot], two ? kStageBytes : kBoxBytes);
+          unsigned char *st = stages + slot * stride;
+          const uint32_t xbytes = PRE ? (two ? 2 : 1) * p.xtile : 0;
+          mbar_arrive_expect_tx(&sh.full[slot], (two ? kStageBytes : kBoxBytes) + xbytes);
+          if (PRE)
+            asm volatile(
+                "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                    smem_addr(st + kStageBytes)),
+                "l"(xpre + ((int64_t)blockIdx.y * p.ktiles + t0 + 2 * i) * p.xtile), "r"(xbytes),
+                "r"(smem_addr(&sh.full[slot]))
+                : "memory");
           tma_load_2d(st, &map, &sh.full[slot], (t0 + 2 * i) * kTileBytes, mb * kRowsPerBlock);
           if (two) tma_load_2d(st + kBoxBytes, &map, &sh.full[slot], (t0 + 2 * i + 1) * kTileBytes, mb * kRowsPerBlock);
         }
@@ -334,7 +355,7 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
     const uint32_t xstep = 4 * 16 * p.xcols;  // bytes of a chunk
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      xcol[n] = smem_addr(xf) + 16 * (t * p.xcols + (n * 8 + g < p.cols ? n * 8 + g : p.cols - 1));
+      xcol[n] = (PRE ? smem_addr(stages) + kStageBytes : smem_addr(xf)) + 16 * (t * p.xcols + (n * 8 + g < p.cols ? n * 8 + g : p.cols - 1));
     // scales of a stage: lane 2 r + h holds row r's of its tile h (the next
     // stage's as loaded: converting them would wait for the load)
     float sc[SLOTS], zc[SLOTS];
@@ -393,8 +414,8 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
       int seg0 = 0;
       for (int j = 0; j < ns; j += 2) {
         const int i = j + odd, tile = 2 * i;  // this warp's stage, and its tiles of this block's range
-        if (2 * j >= seg0 + p.seg) seg0 += p.seg;
-        if (seg0 != staged) {
+        if (!PRE && 2 * j >= seg0 + p.seg) seg0 += p.seg;
+        if (!PRE && seg0 != staged) {
           if (staged >= 0) consumer_sync();  // the segment before has been read
           stage_x<X16, SUB, VS, ZEROS>(a, p, t0 + seg0, nt - seg0 < p.seg ? nt - seg0 : p.seg, v0, xf, sx);
           consumer_sync();
@@ -419,10 +440,13 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
                                        kQWaitNs);
         uint32_t xt[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + (tile - seg0) * 8 * xstep;
+        for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + (PRE ? slot * stride : (tile - seg0) * 8 * xstep);
 #pragma unroll 1
         for (int h = 0; h < 2 && tile + h < nt; ++h) {
-          const uint32_t st = lane_addr + slot * kStageBytes + h * kBoxBytes;
+          if (PRE && h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + slot * stride + p.xtile;
+          const uint32_t st = lane_addr + slot * stride + h * kBoxBytes;
           float part[NT][4];
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
@@ -453,7 +477,9 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
           }
         }
         if (ZEROS && tile + (lane & 1) < nt) {
-          const float *s = sx + (tile + (lane & 1) - seg0) * SLOTS * VS;
+          const float *s = PRE ? reinterpret_cast<const float *>(stages + slot * stride + kStageBytes +
+                                                                 (lane & 1) * p.xtile + 512 * p.xcols)
+                               : sx + (tile + (lane & 1) - seg0) * SLOTS * VS;
 #pragma unroll
           for (int v = 0; v < VS; ++v) {
             if (v >= vectors) break;
@@ -516,18 +542,34 @@ template <bool X16, int NT, int SUB, bool ZEROS>
 static acd_status launch_mma(acd_ctx *ctx, const Quant4Args &a, Quant4Plan &p, int C, const CUtensorMap &map,
                              cudaStream_t s) {
   constexpr int VS = Q4Vectors<X16, NT>::value, RED = SumsStride<8 * NT + (ZEROS ? VS : 0)>::value;
-  constexpr int kStages = Q4Stages<NT>::value;
+  constexpr bool PRE = NT > 1;
   // a tile of x: 32 pieces of 16 bytes a column, 8 / SUB sums
   const int per = 32 * 16 * p.xcols + (ZEROS ? 8 / SUB * 4 * VS : 0);
-  const int fixed = 1024 + kStages * kStageBytes + kRowsPerBlock * RED * 4;
   const int64_t blocks = (int64_t)p.mblocks * C, columns = (a.N + p.vectors - 1) / p.vectors;
-  // whole pairs of stages, of which the warps take one each
-  const bool whole = blocks * columns <= ctx->sm_count || (kBlockSmem - fixed) / per < 4;
-  p.seg = ((whole ? kWholeSmem : kBlockSmem) - fixed) / per & ~3;
-  if (p.seg > ((p.tper + 3) & ~3)) p.seg = (p.tper + 3) & ~3;
-  const int dyn = fixed + p.seg * per;
+  const int fixed = 1024 + kRowsPerBlock * RED * 4;
+  int dyn;
+  unsigned char *xpre = nullptr;
+  if (PRE) {
+    p.xtile = (per + 15) & ~15;
+    const int stage = (kStageBytes + 2 * p.xtile + 1023) & ~1023;
+    p.stages = (kBlockSmem - fixed) / stage;
+    if (p.stages < 2) p.stages = (kWholeSmem - fixed) / stage;  // one block an SM
+    if (p.stages > kMaxStages) p.stages = kMaxStages;
+    dyn = fixed + p.stages * stage;
+    void *scratch;
+    ACD_TRY(get_scratch(ctx, (size_t)columns * p.ktiles * p.xtile, s, &scratch));
+    xpre = static_cast<unsigned char *>(scratch);
+    k_quant4_x<X16, NT, SUB, ZEROS><<<dim3((unsigned)p.ktiles, (unsigned)columns), 256, 0, s>>>(a, p, xpre);
+  } else {
+    p.stages = kMaxStages;
+    // whole pairs of stages, of which the warps take one each
+    const int room = (blocks * columns <= ctx->sm_count ? kWholeSmem : kBlockSmem) - fixed - p.stages * kStageBytes;
+    p.seg = room / per & ~3;
+    if (p.seg > ((p.tper + 3) & ~3)) p.seg = (p.tper + 3) & ~3;
+    dyn = fixed + p.stages * kStageBytes + p.seg * per;
+  }
   auto kern = k_quant4_mma<X16, NT, SUB, ZEROS>;
-  ACD_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn));
+  ACD_TRY(allow_smem(ctx, reinterpret_cast<const void *>(kern), dyn));
   int64_t grid = blocks;
   const int64_t resident = (int64_t)ctx->sm_count * (dyn > kBlockSmem ? 1 : 2);
   if (C == 1 && grid > resident) grid = resident;  // persistent
@@ -543,7 +585,7 @@ static acd_status launch_mma(acd_ctx *ctx, const Quant4Args &a, Quant4Plan &p, i
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  ACD_CUDA(cudaLaunchKernelEx(&cfg, kern, map, a, p, ctx->control));
+  ACD_CUDA(cudaLaunchKernelEx(&cfg, kern, map, a, p, (const unsigned char *)xpre, ctx->control));
   return ACD_OK;
 }
 
