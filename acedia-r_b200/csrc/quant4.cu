@@ -55,10 +55,11 @@ __device__ __forceinline__ void store_f(void *p, bool half, int64_t i, float v) 
 //   y = sum_groups s sum (n - 8) x  +  sum_groups s (8 - z) sum x,
 // the second term from sums of x that are made once.  float32 activations are
 // split into three bfloat16 parts that hold all 24 bits, which go in as three
-// columns.  One instruction's columns (NT = 1) are prepared by each block for
-// itself, a segment of the inputs at a time; more columns would cost the blocks
-// more than their weights do (64 us of 10007 x 8200 with six float32 columns),
-// so a kernel of its own prepares those once and they come in with the weights.
+// columns.  The blocks prepare activations for themselves where all of them fit
+// into shared memory, or where they are one instruction's columns (NT = 1; then
+// a segment of the inputs at a time).  More would cost the blocks more than
+// their weights do (64 us on 10007 x 8200 with six float32 columns, 53 us now):
+// a kernel of its own prepares them once and they come in with the weights.
 constexpr int kRowsPerBlock = 64;
 constexpr int kTileBytes = 128;                       // of one output: 256 inputs, 8 chunks of 32
 constexpr int kBoxBytes = kRowsPerBlock * kTileBytes;
@@ -70,8 +71,8 @@ struct Quant4Plan {
   int mblocks;         // blocks of 64 outputs
   int ktiles, tper;    // tiles of 256 inputs: in all, a block of a cluster (even, or all)
   int stages;          // of the ring
-  int seg;             // tiles whose activations are in shared memory at once (NT = 1)
-  int xtile;           // bytes of a tile's activations and sums as k_quant4_x leaves them (NT > 1)
+  int seg;             // tiles whose activations are in shared memory at once
+  int xtile;           // bytes of a tile's activations and sums where k_quant4_x has prepared them
   int vectors;         // columns of x a block (gridDim.y blocks of them)
   int cols;            // matrix columns: vectors, or three for each
   int xcols;           // places for them: 2 more than a multiple of 4, whose 16-byte reads meet no bank twice
@@ -174,6 +175,8 @@ __device__ __forceinline__ uint4 take_bf16(float (&f)[8]) {
                     __byte_perm(u[3], u[7], 0x7632));
 }
 
+// The two warps of 16 outputs.
+__device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(2 + pair) : "memory"); }
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Shared memory by its 32-bit address, so that the compiler neither widens it
@@ -286,14 +289,14 @@ __global__ void __launch_bounds__(256) k_quant4_x(Quant4Args a, Quant4Plan p, un
 template <bool X16, int NT, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ CUtensorMap map, Quant4Args a,
                                                        Quant4Plan p, const unsigned char *xpre, Control *control) {
-  constexpr bool PRE = NT > 1;
   constexpr int VS = Q4Vectors<X16, NT>::value, RED = SumsStride<8 * NT + (ZEROS ? VS : 0)>::value, SLOTS = 8 / SUB;
+  const bool prepared = NT > 1 && xpre != nullptr;
   extern __shared__ unsigned char smem[];
   __shared__ Quant4Shared sh;
   // the swizzle goes by the address: stages start on 1024 bytes
   unsigned char *stages = smem + ((1024u - (smem_addr(smem) & 1023u)) & 1023u);
   const int kStages = p.stages;
-  const uint32_t stride = PRE ? (uint32_t)(kStageBytes + 2 * p.xtile + 1023) & ~1023u : (uint32_t)kStageBytes;
+  const uint32_t stride = prepared ? (uint32_t)(kStageBytes + 2 * p.xtile + 1023) & ~1023u : (uint32_t)kStageBytes;
   float *red = reinterpret_cast<float *>(stages + kStages * stride);  // [64][RED]
   uint4 *xf = reinterpret_cast<uint4 *>(red + kRowsPerBlock * RED);
   float *sx = reinterpret_cast<float *>(xf + p.seg * 32 * p.xcols);
@@ -318,21 +321,21 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
   __syncthreads();
   if (warp == 8) {
     if (lane == 0) {
-      int n = 0;  // stages filled so far
+      int n = 0, slot = 0;  // stages filled so far, and the next one's place
+      uint32_t phase = 1;
       bool go = true;
       for (int mb = blockIdx.x / C; go && mb < p.mblocks; mb += mstep)
         for (int i = 0; i < ns; ++i, ++n) {
-          const int slot = n % kStages;
-          if (n >= kStages && !mbar_wait_thread(&sh.empty[slot], (uint32_t)(n / kStages - 1) & 1u, &sh.abort, control,
-                                                kQWaitCode, kQWaitNs)) {
+          if (n >= kStages &&
+              !mbar_wait_thread(&sh.empty[slot], phase, &sh.abort, control, kQWaitCode, kQWaitNs)) {
             go = false;
             break;
           }
           const bool two = 2 * i + 1 < nt;  // a tile past the range is not loaded
           unsigned char *st = stages + slot * stride;
-          const uint32_t xbytes = PRE ? (two ? 2 : 1) * p.xtile : 0;
+          const uint32_t xbytes = prepared ? (two ? 2 : 1) * p.xtile : 0;
           mbar_arrive_expect_tx(&sh.full[slot], (two ? kStageBytes : kBoxBytes) + xbytes);
-          if (PRE)
+          if (prepared)
             asm volatile(
                 "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                     smem_addr(st + kStageBytes)),
@@ -341,6 +344,10 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
                 : "memory");
           tma_load_2d(st, &map, &sh.full[slot], (t0 + 2 * i) * kTileBytes, mb * kRowsPerBlock);
           if (two) tma_load_2d(st + kBoxBytes, &map, &sh.full[slot], (t0 + 2 * i + 1) * kTileBytes, mb * kRowsPerBlock);
+          if (++slot == kStages) {
+            slot = 0;
+            phase ^= 1u;
+          }
         }
       // given up: the copies in flight land before the block may end
       if (*reinterpret_cast<volatile int *>(&sh.abort))
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
     const uint32_t xstep = 4 * 16 * p.xcols;  // bytes of a chunk
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      xcol[n] = (PRE ? smem_addr(stages) + kStageBytes : smem_addr(xf)) + 16 * (t * p.xcols + (n * 8 + g < p.cols ? n * 8 + g : p.cols - 1));
+      xcol[n] = (prepared ? smem_addr(stages) + kStageBytes : smem_addr(xf)) + 16 * (t * p.xcols + (n * 8 + g < p.cols ? n * 8 + g : p.cols - 1));
     // scales of a stage: lane 2 r + h holds row r's of its tile h (the next
     // stage's as loaded: converting them would wait for the load)
     float sc[SLOTS], zc[SLOTS];
@@ -405,17 +412,26 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
     const uint32_t lane_addr = smem_addr(stages) + (row0 + g) * kTileBytes + (g << 4) + t * 4;
     bool dead = false;
     int staged = -1;     // first tile of the activations in shared memory
-    uint32_t stage = 0;  // stages of the blocks before
+    // place and phase of the ring at a block's first stage; stages further on
+    const int turn = ns % kStages;
+    const uint32_t turns = (uint32_t)(ns / kStages) & 1u;
+    int slot0 = 0;
+    uint32_t phase0 = 0;
     scale_row(blockIdx.x / C);
     if (odd < ns) load_scales(t0 + 2 * odd);
-    for (int mb = blockIdx.x / C; mb < p.mblocks; mb += mstep, stage += ns) {
+    for (int mb = blockIdx.x / C; mb < p.mblocks; mb += mstep) {
       float tot[NT][4] = {};
       float corr[ZEROS ? VS : 1] = {};
-      int seg0 = 0;
+      int seg0 = 0, slot = slot0 + odd;
+      uint32_t phase = phase0;
+      if (slot >= kStages) {
+        slot -= kStages;
+        phase ^= 1u;
+      }
       for (int j = 0; j < ns; j += 2) {
         const int i = j + odd, tile = 2 * i;  // this warp's stage, and its tiles of this block's range
-        if (!PRE && 2 * j >= seg0 + p.seg) seg0 += p.seg;
-        if (!PRE && seg0 != staged) {
+        if (!prepared && 2 * j >= seg0 + p.seg) seg0 += p.seg;
+        if (!prepared && seg0 != staged) {
           if (staged >= 0) consumer_sync();  // the segment before has been read
           stage_x<X16, SUB, VS, ZEROS>(a, p, t0 + seg0, nt - seg0 < p.seg ? nt - seg0 : p.seg, v0, xf, sx);
           consumer_sync();
@@ -434,16 +450,14 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
           scale_row(mb + mstep);
           load_scales(t0 + 2 * odd);
         }
-        const uint32_t slot = (stage + i) % kStages;
         // once given up, the warps go on without waiting: all of them reach the barriers
-        dead = dead || !mbar_wait_warp(&sh.full[slot], (stage + i) / kStages & 1u, &sh.abort, control, kQWaitCode,
-                                       kQWaitNs);
+        dead = dead || !mbar_wait_warp(&sh.full[slot], phase, &sh.abort, control, kQWaitCode, kQWaitNs);
         uint32_t xt[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + (PRE ? slot * stride : (tile - seg0) * 8 * xstep);
+        for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + (prepared ? slot * stride : (tile - seg0) * 8 * xstep);
 #pragma unroll 1
         for (int h = 0; h < 2 && tile + h < nt; ++h) {
-          if (PRE && h)
+          if (prepared && h)
 #pragma unroll
             for (int n = 0; n < NT; ++n) xt[n] = xcol[n] + slot * stride + p.xtile;
           const uint32_t st = lane_addr + slot * stride + h * kBoxBytes;
@@ -477,7 +491,7 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
           }
         }
         if (ZEROS && tile + (lane & 1) < nt) {
-          const float *s = PRE ? reinterpret_cast<const float *>(stages + slot * stride + kStageBytes +
+          const float *s = prepared ? reinterpret_cast<const float *>(stages + slot * stride + kStageBytes +
                                                                  (lane & 1) * p.xtile + 512 * p.xcols)
                                : sx + (tile + (lane & 1) - seg0) * SLOTS * VS;
 #pragma unroll
@@ -489,6 +503,17 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.empty[slot]);
+        slot += 2;
+        if (slot >= kStages) {
+          slot -= kStages;
+          phase ^= 1u;
+        }
+      }
+      slot0 += turn;
+      phase0 ^= turns;
+      if (slot0 >= kStages) {
+        slot0 -= kStages;
+        phase0 ^= 1u;
       }
       // the odd stages' sums join the even ones'
       auto exchange = [&](auto f) {
@@ -505,7 +530,7 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
 #pragma unroll
         for (int v = 0; v < VS; ++v) corr[v] += __shfl_xor_sync(~0u, corr[v], 1);
       if (odd) exchange([](float &r, float x) { r = x; });
-      consumer_sync();
+      pair_sync(warp & 3);
       if (!odd) {
         exchange([](float &r, float x) { r += x; });
         __syncwarp();
@@ -516,7 +541,7 @@ __global__ void __launch_bounds__(288, 2) k_quant4_mma(const __grid_constant__ C
             if (o < a.M) store_f(a.out, a.out16, o * a.os + (v0 + v) * a.oc, row_value<X16, NT, ZEROS>(red + r * RED, v));
           }
       }
-      if (mb + mstep < p.mblocks) consumer_sync();  // red is written again
+      if (mb + mstep < p.mblocks) pair_sync(warp & 3);  // red is written again
     }
   }
   if (C == 1) return;
@@ -542,14 +567,25 @@ template <bool X16, int NT, int SUB, bool ZEROS>
 static acd_status launch_mma(acd_ctx *ctx, const Quant4Args &a, Quant4Plan &p, int C, const CUtensorMap &map,
                              cudaStream_t s) {
   constexpr int VS = Q4Vectors<X16, NT>::value, RED = SumsStride<8 * NT + (ZEROS ? VS : 0)>::value;
-  constexpr bool PRE = NT > 1;
   // a tile of x: 32 pieces of 16 bytes a column, 8 / SUB sums
   const int per = 32 * 16 * p.xcols + (ZEROS ? 8 / SUB * 4 * VS : 0);
   const int64_t blocks = (int64_t)p.mblocks * C, columns = (a.N + p.vectors - 1) / p.vectors;
   const int fixed = 1024 + kRowsPerBlock * RED * 4;
   int dyn;
   unsigned char *xpre = nullptr;
-  if (PRE) {
+  // the stages of the ring, and with them the tiles of activations there is room
+  // for: all of a block's range, or whole pairs of stages (a warp takes one each)
+  auto room = [&](int stages, int smem) {
+    const int tiles = (smem - fixed - stages * kStageBytes) / per;
+    return tiles >= p.tper ? p.tper : tiles & ~3;
+  };
+  p.stages = kMaxStages;
+  p.seg = room(p.stages, blocks * columns <= ctx->sm_count ? kWholeSmem : kBlockSmem);
+  if (NT > 1 && p.seg < p.tper) p.seg = room(p.stages = 3, kBlockSmem);
+  // all inputs at once are prepared by the blocks, which mostly have several
+  // blocks of outputs to use them for
+  if (NT > 1 && p.seg < p.tper) {
+    p.seg = 0;
     p.xtile = (per + 15) & ~15;
     const int stage = (kStageBytes + 2 * p.xtile + 1023) & ~1023;
     p.stages = (kBlockSmem - fixed) / stage;
@@ -561,11 +597,6 @@ static acd_status launch_mma(acd_ctx *ctx, const Quant4Args &a, Quant4Plan &p, i
     xpre = static_cast<unsigned char *>(scratch);
     k_quant4_x<X16, NT, SUB, ZEROS><<<dim3((unsigned)p.ktiles, (unsigned)columns), 256, 0, s>>>(a, p, xpre);
   } else {
-    p.stages = kMaxStages;
-    // whole pairs of stages, of which the warps take one each
-    const int room = (blocks * columns <= ctx->sm_count ? kWholeSmem : kBlockSmem) - fixed - p.stages * kStageBytes;
-    p.seg = room / per & ~3;
-    if (p.seg > ((p.tper + 3) & ~3)) p.seg = (p.tper + 3) & ~3;
     dyn = fixed + p.stages * kStageBytes + p.seg * per;
   }
   auto kern = k_quant4_mma<X16, NT, SUB, ZEROS>;
