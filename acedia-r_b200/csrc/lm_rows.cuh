@@ -228,20 +228,8 @@ __device__ __forceinline__ int row_shift(const T *x) {
   return V == 1 ? 0 : (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % V);
 }
 
-// Elements first .. first + V - 1 of a row of D, `fill` beyond its ends.  V = 1:
-// any stride.
-template <typename T, typename A, int V>
-__device__ __forceinline__ void load_piece(const T *x, int64_t sd, int first, int D, A fill, A *out) {
-  if (V == 1) {
-    out[0] = first < D ? to_acc(x[first * sd]) : fill;
-  } else if (first >= 0 && first + V <= D) {
-    reinterpret_cast<const Piece<T, V> *>(x + first)->widen(out);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = first + j >= 0 && first + j < D ? to_acc(x[first + j]) : fill;
-  }
-}
-
+// Elements first .. first + V - 1 of a row of D, as far as the row has them.
+// V = 1: any stride.
 template <typename T, typename A, int V>
 __device__ __forceinline__ void store_piece(T *x, int64_t sd, int first, int D, const A *v) {
   if (V > 1 && first >= 0 && first + V <= D) {

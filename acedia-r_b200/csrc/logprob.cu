@@ -5,7 +5,7 @@
 //   S = sum e^{c(x_v - m)},  T = sum c(x_v - m) e^{c(x_v - m)}
 // everything the forward call returns follows from (m, S, T):
 //   lse = c m + ln S,  logprob = c(x_t - m) - ln S,  entropy = ln S - T / S.
-// The gradient is one expression a logit (see k_logprob_grad).
+// The gradient is one expression a logit (see grad_values).
 #include <cooperative_groups.h>
 
 #include "lm_rows.cuh"
