@@ -293,7 +293,9 @@ __device__ __forceinline__ void row_sum(A (&v)[N], A *sh) {
 }
 
 // TPR threads a row, NV pieces of V columns a thread; the row stays in registers
-// between the two sums.
+// between the two sums.  Bound by its reads and writes (16384 x 4096 float16 with
+// 16 gate rows: 101 us, 0.81 of a copy's rate); what is left is the two
+// reductions a row, during which the block waits.
 template <typename T, int TPR, int NV, bool WHOLE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) {
   using A = typename AccOf<T>::type;
@@ -491,7 +493,12 @@ __device__ __forceinline__ void store_sums(A *dst, int64_t sd, int tid, int n, i
 }
 
 // V columns a thread, TPR threads a row; the column sums stay in registers.  The
-// next row is under way while one is worked on.
+// next row is under way while one is worked on.  Both means of a row come from
+// one reduction of three sums: the mean of the post norm's gradient splits into
+// two that do not wait for the other mean.  16384 x 4096 float16 with 16 gate rows
+// in 184 us, 0.67 of a copy's rate: its registers leave one block of 512 threads
+// an SM, which waits at the reduction's barrier.  Rows that do not start on 16
+// bytes are read an element at a time: 5000 x 1001 float32 in 37 us, 0.50.
 template <typename T, int TPR, bool WHOLE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 256 || sizeof(T) == 8 ? 1 : 2)
     k_norm_grad_vec(NormGradArgs a, GradPlan plan) {
@@ -580,19 +587,23 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
   }
 }
 
-// The same with rows brought in by bulk copies through a ring of stages, so that
-// several rows are under way while one is worked on.  A row stays in shared
-// memory: it is read once for its sums and once more for its gradients, which
-// leaves the registers to the column sums of NV pieces a thread and allows two
-// blocks on an SM, whose barriers then overlap (one block of 512 threads with
-// the row in registers: 220 us on 16384 x 4096 float16; two of 512 with 64
-// registers a thread: 369 us).  A cluster of CL blocks divides the columns of wider rows; the rows'
-// sums go to the other blocks by asynchronous stores that count on a barrier
-// there.
+// The same for wider rows: a cluster of CL blocks divides the columns, and the
+// rows come in by bulk copies through a ring of stages, so that several rows are
+// under way while one is worked on.  A row stays in shared memory: it is read
+// once for its sums and once more for its gradients, which leaves the registers
+// to the column sums of NV pieces a thread and allows two blocks on an SM, whose
+// barriers then overlap.  The rows' sums go to the other blocks by asynchronous
+// stores that count on a barrier there.
+//   What bounds it is that exchange, once a row, where a row's bytes do not
+// cover it: 16384 x 4096 float32 in 264 us (0.93 of a copy's rate), 16384 x 8192
+// float16 in 494 us (0.50), x 5120 in 485 us (0.32).  One piece a thread and
+// twice the blocks: 378, 605 and 610 us; k_norm_grad_vec with 1024 threads: 383,
+// 593 and 514 us.
 constexpr uint64_t kRingWaitNs = 1000000000ull;  // 1 s
 constexpr int kRingWaitCode = 6;
 constexpr int kRingStages = 3;
 constexpr int kRingCluster = 8;
+constexpr int kRingPieces = 2;  // of 16 bytes a thread
 
 template <typename A>
 struct RingShared {
@@ -621,10 +632,9 @@ __device__ __forceinline__ void send16(const void *at, const uint64_t *bar, int 
 
 constexpr int kRingThreads = 256;
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_ring(NormGradArgs a, GradPlan plan,
-                                                                                  Control *control) {
-  constexpr int TPR = kRingThreads;
+template <typename T>
+__global__ void __launch_bounds__(kRingThreads, 2) k_norm_grad_ring(NormGradArgs a, GradPlan plan, Control *control) {
+  constexpr int TPR = kRingThreads, NV = kRingPieces;
   using A = typename AccOf<T>::type;
   using P = Pk<A>;
   constexpr int V = 16 / sizeof(T), M = V / P::N, NW = TPR / 32, N = kRingStages;
@@ -647,10 +657,7 @@ __global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_rin
   // what no copy writes
   for (int i = tid; i < N * 4 * NV * TPR; i += TPR)
     if (i % (NV * TPR) * V >= D) reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0, 0, 0, 0);
-  if (CL > 1)
-    cluster.sync();
-  else
-    __syncthreads();
+  cluster.sync();
   // thread 0 walks ahead over the rows of this block's units and issues their copies
   int64_t fu = cid, frow = 0, fend = 0;
   int issued = 0;
@@ -756,27 +763,25 @@ __global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_rin
         for (int j = 0; j < 3; ++j) s[j] += __shfl_xor_sync(~0u, s[j], q);
 #pragma unroll
       for (int j = 0; j < 3; ++j) s[j] = __shfl_sync(~0u, s[j], 0);
-      if (CL > 1) {
-        if (warp == 0 && lane < CL) {
-          if (lane == 0) mbar_arrive_expect_tx(&sh.joined[flip], CL * 4 * (uint32_t)sizeof(A));
-          // the block's sums to every block, its own included
-          if constexpr (sizeof(A) == 4) {
-            send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, pack2(s[0], s[1]), pack2(s[2], 0.0f));
-          } else {
-            send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, __double_as_longlong(s[0]),
-                   __double_as_longlong(s[1]));
-            send16(&sh.other[flip][rank][2], &sh.joined[flip], lane, __double_as_longlong(s[2]), 0);
-          }
+      if (warp == 0 && lane < CL) {
+        if (lane == 0) mbar_arrive_expect_tx(&sh.joined[flip], CL * 4 * (uint32_t)sizeof(A));
+        // the block's sums to every block, its own included
+        if constexpr (sizeof(A) == 4) {
+          send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, pack2(s[0], s[1]), pack2(s[2], 0.0f));
+        } else {
+          send16(&sh.other[flip][rank][0], &sh.joined[flip], lane, __double_as_longlong(s[0]),
+                 __double_as_longlong(s[1]));
+          send16(&sh.other[flip][rank][2], &sh.joined[flip], lane, __double_as_longlong(s[2]), 0);
         }
-        __syncwarp();
-        dead = dead || !mbar_wait_warp(&sh.joined[flip], joined, &sh.abort, control, kRingWaitCode, kRingWaitNs);
-#pragma unroll
-        for (int j = 0; j < 3; ++j) {
-          s[j] = A(0);
-          for (int q = 0; q < CL; ++q) s[j] += sh.other[flip][q][j];
-        }
-        joined ^= (uint32_t)flip;  // both barriers have had a phase
       }
+      __syncwarp();
+      dead = dead || !mbar_wait_warp(&sh.joined[flip], joined, &sh.abort, control, kRingWaitCode, kRingWaitNs);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        s[j] = A(0);
+        for (int q = 0; q < CL; ++q) s[j] += sh.other[flip][q][j];
+      }
+      joined ^= (uint32_t)flip;  // both barriers have had a phase
       flip ^= 1;
       asm volatile("" ::: "memory");  // read again, not kept
 #pragma unroll
@@ -827,7 +832,7 @@ __global__ void __launch_bounds__(kRingThreads, NV == 1 ? 3 : 2) k_norm_grad_rin
     for (int q = issued > N ? issued - N : 0; q < issued; ++q)
       mbar_wait_bounded(&sh.full[q % N], (uint32_t)(q / N) & 1u, kRingWaitNs);
   __syncwarp();
-  if (CL > 1) cluster.sync();  // no block leaves while another may still write to it
+  cluster.sync();  // no block leaves while another may still write to it
 }
 
 // Column sums of `n` partial rows: a block takes 32 W columns, its 8 warps split
@@ -909,11 +914,14 @@ static acd_status launch_norm(acd_ctx *ctx, const NormArgs &a, cudaStream_t s) {
                      whole_rows(a.y, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
   const int64_t pieces = (a.s.D + V - 1) / V;
   if (pieces <= 4096) {
-    // a warp a row up to four pieces a lane, then two to four pieces a thread
+    // A warp a row up to three pieces a lane, whose sums need no barrier, then
+    // one to four pieces a thread.  16384 rows of float16 with a warp or 128
+    // threads: 64 pieces 16.4 or 24.1 us, 128 pieces 33.5 or 29.0 us; 512 pieces
+    // with 128 threads 128 us, with 256 101 us, with 512 113 us.
     if (pieces <= 32) return launch_norm_vec<T, 32, 1>(a, whole, s);
     if (pieces <= 64) return launch_norm_vec<T, 32, 2>(a, whole, s);
     if (pieces <= 96) return launch_norm_vec<T, 32, 3>(a, whole, s);
-    if (pieces <= 128) return launch_norm_vec<T, 32, 4>(a, whole, s);
+    if (pieces <= 128) return launch_norm_vec<T, 128, 1>(a, whole, s);
     if (pieces <= 256) return launch_norm_vec<T, 128, 2>(a, whole, s);
     if (pieces <= 384) return launch_norm_vec<T, 128, 3>(a, whole, s);
     if (pieces <= 512) return launch_norm_vec<T, 256, 2>(a, whole, s);
@@ -977,7 +985,9 @@ static acd_status run_norm_grad(acd_ctx *ctx, const NormGradArgs &a, int64_t gri
 template <typename T, int TPR>
 static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool whole, cudaStream_t s) {
   constexpr int BLOCK = TPR < 256 ? 256 : TPR;
-  auto kern = whole ? k_norm_grad_vec<T, TPR, true> : k_norm_grad_vec<T, TPR, false>;
+  auto kern = k_norm_grad_vec<T, TPR, false>;
+  if constexpr (TPR <= 512)  // wider whole rows go through the ring
+    if (whole) kern = k_norm_grad_vec<T, TPR, true>;
   const int64_t grid = (int64_t)ctx->sm_count * resident_blocks(reinterpret_cast<const void *>(kern), BLOCK, 0);
   return run_norm_grad<typename AccOf<T>::type>(ctx, a, grid, BLOCK / TPR, s, [&](int64_t blocks, const GradPlan &p) {
     kern<<<(unsigned)blocks, BLOCK, 0, s>>>(a, p);
@@ -985,13 +995,13 @@ static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool
   });
 }
 
-template <typename T, int NV>
+template <typename T>
 static acd_status launch_norm_grad_ring(acd_ctx *ctx, const NormGradArgs &a, int CL, cudaStream_t s) {
-  auto kern = k_norm_grad_ring<T, NV>;
-  const int dyn = kRingStages * 4 * NV * kRingThreads * 16;
+  auto kern = k_norm_grad_ring<T>;
+  const int dyn = kRingStages * 4 * kRingPieces * kRingThreads * 16;
   ACD_TRY(allow_smem(ctx, reinterpret_cast<const void *>(kern), dyn));
   return run_norm_grad<typename AccOf<T>::type>(
-      ctx, a, (int64_t)ctx->sm_count * (NV == 1 ? 3 : 2) / CL, 1, s, [&](int64_t clusters, const GradPlan &p) {
+      ctx, a, (int64_t)ctx->sm_count * 2 / CL, 1, s, [&](int64_t clusters, const GradPlan &p) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(clusters * CL), 1, 1);
         cfg.blockDim = dim3(kRingThreads, 1, 1);
@@ -1017,11 +1027,12 @@ static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStre
                      (!a.dh.p || whole_rows(a.dh, V)) && whole_rows(a.dy, V) && whole_rows(a.h, V) &&
                      whole_rows(a.b, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
   const int64_t pieces = (a.s.D + V - 1) / V;
-  // rows of 2 KB and more are worth a bulk copy each
-  if (whole && pieces > 128 && pieces <= 512 * kRingCluster) {
-    if (pieces <= 256) return launch_norm_grad_ring<T, 1>(ctx, a, 1, s);
-    return launch_norm_grad_ring<T, 2>(ctx, a, (int)((pieces + 511) / 512), s);
-  }
+  // Up to 512 pieces of 16 bytes a row a block keeps the row in registers, one
+  // piece a thread (16384 rows of float16: 256 pieces 94 us, 512 pieces 184 us; a
+  // single block of the ring 113 and 207 us); see k_norm_grad_ring for wider rows.
+  constexpr int block = kRingPieces * kRingThreads;
+  if (whole && pieces > block && pieces <= block * kRingCluster)
+    return launch_norm_grad_ring<T>(ctx, a, (int)((pieces + block - 1) / block), s);
   if (pieces <= 1024) {
     if (pieces <= 32) return launch_norm_grad_vec<T, 32>(ctx, a, whole, s);
     if (pieces <= 64) return launch_norm_grad_vec<T, 64>(ctx, a, whole, s);
