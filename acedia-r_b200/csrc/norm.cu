@@ -214,40 +214,49 @@ __global__ void __launch_bounds__(256) k_norm_grad_cols(NormGradArgs a, const ty
 // contiguous rows
 // ---------------------------------------------------------------------------
 // The V columns of a row that thread `tid` of TPR has in its n-th piece.
-// WHOLE: 16 consecutive bytes; every row, weight and gate row starts on a
-// 16-byte boundary and D is a multiple of V.  Otherwise TPR apart, so that a
-// warp still reads neighbouring elements: any alignment, width and stride, and
-// a thread's columns are the same in every row (a piece moved by each row's
-// misalignment would not be, and its weights would be read 16 bytes apart).
-template <int V, int TPR, bool WHOLE>
+// They come in groups of G that are read at once, and start on a boundary of as
+// many elements in every row, weight and gate row; the threads' groups lie side by
+// side, so that a warp reads neighbouring elements.  G = V: whole pieces.  G = 2:
+// rows of even width (16384 x 1634 float16, the gradient: 88 us, 216 with G = 1).
+// G = 1: any alignment, width and stride.  (A thread's columns are the same in
+// every row; a piece moved by each row's misalignment would not be, and its
+// weights would be read 16 bytes apart.)
+template <int V, int TPR, int G>
 __device__ __forceinline__ int column(int tid, int n, int j) {
-  return WHOLE ? (n * TPR + tid) * V + j : (n * V + j) * TPR + tid;
+  return ((n * (V / G) + j / G) * TPR + tid) * G + j % G;
 }
 
-template <typename T, int V, int TPR, bool WHOLE>
+template <typename T, int V, int TPR, int G>
 __device__ __forceinline__ Piece<T, V> fetch_cols(const T *x, int64_t sd, int tid, int n, int D) {
   Piece<T, V> p;
-  if (WHOLE && column<V, TPR, true>(tid, n, 0) < D)
-    p = *reinterpret_cast<const Piece<T, V> *>(x + column<V, TPR, true>(tid, n, 0));
-  if (!WHOLE || column<V, TPR, true>(tid, n, 0) >= D) {
+  if (G == V && column<V, TPR, V>(tid, n, 0) < D) {
+    p = *reinterpret_cast<const Piece<T, V> *>(x + column<V, TPR, V>(tid, n, 0));
+    return p;
+  }
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int d = column<V, TPR, WHOLE>(tid, n, j);
-      p.set(j, !WHOLE && d < D ? x[d * sd] : (T)0.0f);
+  for (int j = 0; j < V; j += G == V ? 1 : G) {
+    const int d = column<V, TPR, G>(tid, n, j);
+    if (G == 2 && G < V) {
+      Vec<T, 2> w = {};
+      if (d < D) w = *reinterpret_cast<const Vec<T, 2> *>(x + d);
+      p.set(j, w.v[0]);
+      p.set(j + 1, w.v[1]);
+    } else {
+      p.set(j, G < V && d < D ? x[d * sd] : (T)0.0f);
     }
   }
   return p;
 }
 
-template <typename T, typename A, int V, int TPR, bool WHOLE>
+template <typename T, typename A, int V, int TPR, int G>
 __device__ __forceinline__ void load_cols(const T *x, int64_t sd, int tid, int n, int D, A *out) {
-  fetch_cols<T, V, TPR, WHOLE>(x, sd, tid, n, D).widen(out);
+  fetch_cols<T, V, TPR, G>(x, sd, tid, n, D).widen(out);
 }
 
-template <typename T, typename A, int V, int TPR, bool WHOLE>
+template <typename T, typename A, int V, int TPR, int G>
 __device__ __forceinline__ void store_cols(T *x, int64_t sd, int tid, int n, int D, const A *v) {
-  if (WHOLE) {
-    const int first = column<V, TPR, true>(tid, n, 0);
+  if (G == V) {
+    const int first = column<V, TPR, V>(tid, n, 0);
     if (first < D) {
       Piece<T, V> w;
       w.round(v);
@@ -255,9 +264,15 @@ __device__ __forceinline__ void store_cols(T *x, int64_t sd, int tid, int n, int
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int d = column<V, TPR, false>(tid, n, j);
-      if (d < D) x[d * sd] = from_acc<T, A>(v[j]);
+    for (int j = 0; j < V; j += G) {
+      const int d = column<V, TPR, G>(tid, n, j);
+      if (d >= D) continue;
+      if (G == 2) {
+        Vec<T, 2> w = {from_acc<T, A>(v[j]), from_acc<T, A>(v[j + G - 1])};
+        *reinterpret_cast<Vec<T, 2> *>(x + d) = w;
+      } else {
+        x[d * sd] = from_acc<T, A>(v[j]);
+      }
     }
   }
 }
@@ -296,7 +311,7 @@ __device__ __forceinline__ void row_sum(A (&v)[N], A *sh) {
 // between the two sums.  Bound by its reads and writes (16384 x 4096 float16 with
 // 16 gate rows: 101 us, 0.81 of a copy's rate); what is left is the two
 // reductions a row, during which the block waits.
-template <typename T, int TPR, int NV, bool WHOLE>
+template <typename T, int TPR, int NV, int G>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) {
   using A = typename AccOf<T>::type;
   using P = Pk<A>;
@@ -313,8 +328,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) 
   Piece<T, V> br[NV], rr_[NV];
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    br[n] = fetch_cols<T, V, TPR, WHOLE>(b, a.b.sd, tid, n, D);
-    rr_[n] = fetch_cols<T, V, TPR, WHOLE>(r, a.r.sd, tid, n, D);
+    br[n] = fetch_cols<T, V, TPR, G>(b, a.b.sd, tid, n, D);
+    rr_[n] = fetch_cols<T, V, TPR, G>(r, a.r.sd, tid, n, D);
   }
   P h[NV][M];
   A f[V];
@@ -340,7 +355,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) 
     const P prb = P::all(rb);
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      load_cols<T, A, V, TPR, WHOLE>(w_post, 1, tid, n, D, f);
+      load_cols<T, A, V, TPR, G>(w_post, 1, tid, n, D, f);
 #pragma unroll
       for (int j = 0; j < M; ++j) h[n][j] = pmul(pmul(h[n][j], prb), P::from(f + j * P::N));
     }
@@ -349,7 +364,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) 
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     if (a.gate) {
-      load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + (int64_t)((uint32_t)rr / (uint32_t)a.per) * a.gate_sg, a.gate_sd, tid, n, D, f);
+      load_cols<T, A, V, TPR, G>(static_cast<const T *>(a.gate) + (int64_t)((uint32_t)rr / (uint32_t)a.per) * a.gate_sg, a.gate_sd, tid, n, D, f);
 #pragma unroll
       for (int j = 0; j < M; ++j) h[n][j] = pmul(h[n][j], P::from(f + j * P::N));
     }
@@ -366,13 +381,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_vec(NormArgs a) 
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
     A y[V];
-    load_cols<T, A, V, TPR, WHOLE>(w_pre, 1, tid, n, D, f);
+    load_cols<T, A, V, TPR, G>(w_pre, 1, tid, n, D, f);
 #pragma unroll
     for (int j = 0; j < M; ++j) pmul(pmul(h[n][j], prh), P::from(f + j * P::N)).to(y + j * P::N);
-    store_cols<T, A, V, TPR, WHOLE>(yo, a.y.sd, tid, n, D, y);
+    store_cols<T, A, V, TPR, G>(yo, a.y.sd, tid, n, D, y);
 #pragma unroll
     for (int j = 0; j < M; ++j) h[n][j].to(f + j * P::N);
-    store_cols<T, A, V, TPR, WHOLE>(ho, a.h.sd, tid, n, D, f);
+    store_cols<T, A, V, TPR, G>(ho, a.h.sd, tid, n, D, f);
   }
   if (tid == 0) {
     if (a.rstd_h) static_cast<A *>(a.rstd_h)[row] = rh;
@@ -455,14 +470,14 @@ struct GradCols {
 };
 
 // The operands that stay while the gate row does: w_pre, and f = gate w_post.
-template <typename T, typename A, int V, int TPR, bool WHOLE>
+template <typename T, typename A, int V, int TPR, int G>
 __device__ __forceinline__ void load_operands(const NormGradArgs &a, int64_t row, int tid, int n, int D, A (&wo)[V], A (&g)[V],
                                               Pk<A> (&f)[V / Pk<A>::N]) {
 #pragma unroll
   for (int j = 0; j < V; ++j) wo[j] = g[j] = A(1);
-  if (a.w_post) load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.w_post), 1, tid, n, D, wo);
+  if (a.w_post) load_cols<T, A, V, TPR, G>(static_cast<const T *>(a.w_post), 1, tid, n, D, wo);
   if (a.gate)
-    load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.gate) + (int64_t)((uint32_t)row / (uint32_t)a.per) * a.gate_sg, a.gate_sd, tid, n, D, g);
+    load_cols<T, A, V, TPR, G>(static_cast<const T *>(a.gate) + (int64_t)((uint32_t)row / (uint32_t)a.per) * a.gate_sg, a.gate_sd, tid, n, D, g);
 #pragma unroll
   for (int j = 0; j < V / Pk<A>::N; ++j)
     f[j] = pmul(Pk<A>::from(wo + j * Pk<A>::N), Pk<A>::from(g + j * Pk<A>::N));
@@ -483,11 +498,11 @@ __device__ __forceinline__ void add_subs(A (&acc)[V], A (*join)[V]) {
       for (int j = 0; j < V; ++j) acc[j] += join[q * TPR + tid][j];
 }
 
-template <typename A, int V, int TPR, bool WHOLE>
+template <typename A, int V, int TPR, int G>
 __device__ __forceinline__ void store_sums(A *dst, int64_t sd, int tid, int n, int D, const A (&v)[V]) {
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int d = column<V, TPR, WHOLE>(tid, n, j);
+    const int d = column<V, TPR, G>(tid, n, j);
     if (d < D) dst[d * sd] = v[j];
   }
 }
@@ -497,9 +512,9 @@ __device__ __forceinline__ void store_sums(A *dst, int64_t sd, int tid, int n, i
 // one reduction of three sums: the mean of the post norm's gradient splits into
 // two that do not wait for the other mean.  16384 x 4096 float16 with 16 gate rows
 // in 184 us, 0.67 of a copy's rate: its registers leave one block of 512 threads
-// an SM, which waits at the reduction's barrier.  Rows that do not start on 16
-// bytes are read an element at a time: 5000 x 1001 float32 in 37 us, 0.50.
-template <typename T, int TPR, bool WHOLE>
+// an SM, which waits at the reduction's barrier.  Rows of odd width are
+// read an element at a time: 5000 x 1001 float32 in 37 us, 0.50.
+template <typename T, int TPR, int G>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 256 || sizeof(T) == 8 ? 1 : 2)
     k_norm_grad_vec(NormGradArgs a, GradPlan plan) {
   using A = typename AccOf<T>::type;
@@ -513,7 +528,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
   const A alpha = (A)a.alpha, inv = A(1) / (A)a.s.D;
   P wp[M], f[M], pre[M], pst[M];
   A wo[V], g[V], c[V];
-  load_cols<T, A, V, TPR, WHOLE>(static_cast<const T *>(a.w_pre), 1, tid, 0, D, c);
+  load_cols<T, A, V, TPR, G>(static_cast<const T *>(a.w_pre), 1, tid, 0, D, c);
 #pragma unroll
   for (int j = 0; j < M; ++j) {
     wp[j] = P::from(c + j * P::N);
@@ -523,7 +538,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
   for (int64_t u = blockIdx.x; u < plan.groups * plan.parts; u += gridDim.x) {
     int64_t r0, r1;
     unit_rows(plan, u, r0, r1);
-    load_operands<T, A, V, TPR, WHOLE>(a, r0, tid, 0, D, wo, g, f);
+    load_operands<T, A, V, TPR, G>(a, r0, tid, 0, D, wo, g, f);
     P tb[M];
 #pragma unroll
     for (int j = 0; j < M; ++j) tb[j] = P::all(A(0));
@@ -535,10 +550,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
       const bool ok = rr + sub < r1;
       const int64_t row = ok ? rr + sub : r0;
       const int n = ok ? D : 0;
-      if (a.dh.p) x.dh = fetch_cols<T, V, TPR, WHOLE>(row_ptr<T>(a.dh, row, a.s.L), a.dh.sd, tid, 0, n);
-      x.dy = fetch_cols<T, V, TPR, WHOLE>(row_ptr<T>(a.dy, row, a.s.L), a.dy.sd, tid, 0, n);
-      x.h = fetch_cols<T, V, TPR, WHOLE>(row_ptr<T>(a.h, row, a.s.L), a.h.sd, tid, 0, n);
-      x.b = fetch_cols<T, V, TPR, WHOLE>(row_ptr<T>(a.b, row, a.s.L), a.b.sd, tid, 0, n);
+      if (a.dh.p) x.dh = fetch_cols<T, V, TPR, G>(row_ptr<T>(a.dh, row, a.s.L), a.dh.sd, tid, 0, n);
+      x.dy = fetch_cols<T, V, TPR, G>(row_ptr<T>(a.dy, row, a.s.L), a.dy.sd, tid, 0, n);
+      x.h = fetch_cols<T, V, TPR, G>(row_ptr<T>(a.h, row, a.s.L), a.h.sd, tid, 0, n);
+      x.b = fetch_cols<T, V, TPR, G>(row_ptr<T>(a.b, row, a.s.L), a.b.sd, tid, 0, n);
       x.rh = ok ? static_cast<const A *>(a.rstd_h)[row] : A(0);
       x.rb = post && ok ? static_cast<const A *>(a.rstd_b)[row] : A(1);
     };
@@ -559,13 +574,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
       flip ^= 1;
       p.finish(s, inv, cur.rh, cur.rb, alpha, post, f, pre, tb, dh, dy);
       if (rr + sub < r1) {
-        store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.dr, rr + sub, a.s.L), a.dr.sd, tid, 0, D, dh);
-        store_cols<T, A, V, TPR, WHOLE>(row_ptr<T>(a.db, rr + sub, a.s.L), a.db.sd, tid, 0, D, dy);
+        store_cols<T, A, V, TPR, G>(row_ptr<T>(a.dr, rr + sub, a.s.L), a.dr.sd, tid, 0, D, dh);
+        store_cols<T, A, V, TPR, G>(row_ptr<T>(a.db, rr + sub, a.s.L), a.db.sd, tid, 0, D, dy);
       }
       cur = next;
     }
     // (read again: they are wanted once a unit only)
-    load_operands<T, A, V, TPR, WHOLE>(a, r0, tid, 0, D, wo, g, f);
+    load_operands<T, A, V, TPR, G>(a, r0, tid, 0, D, wo, g, f);
 #pragma unroll
     for (int j = 0; j < M; ++j) {
       pst[j] = pfma(P::from(g + j * P::N), tb[j], pst[j]);
@@ -573,7 +588,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
     }
     if (plan.gate) {
       add_subs<A, V, TPR, RPB>(c, join);
-      if (sub == 0) store_sums<A, V, TPR, WHOLE>(static_cast<A *>(plan.gate) + u * plan.gate_su, plan.gate_sd, tid, 0, D, c);
+      if (sub == 0) store_sums<A, V, TPR, G>(static_cast<A *>(plan.gate) + u * plan.gate_su, plan.gate_sd, tid, 0, D, c);
     }
   }
 #pragma unroll
@@ -583,7 +598,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
 #pragma unroll
     for (int j = 0; j < M; ++j) (w ? pst[j] : pre[j]).to(c + j * P::N);
     add_subs<A, V, TPR, RPB>(c, join);
-    if (sub == 0) store_sums<A, V, TPR, WHOLE>(dst + (int64_t)blockIdx.x * D, 1, tid, 0, D, c);
+    if (sub == 0) store_sums<A, V, TPR, G>(dst + (int64_t)blockIdx.x * D, 1, tid, 0, D, c);
   }
 }
 
@@ -691,7 +706,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) k_norm_grad_ring(NormGradArgs
   P f[NV][M], pre[NV][M], tb[NV][M];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    wraw[v] = fetch_cols<T, V, TPR, true>(static_cast<const T *>(slice.w_pre), 1, tid, v, D);
+    wraw[v] = fetch_cols<T, V, TPR, V>(static_cast<const T *>(slice.w_pre), 1, tid, v, D);
 #pragma unroll
     for (int j = 0; j < M; ++j) pre[v][j] = P::all(A(0));
   }
@@ -704,7 +719,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) k_norm_grad_ring(NormGradArgs
     A wo[V], g[V], c[V];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      load_operands<T, A, V, TPR, true>(slice, r0, tid, v, D, wo, g, f[v]);
+      load_operands<T, A, V, TPR, V>(slice, r0, tid, v, D, wo, g, f[v]);
 #pragma unroll
       for (int j = 0; j < M; ++j) tb[v][j] = P::all(A(0));
     }
@@ -789,8 +804,8 @@ __global__ void __launch_bounds__(kRingThreads, 2) k_norm_grad_ring(NormGradArgs
         A dr[V], db[V];
         read(v);
         p.finish(s, inv, rh, rb, alpha, post, f[v], pre[v], tb[v], dr, db);
-        store_cols<T, A, V, TPR, true>(row_ptr<T>(a.dr, row, a.s.L) + c0, 1, tid, v, D, dr);
-        store_cols<T, A, V, TPR, true>(row_ptr<T>(a.db, row, a.s.L) + c0, 1, tid, v, D, db);
+        store_cols<T, A, V, TPR, V>(row_ptr<T>(a.dr, row, a.s.L) + c0, 1, tid, v, D, dr);
+        store_cols<T, A, V, TPR, V>(row_ptr<T>(a.db, row, a.s.L) + c0, 1, tid, v, D, db);
       }
       if (++slot == N) {
         slot = 0;
@@ -801,9 +816,9 @@ __global__ void __launch_bounds__(kRingThreads, 2) k_norm_grad_ring(NormGradArgs
     // straight to this block's row of the partial sums)
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      load_operands<T, A, V, TPR, true>(slice, r0, tid, v, D, wo, g, f[v]);
-      if (plan.post && column<V, TPR, true>(tid, v, 0) < D) {
-        A *dst = static_cast<A *>(plan.post) + cid * a.s.D + c0 + column<V, TPR, true>(tid, v, 0);
+      load_operands<T, A, V, TPR, V>(slice, r0, tid, v, D, wo, g, f[v]);
+      if (plan.post && column<V, TPR, V>(tid, v, 0) < D) {
+        A *dst = static_cast<A *>(plan.post) + cid * a.s.D + c0 + column<V, TPR, V>(tid, v, 0);
 #pragma unroll
         for (int j = 0; j < M; ++j) pmul(P::from(g + j * P::N), tb[v][j]).to(c + j * P::N);
 #pragma unroll
@@ -812,7 +827,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) k_norm_grad_ring(NormGradArgs
       if (plan.gate) {
 #pragma unroll
         for (int j = 0; j < M; ++j) pmul(P::from(wo + j * P::N), tb[v][j]).to(c + j * P::N);
-        store_sums<A, V, TPR, true>(static_cast<A *>(plan.gate) + u * plan.gate_su + c0 * plan.gate_sd, plan.gate_sd, tid, v,
+        store_sums<A, V, TPR, V>(static_cast<A *>(plan.gate) + u * plan.gate_su + c0 * plan.gate_sd, plan.gate_sd, tid, v,
                                     D, c);
       }
     }
@@ -824,7 +839,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) k_norm_grad_ring(NormGradArgs
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
       for (int j = 0; j < M; ++j) pre[v][j].to(c + j * P::N);
-      store_sums<A, V, TPR, true>(static_cast<A *>(plan.pre) + cid * a.s.D + c0, 1, tid, v, D, c);
+      store_sums<A, V, TPR, V>(static_cast<A *>(plan.pre) + cid * a.s.D + c0, 1, tid, v, D, c);
     }
   }
   // given up: the copies in flight land before the block may end
@@ -885,51 +900,64 @@ __global__ void __launch_bounds__(256) k_norm_grad_join(JoinArgs<A> a) {
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// Whether the rows of `v` are contiguous and start on 16-byte boundaries (the
-// width is checked once, for all of them).
-static bool whole_rows(const Rows &v, int V) {
-  return v.sd == 1 && aligned_to<char>(v.p, 16) && v.sl % V == 0 && v.so % V == 0;
+// Whether the rows of `v` are contiguous and start on boundaries of g elements
+// (the width is checked once, for all of them).
+template <typename T>
+static bool whole_rows(const Rows &v, int g) {
+  return v.sd == 1 && aligned_to<char>(v.p, g * (int)sizeof(T)) && v.sl % g == 0 && v.so % g == 0;
 }
 // Weights and gate rows too.
-static bool whole_weights(const void *w_pre, const void *w_post, const void *gate, int64_t sd, int64_t sg, int V) {
-  return aligned_to<char>(w_pre, 16) && (!w_post || aligned_to<char>(w_post, 16)) &&
-         (!gate || (aligned_to<char>(gate, 16) && sd == 1 && sg % V == 0));
+template <typename T>
+static bool whole_weights(const void *w_pre, const void *w_post, const void *gate, int64_t sd, int64_t sg, int g) {
+  const int bytes = g * (int)sizeof(T);
+  return aligned_to<char>(w_pre, bytes) && (!w_post || aligned_to<char>(w_post, bytes)) &&
+         (!gate || (aligned_to<char>(gate, bytes) && sd == 1 && sg % g == 0));
+}
+// Elements that are read at once: a piece, two, or one.
+template <typename T, typename Fits>
+static int granule(int64_t D, Fits fits) {
+  constexpr int V = 16 / sizeof(T);
+  return D % V == 0 && fits(V) ? V : D % 2 == 0 && fits(2) ? 2 : 1;
 }
 
 template <typename T, int TPR, int NV>
-static acd_status launch_norm_vec(const NormArgs &a, bool whole, cudaStream_t s) {
-  constexpr int BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
+static acd_status launch_norm_vec(const NormArgs &a, int g, cudaStream_t s) {
+  constexpr int BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR, V = 16 / sizeof(T);
   const int64_t grid = (a.s.rows() + RPB - 1) / RPB;
-  if (whole)
-    k_norm_vec<T, TPR, NV, true><<<(unsigned)grid, BLOCK, 0, s>>>(a);
-  else
-    k_norm_vec<T, TPR, NV, false><<<(unsigned)grid, BLOCK, 0, s>>>(a);
+  auto kern = k_norm_vec<T, TPR, NV, 1>;
+  if (g == V)
+    kern = k_norm_vec<T, TPR, NV, V>;
+  else if (g == 2)
+    kern = k_norm_vec<T, TPR, NV, 2>;
+  kern<<<(unsigned)grid, BLOCK, 0, s>>>(a);
   return ACD_OK;
 }
 
 template <typename T>
 static acd_status launch_norm(acd_ctx *ctx, const NormArgs &a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  const bool whole = a.s.D % V == 0 && whole_rows(a.r, V) && whole_rows(a.b, V) && whole_rows(a.h, V) &&
-                     whole_rows(a.y, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
+  const int g = granule<T>(a.s.D, [&](int n) {
+    return whole_rows<T>(a.r, n) && whole_rows<T>(a.b, n) && whole_rows<T>(a.h, n) && whole_rows<T>(a.y, n) &&
+           whole_weights<T>(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, n);
+  });
   const int64_t pieces = (a.s.D + V - 1) / V;
   if (pieces <= 4096) {
     // A warp a row up to three pieces a lane, whose sums need no barrier, then
     // one to four pieces a thread.  16384 rows of float16 with a warp or 128
     // threads: 64 pieces 16.4 or 24.1 us, 128 pieces 33.5 or 29.0 us; 512 pieces
     // with 128 threads 128 us, with 256 101 us, with 512 113 us.
-    if (pieces <= 32) return launch_norm_vec<T, 32, 1>(a, whole, s);
-    if (pieces <= 64) return launch_norm_vec<T, 32, 2>(a, whole, s);
-    if (pieces <= 96) return launch_norm_vec<T, 32, 3>(a, whole, s);
-    if (pieces <= 128) return launch_norm_vec<T, 128, 1>(a, whole, s);
-    if (pieces <= 256) return launch_norm_vec<T, 128, 2>(a, whole, s);
-    if (pieces <= 384) return launch_norm_vec<T, 128, 3>(a, whole, s);
-    if (pieces <= 512) return launch_norm_vec<T, 256, 2>(a, whole, s);
-    if (pieces <= 768) return launch_norm_vec<T, 256, 3>(a, whole, s);
-    if (pieces <= 1024) return launch_norm_vec<T, 512, 2>(a, whole, s);
-    if (pieces <= 1536) return launch_norm_vec<T, 512, 3>(a, whole, s);
-    if (pieces <= 2048) return launch_norm_vec<T, 512, 4>(a, whole, s);
-    return launch_norm_vec<T, 1024, 4>(a, whole, s);
+    if (pieces <= 32) return launch_norm_vec<T, 32, 1>(a, g, s);
+    if (pieces <= 64) return launch_norm_vec<T, 32, 2>(a, g, s);
+    if (pieces <= 96) return launch_norm_vec<T, 32, 3>(a, g, s);
+    if (pieces <= 128) return launch_norm_vec<T, 128, 1>(a, g, s);
+    if (pieces <= 256) return launch_norm_vec<T, 128, 2>(a, g, s);
+    if (pieces <= 384) return launch_norm_vec<T, 128, 3>(a, g, s);
+    if (pieces <= 512) return launch_norm_vec<T, 256, 2>(a, g, s);
+    if (pieces <= 768) return launch_norm_vec<T, 256, 3>(a, g, s);
+    if (pieces <= 1024) return launch_norm_vec<T, 512, 2>(a, g, s);
+    if (pieces <= 1536) return launch_norm_vec<T, 512, 3>(a, g, s);
+    if (pieces <= 2048) return launch_norm_vec<T, 512, 4>(a, g, s);
+    return launch_norm_vec<T, 1024, 4>(a, g, s);
   }
   const int grid = persistent_grid(ctx, k_norm_rows<T>, 256, 0, a.s.rows());
   k_norm_rows<T><<<grid, 256, 0, s>>>(a);
@@ -983,11 +1011,13 @@ static acd_status run_norm_grad(acd_ctx *ctx, const NormGradArgs &a, int64_t gri
 }
 
 template <typename T, int TPR>
-static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, bool whole, cudaStream_t s) {
-  constexpr int BLOCK = TPR < 256 ? 256 : TPR;
-  auto kern = k_norm_grad_vec<T, TPR, false>;
+static acd_status launch_norm_grad_vec(acd_ctx *ctx, const NormGradArgs &a, int g, cudaStream_t s) {
+  constexpr int BLOCK = TPR < 256 ? 256 : TPR, V = 16 / sizeof(T);
+  auto kern = k_norm_grad_vec<T, TPR, 1>;
   if constexpr (TPR <= 512)  // wider whole rows go through the ring
-    if (whole) kern = k_norm_grad_vec<T, TPR, true>;
+    if (g == V) kern = k_norm_grad_vec<T, TPR, V>;
+  if constexpr (V > 2)
+    if (g == 2) kern = k_norm_grad_vec<T, TPR, 2>;
   const int64_t grid = (int64_t)ctx->sm_count * resident_blocks(reinterpret_cast<const void *>(kern), BLOCK, 0);
   return run_norm_grad<typename AccOf<T>::type>(ctx, a, grid, BLOCK / TPR, s, [&](int64_t blocks, const GradPlan &p) {
     kern<<<(unsigned)blocks, BLOCK, 0, s>>>(a, p);
@@ -1023,23 +1053,25 @@ template <typename T>
 static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStream_t s) {
   using A = typename AccOf<T>::type;
   constexpr int V = 16 / sizeof(T);
-  const bool whole = a.s.D % V == 0 && whole_rows(a.dr, V) && whole_rows(a.db, V) &&
-                     (!a.dh.p || whole_rows(a.dh, V)) && whole_rows(a.dy, V) && whole_rows(a.h, V) &&
-                     whole_rows(a.b, V) && whole_weights(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, V);
+  const int g = granule<T>(a.s.D, [&](int n) {
+    return whole_rows<T>(a.dr, n) && whole_rows<T>(a.db, n) && (!a.dh.p || whole_rows<T>(a.dh, n)) &&
+           whole_rows<T>(a.dy, n) && whole_rows<T>(a.h, n) && whole_rows<T>(a.b, n) &&
+           whole_weights<T>(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, n);
+  });
   const int64_t pieces = (a.s.D + V - 1) / V;
   // Up to 512 pieces of 16 bytes a row a block keeps the row in registers, one
   // piece a thread (16384 rows of float16: 256 pieces 94 us, 512 pieces 184 us; a
   // single block of the ring 113 and 207 us); see k_norm_grad_ring for wider rows.
   constexpr int block = kRingPieces * kRingThreads;
-  if (whole && pieces > block && pieces <= block * kRingCluster)
+  if (g == V && pieces > block && pieces <= block * kRingCluster)
     return launch_norm_grad_ring<T>(ctx, a, (int)((pieces + block - 1) / block), s);
   if (pieces <= 1024) {
-    if (pieces <= 32) return launch_norm_grad_vec<T, 32>(ctx, a, whole, s);
-    if (pieces <= 64) return launch_norm_grad_vec<T, 64>(ctx, a, whole, s);
-    if (pieces <= 128) return launch_norm_grad_vec<T, 128>(ctx, a, whole, s);
-    if (pieces <= 256) return launch_norm_grad_vec<T, 256>(ctx, a, whole, s);
-    if (pieces <= 512) return launch_norm_grad_vec<T, 512>(ctx, a, whole, s);
-    return launch_norm_grad_vec<T, 1024>(ctx, a, whole, s);
+    if (pieces <= 32) return launch_norm_grad_vec<T, 32>(ctx, a, g, s);
+    if (pieces <= 64) return launch_norm_grad_vec<T, 64>(ctx, a, g, s);
+    if (pieces <= 128) return launch_norm_grad_vec<T, 128>(ctx, a, g, s);
+    if (pieces <= 256) return launch_norm_grad_vec<T, 256>(ctx, a, g, s);
+    if (pieces <= 512) return launch_norm_grad_vec<T, 512>(ctx, a, g, s);
+    return launch_norm_grad_vec<T, 1024>(ctx, a, g, s);
   }
   void *scratch;
   ACD_TRY(get_scratch(ctx, sizeof(A) * (size_t)a.s.rows(), s, &scratch));

@@ -164,6 +164,22 @@ def test_views(acd, dtype):
     check(acd, (96, 7, 5), 1, dtype, seed=5, wrap=permuted)
 
 
+@pytest.mark.parametrize("dtype", ["float", "float16"])
+@pytest.mark.parametrize("D,pitch,offset", [(2, 2, 0), (6, 6, 0), (98, 98, 2), (98, 99, 0), (130, 132, 1), (634, 640, 4),
+                                            (1634, 1636, 2), (1634, 1634, 1), (4098, 4100, 0), (6146, 6146, 0)])
+def test_even_widths(acd, dtype, D, pitch, offset):
+    """Rows of even width on every second element's boundary, and off it."""
+    def wrap(a):
+        rows = a.shape[1]
+        host = np.zeros(offset + pitch * rows, NP[dtype])
+        for k in range(rows):
+            host[offset + pitch * k: offset + pitch * k + D] = a[:, k]
+        st = torch.from_numpy(host).to("cuda")
+        return acd.gpuTensor(st, (D, rows), dtype, (1, pitch), offset)
+    check(acd, (D, 21), 1, dtype, gshape=(D,), seed=D, wrap=wrap)
+    check(acd, (D, 21), 1, dtype, post=False, gshape=(D, 21), alpha=0.5, seed=D + 1, wrap=wrap, with_dh=False)
+
+
 def test_zero_rows_and_zero_blocks(acd):
     """A row of zeros: rstd = 1 / sqrt(eps), y = 0; no rows: nothing, sums of 0."""
     z = acd.as_tensor(np.zeros((64, 3)), dtype="float")
