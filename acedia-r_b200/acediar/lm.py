@@ -7,6 +7,7 @@ formulas and every rule on masked, missing and empty values stand beside the C
 functions in include/acd.h.  The reference has none of these operators.
 """
 import ctypes
+import functools
 import numbers
 import struct
 from collections import namedtuple
@@ -24,22 +25,40 @@ Quant4 = namedtuple("Quant4", "weights scales zeros")
 _UNSUPPORTED = 8
 
 
-def _new(shape, dtype, device):
-    """An uninitialised tensor; shape is a tuple of ints.  (A small call's time is
-    its host time: the attributes are set without the constructor's checks.)"""
-    t = gpuTensor.__new__(gpuTensor)
+# A small call's time is its host time, so what follows from a shape alone is
+# worked out once a shape.
+@functools.lru_cache(maxsize=4096)
+def _layout(shape):
+    """Elements to allocate and column-major strides."""
     n, strides = 1, []
     for s in shape:
         strides.append(n)
         n *= s
-    t.storage = torch.empty(n or 1, dtype=_TORCH[dtype], device=device)
-    t.shape, t.dtype, t.strides, t.offset = shape, dtype, tuple(strides), 0
+    return n or 1, tuple(strides)
+
+
+def _new(shape, dtype, device):
+    """An uninitialised tensor; shape is a tuple of ints.  (The attributes are set
+    without the constructor's checks.)"""
+    t = gpuTensor.__new__(gpuTensor)
+    n, t.strides = _layout(shape)
+    t.storage = torch.empty(n, dtype=_TORCH[dtype], device=device)
+    t.shape, t.dtype, t.offset = shape, dtype, 0
     return t
 
 
-_pack_desc = struct.Struct("Pq%dq%dqii" % (L.MAX_DIMS, L.MAX_DIMS)).pack  # the layout of acd_desc
+# the layout of acd_desc in two parts: where the data is, and its form
+_pack_at = struct.Struct("Pq").pack
+_pack_form = struct.Struct("%dq%dqii" % (L.MAX_DIMS, L.MAX_DIMS)).pack
 assert struct.calcsize("Pq%dq%dqii" % (L.MAX_DIMS, L.MAX_DIMS)) == ctypes.sizeof(L.Desc)
-_pad = [(0,) * (L.MAX_DIMS - n) for n in range(L.MAX_DIMS + 1)]
+
+
+@functools.lru_cache(maxsize=4096)
+def _form(shape, strides, dtype):
+    pad = (0,) * (L.MAX_DIMS - len(shape))
+    return _pack_form(*shape, *pad, *strides, *pad, len(shape), L.DTYPE_CODES[dtype])
+
+
 _functions = {}
 
 
@@ -59,9 +78,7 @@ def _call(name):
 def _desc(t):
     if t is None:
         return None
-    n = len(t.shape)
-    pad = _pad[n]
-    return _pack_desc(t.storage.data_ptr(), t.offset, *t.shape, *pad, *t.strides, *pad, n, L.DTYPE_CODES[t.dtype])
+    return _pack_at(t.storage.data_ptr(), t.offset) + _form(t.shape, t.strides, t.dtype)
 
 
 def _dense(t):
