@@ -53,6 +53,13 @@ struct LpMath<float> {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(kFloor));
     return r;
   }
+  // A log probability: floor_z, and never above 0.
+  static __device__ __forceinline__ float limit_lp(float z) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(floor_z(z)), "f"(0.0f));
+    return r;
+  }
+  static constexpr float kFar = -1048576.0f, kNear = 512.0f;  // -2^20, 2^9
   static __device__ __forceinline__ float lowest() { return -FLT_MAX; }
   static __device__ __forceinline__ float max2(float a, float b) { return fmaxf(a, b); }
   static __device__ __forceinline__ float min2(float a, float b) { return fminf(a, b); }
@@ -63,6 +70,8 @@ struct LpMath<double> {
   static __device__ __forceinline__ double factor(double scale) { return scale; }
   static __device__ __forceinline__ double ex(double z) { return exp(z); }
   static __device__ __forceinline__ double floor_z(double z) { return z < -1000.0 ? -1000.0 : z; }  // e^-1000 = 0
+  static __device__ __forceinline__ double limit_lp(double z) { return z > 0.0 ? 0.0 : floor_z(z); }
+  static constexpr double kFar = -562949953421312.0, kNear = 512.0;  // -2^49
   static __device__ __forceinline__ double lowest() { return -DBL_MAX; }
   static __device__ __forceinline__ double max2(double a, double b) { return fmax(a, b); }
   static __device__ __forceinline__ double min2(double a, double b) { return fmin(a, b); }
@@ -996,8 +1005,10 @@ struct LogprobGradArgs {
 
 // A row's coefficients, scale included.  With d = c x_v - lse = log p_v:
 //   grad_v = p_v (a0 - a1 d) + [v = t] gt,  a0 = c (g_lse - g - g_H H), a1 = c g_H.
-// d is rounded once (fma) before the exponential, so its error is that of its
-// own size and not of the logit's.
+// d is rounded once (fma) before the exponential, so that rounding is of its own
+// size and not of the logit's.  lse was rounded when it was stored: p is off by up
+// to |lse| u of itself, and far from 0 d, the log of a probability, has to be kept
+// from being above 0, which the rounded lse alone would allow by any amount.
 template <typename A>
 struct GradRow {
   A lse, a0, a1, gt;
@@ -1025,18 +1036,22 @@ __device__ __forceinline__ GradRow<A> grad_row(const LogprobGradArgs &a, int64_t
     g.a0 = fma_a(-g.a1, static_cast<const A *>(a.entropy)[r], g.a0);
   }
   // a row without mass: p = 0 everywhere and no token term.  So is one masked
-  // throughout by the type's lowest value: its lse has no digits left for ln S.
-  if (g.lse <= (std::is_same<A, double>::value ? (A)(-DBL_MAX / 4) : (A)(-FLT_MAX / 4))) {
+  // throughout by a large finite value: at -2^20 (float64: -2^49) lse has three
+  // binary digits left after the point, at -2^24 (-2^53) none for ln S.
+  if (g.lse <= LpMath<A>::kFar) {
     g.lse = A(INFINITY);
     g.a0 = g.a1 = g.gt = A(0);
   }
   return g;
 }
 
-// N logits of one row (or, with G = N, of N rows side by side).
-template <typename A, int N, int G>
+// N logits of one row (or, with G = N, of N rows side by side).  NEAR: |lse| is at
+// most kNear, where its rounding (2^-15 of p in float32) can stay.
+template <typename A, int N, int G, bool NEAR>
 __device__ __forceinline__ void grad_values(const GradRow<A> (&g)[G], A (&x)[N], A c) {
   using M = LpMath<A>;
+  // p = 0 where d is below the floor: 0 log 0 = 0
+  auto limit = [](A d) { return NEAR ? M::floor_z(d) : M::limit_lp(d); };
   if constexpr (std::is_same<A, float>::value && N % 2 == 0) {
     const uint64_t cc = pack2(c, c), l2e = pack2(1.44269504088896341f, 1.44269504088896341f);
 #pragma unroll
@@ -1044,8 +1059,8 @@ __device__ __forceinline__ void grad_values(const GradRow<A> (&g)[G], A (&x)[N],
       const GradRow<A> &p = g[G == 1 ? 0 : j], &q = g[G == 1 ? 0 : j + 1];
       float d0, d1, z0, z1;
       unpack2(fma2(cc, pack2(x[j], x[j + 1]), pack2(-p.lse, -q.lse)), d0, d1);
-      d0 = M::floor_z(d0);  // p = 0 where d is below the floor: 0 log 0 = 0
-      d1 = M::floor_z(d1);
+      d0 = limit(d0);
+      d1 = limit(d1);
       const uint64_t d = pack2(d0, d1);
       unpack2(mul2(d, l2e), z0, z1);
       unpack2(mul2(pack2(M::ex(z0), M::ex(z1)), fma2(pack2(-p.a1, -q.a1), d, pack2(p.a0, q.a0))), x[j], x[j + 1]);
@@ -1054,7 +1069,7 @@ __device__ __forceinline__ void grad_values(const GradRow<A> (&g)[G], A (&x)[N],
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const GradRow<A> &p = g[G == 1 ? 0 : j];
-      const A d = M::floor_z(fma_a(c, x[j], -p.lse));
+      const A d = limit(fma_a(c, x[j], -p.lse));
       const A e = std::is_same<A, float>::value ? M::ex(d * A(1.44269504088896341)) : M::ex(d);
       x[j] = e * fma_a(-p.a1, d, p.a0);
     }
@@ -1081,19 +1096,25 @@ __global__ void __launch_bounds__(256, sizeof(T) == 8 ? 2 : 5) k_logprob_grad_ro
     Piece<T, V> raw[U];
     load_batch<T, V, U>(x, a.x.sd, D, shift, (int)seg, raw);
     const GradRow<A> g[1] = {grad_row<A>(a, r)};
+    auto finish = [&](auto near) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int first = base + (u * 32 + lane) * V;
-      A v[V];
-      raw[u].widen(v);
-      grad_values<A, V, 1>(g, v, c);
-      if (g[0].t >= first && g[0].t < first + V) {
+      for (int u = 0; u < U; ++u) {
+        const int first = base + (u * 32 + lane) * V;
+        A v[V];
+        raw[u].widen(v);
+        grad_values<A, V, 1, decltype(near)::value>(g, v, c);
+        if (g[0].t >= first && g[0].t < first + V) {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (first + j == g[0].t) v[j] += g[0].gt;
+          for (int j = 0; j < V; ++j)
+            if (first + j == g[0].t) v[j] += g[0].gt;
+        }
+        store_piece<T, A, V>(out, a.g.sd, first, D, v);
       }
-      store_piece<T, A, V>(out, a.g.sd, first, D, v);
-    }
+    };
+    if (fabs(g[0].lse) <= LpMath<A>::kNear)
+      finish(std::true_type());
+    else
+      finish(std::false_type());
   }
 }
 
@@ -1129,7 +1150,7 @@ __global__ void __launch_bounds__(256) k_logprob_grad_lanes(LogprobGradArgs a, i
       if (s + u * by >= s1) break;
       A v[V];
       w[u].widen(v);
-      grad_values<A, V, V>(g, v, c);
+      grad_values<A, V, V, false>(g, v, c);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (g[j].t == (int)(s + u * by)) v[j] += g[j].gt;

@@ -420,9 +420,12 @@ acd_status acd_token_logprob(acd_ctx *ctx, const acd_desc *logprob, const acd_de
  *            + p_v (d_lse - d_logprob - d_entropy (log p_v + entropy)))
  * grad has the logits' shape and dtype and may be the logits' own view
  * (otherwise the two must not overlap).  A token that asks for nothing, and
- * one outside the vocabulary, takes d_logprob as 0.  A row without mass has
- * gradient 0, and so has one whose lse is below a quarter of the statistics
- * type's lowest value (every logit masked by that value).  tokens goes with
+ * one outside the vocabulary, takes d_logprob as 0.  p_v = exp(scale * x_v -
+ * lse) is as exact as lse, whose rounding to the statistics' type makes p_v off
+ * by up to |lse| 2^-24 (FLOAT64: 2^-53) of itself, and never above 1 by more
+ * than 2^-15.  A row without mass has gradient 0, and so has one whose lse is
+ * -2^20 (FLOAT64: -2^49) or lower, which has no digits left for the sum: every
+ * logit of it is masked by a large finite value such as -1e9.  tokens goes with
  * d_logprob, entropy with d_entropy. */
 acd_status acd_token_logprob_grad(acd_ctx *ctx, const acd_desc *grad, const acd_desc *logits, const acd_desc *tokens,
                                   int32_t axis, double scale, const acd_desc *lse, const acd_desc *entropy,
