@@ -485,8 +485,11 @@ acd_status acd_quant4_matvec(acd_ctx *ctx, const acd_desc *out, const acd_desc *
  * FLOAT32 or FLOAT64.  zeros NULL: scale = max|w| / 7 and q = round(w / scale)
  * + 8.  Otherwise scale = (max(w, 0) - min(w, 0)) / 15, zero = round(-min(w, 0)
  * / scale) and q = round(w / scale) + zero, both limited to 0..15.  Rounding
- * is to nearest, ties to even, with the scale as it is stored; a group whose
- * scale is 0 holds q = zero.  A group with a NaN or infinite weight gets a
+ * is to nearest, ties to even, with the scale as it is stored (it is worked out
+ * in float64 and rounded once); a group whose scale is 0 holds q = zero.  A
+ * scale above the largest value of the scales' type is stored as that value:
+ * the weights are cut off at both ends of the range, with the zero point of the
+ * scale that it should have been.  A group with a NaN or infinite weight gets a
  * scale of NaN. */
 acd_status acd_quant4_encode(acd_ctx *ctx, const acd_desc *weights, const acd_desc *scales, const acd_desc *zeros,
                              const acd_desc *w, int32_t group, acd_stream stream);
