@@ -1163,11 +1163,21 @@ __global__ void __launch_bounds__(256) k_logprob_grad_lanes(LogprobGradArgs a, i
 static bool row_dtype(int32_t dt) { return dt == ACD_FLOAT32 || dt == ACD_FLOAT64 || dt == ACD_FLOAT16; }
 static int32_t stat_dtype(int32_t dt) { return dt == ACD_FLOAT64 ? ACD_FLOAT64 : ACD_FLOAT32; }
 
+// What float32 statistics work with: c log2(e) is a finite float32, and c not
+// below the smallest one (0 would make 0 * Inf of masked logits; 2^-149 moves no
+// scaled logit by more than 2^-21).
+constexpr double kMaxScale32 = 2.3e38, kMinScale32 = 0x1p-149;
+static double stat_scale(const acd_desc *logits, double scale) {
+  return logits->dtype != ACD_FLOAT64 && scale < kMinScale32 ? kMinScale32 : scale;
+}
+
 static acd_status check_logits(const char *op, const acd_desc *logits, int32_t axis, double scale) {
   ACD_TRY(check_desc(logits, "logits"));
   if (!row_dtype(logits->dtype)) return fail(ACD_ERR_DTYPE, "%s: float32, float64 or float16 logits required", op);
   if (axis < 0 || axis >= logits->ndim) return fail(ACD_ERR_AXIS, "%s: axis %d out of range", op, axis);
   if (!(scale > 0.0) || !std::isfinite(scale)) return fail(ACD_ERR_INVALID, "%s: scale must be positive and finite", op);
+  if (logits->dtype != ACD_FLOAT64 && scale > kMaxScale32)
+    return fail(ACD_ERR_INVALID, "%s: scale is beyond float32's range", op);
   // positions are ints, with room for the last batch
   if (logits->shape[axis] > INT32_MAX - 65536) return fail(ACD_ERR_UNSUPPORTED, "%s: more than 2^31 - 65537 tokens", op);
   return ACD_OK;
@@ -1409,7 +1419,7 @@ acd_status acd_token_logprob(acd_ctx *ctx, const acd_desc *logprob, const acd_de
   if (a.s.rows() == 0) return ACD_OK;
   if (a.s.D == 0) return fail(ACD_ERR_SHAPE, "%s: rows without tokens", op);
   if (a.s.rows() > INT32_MAX) return fail(ACD_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows", op);
-  a.scale = scale;
+  a.scale = stat_scale(logits, scale);
   a.tokens = ptr_or_null(tokens);
   a.wide_token = tokens && tokens->dtype == ACD_INT64;
   a.one_based = one_based != 0;
@@ -1456,7 +1466,7 @@ acd_status acd_token_logprob_grad(acd_ctx *ctx, const acd_desc *grad, const acd_
     return fail(ACD_ERR_UNSUPPORTED, "%s: view not collapsible around the axis; make it contiguous first", op);
   if (a.s.rows() == 0 || a.s.D == 0) return ACD_OK;
   if (a.s.rows() > INT32_MAX) return fail(ACD_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows", op);
-  a.scale = scale;
+  a.scale = stat_scale(logits, scale);
   a.tokens = d_logprob ? desc_ptr(tokens) : nullptr;
   a.wide_token = d_logprob && tokens->dtype == ACD_INT64;
   a.one_based = one_based != 0;

@@ -408,7 +408,8 @@ acd_status acd_argmax_keys_decode(acd_ctx *ctx, const acd_desc *out_index, const
  * logit -Inf) has lse = logprob = -Inf and entropy 0.  A NaN or +Inf logit
  * makes the row's lse, logprob and entropy NaN.
  * Any output may be NULL; tokens and logprob go together, top_index and
- * top_logprob too.  scale is positive and finite. */
+ * top_logprob too.  scale is positive and finite (FLOAT16 and FLOAT32 logits: at
+ * most 2.3e38). */
 acd_status acd_token_logprob(acd_ctx *ctx, const acd_desc *logprob, const acd_desc *entropy, const acd_desc *lse,
                              const acd_desc *top_index, const acd_desc *top_logprob, const acd_desc *logits,
                              const acd_desc *tokens, int32_t axis, double scale, int32_t one_based,
