@@ -417,8 +417,8 @@ __device__ __forceinline__ void unit_rows(const GradPlan &p, int64_t u, int64_t 
 // V columns of a row's gradient, in two steps around the row's sums.  With
 //   u = d_y w_pre,  q = d_h + rs_h u,  f = gate w_post,  e = f b
 // and the sums s0 = sum u h, s1 = sum q e, s2 = sum h e over the row,
-//   m1 = mean(d_y w_pre hn) = rs_h s0 / D,  t = q - rs_h^2 m1 h / rs_h,
-//   mean(u w_post bn) = rs_b (s1 - rs_h m1 s2) / D:
+//   m1 = rs_h mean(d_y w_pre hn) = rs_h^2 s0 / D,  t = q - m1 hn,
+//   mean(u w_post bn) = rs_b (s1 - m1 rs_h s2) / D:
 // one reduction a row.  sum t bn is what the gradients of the gate (times
 // w_post) and of w_post (times gate) have in common while the gate row stays.
 template <typename A, int V>
@@ -453,13 +453,14 @@ struct GradCols {
   // s: the row's sums; adds to pre and tb, leaves the gradients in dr and db.
   __device__ __forceinline__ void finish(const A (&s)[3], A inv, A rh, A rb, A alpha, bool post, const P (&f)[M],
                                          P (&pre)[M], P (&tb)[M], A (&dr)[V], A (&db)[V]) const {
-    const A m1 = rh * (s[0] * inv) * rh;  // times rs_h once more: t = q - (rs_h m1) h
-    const P nm1 = P::all(-m1 * rh), prh = P::all(rh), prb = P::all(rb), pal = P::all(alpha);
-    const P nm2 = P::all(post ? -(rb * inv) * (s[1] - m1 * rh * s[2]) : A(0));
+    // (rs_h is put to h before the mean, and to s2: rs_h^3 alone may be beyond the type)
+    const A m1 = rh * (s[0] * inv) * rh;
+    const P nm1 = P::all(-m1), prh = P::all(rh), prb = P::all(rb), pal = P::all(alpha);
+    const P nm2 = P::all(post ? -(rb * inv) * (s[1] - m1 * (rh * s[2])) : A(0));
 #pragma unroll
     for (int j = 0; j < M; ++j) {
-      const P t = pfma(h[j], nm1, q[j]), bn = pmul(b[j], prb);
-      pre[j] = pfma(dy[j], pmul(h[j], prh), pre[j]);
+      const P hn = pmul(h[j], prh), t = pfma(hn, nm1, q[j]), bn = pmul(b[j], prb);
+      pre[j] = pfma(dy[j], hn, pre[j]);
       tb[j] = pfma(t, bn, tb[j]);
       pmul(pal, t).to(dr + j * P::N);
       P x = pmul(t, f[j]);
