@@ -87,6 +87,15 @@ struct acd_ctx {
   acd_alloc_fn alloc = nullptr;
   acd_free_fn free_fn = nullptr;
   void *alloc_user = nullptr;
+  // Regions that were outgrown after a stream capture had used the workspace.
+  struct Retired {
+    void *p;
+    acd_free_fn free_fn;
+    void *user;
+    Retired *next;
+  };
+  bool captured = false;
+  Retired *retired = nullptr;
   int64_t scan_fault_tile = -1;
   int64_t scan_timeout_ns = 1000000000LL;
 };
@@ -94,7 +103,9 @@ struct acd_ctx {
 namespace acd {
 
 // Scratch for partial results: at least `bytes`, contents undefined.
-// Growing synchronises `stream` first (the old region may be in use).
+// Growing synchronises `stream` first (the old region may be in use); in a stream
+// capture it is refused, and a region that a capture has used is kept when it is
+// outgrown.
 acd_status get_scratch(acd_ctx *ctx, size_t bytes, cudaStream_t stream, void **out);
 // `n` tile counters, zero at rest: every kernel that increments one resets it.
 // Nothing else ever writes this region.

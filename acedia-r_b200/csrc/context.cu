@@ -11,6 +11,7 @@
 #include <string>
 #include <algorithm>
 #include <mutex>
+#include <new>
 
 #include "common.cuh"
 
@@ -56,18 +57,51 @@ static void dev_free(acd_ctx *ctx, void *p) {
     cudaFree(p);
 }
 
+// Frees a region of the workspace that has been outgrown.  A graph that was
+// captured while it was in use still has its address: then it is kept for the
+// context's life.
+static void release(acd_ctx *ctx, void *p) {
+  if (!p) return;
+  if (!ctx->captured) {
+    dev_free(ctx, p);
+    return;
+  }
+  auto *r = new (std::nothrow) acd_ctx::Retired{p, ctx->free_fn, ctx->alloc_user, ctx->retired};
+  if (r) ctx->retired = r;  // (else it is left to the end of the process)
+}
+
+// Notes a capture under way on `stream`, during which nothing can be allocated.
+static bool capturing(acd_ctx *ctx, cudaStream_t stream) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &st) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (st == cudaStreamCaptureStatusNone) return false;
+  ctx->captured = true;
+  return true;
+}
+
+static acd_status fail_captured(const char *what, size_t bytes) {
+  return fail(ACD_ERR_ALLOC,
+              "the %s has to grow to %zu bytes, which cannot be done in a stream capture: make the call once before it",
+              what, bytes);
+}
+
 acd_status get_scratch(acd_ctx *ctx, size_t bytes, cudaStream_t stream, void **out) {
   if (bytes == 0) bytes = 256;
+  const bool capture = capturing(ctx, stream);
   if (ctx->scratch && ctx->scratch_bytes >= bytes) {
     *out = ctx->scratch;
     return ACD_OK;
   }
+  if (capture) return fail_captured("workspace", bytes);
   size_t want = bytes;
   if (want < 2 * ctx->scratch_bytes) want = 2 * ctx->scratch_bytes;
   want = (want + 4095) & ~(size_t)4095;
   if (ctx->scratch) {
     ACD_CUDA(cudaStreamSynchronize(stream));
-    dev_free(ctx, ctx->scratch);
+    release(ctx, ctx->scratch);
     ctx->scratch = nullptr;
     ctx->scratch_bytes = 0;
   }
@@ -83,12 +117,14 @@ template <typename W>
 static acd_status get_zeroed(acd_ctx *ctx, W **region, size_t *have, size_t n, cudaStream_t stream,
                              const char *what) {
   if (n == 0) n = 1;
+  const bool capture = capturing(ctx, stream);
   if (*region && *have >= n) return ACD_OK;
+  if (capture) return fail_captured(what, n * sizeof(W));
   size_t want = n < 2 * *have ? 2 * *have : n;
   want = (want + 1023) & ~(size_t)1023;
   if (*region) {
     ACD_CUDA(cudaStreamSynchronize(stream));
-    dev_free(ctx, *region);
+    release(ctx, *region);
     *region = nullptr;
     *have = 0;
   }
@@ -364,6 +400,14 @@ acd_status acd_ctx_destroy(acd_ctx *ctx) {
   dev_free(ctx, ctx->scratch);
   dev_free(ctx, ctx->counters);
   dev_free(ctx, ctx->flags);
+  while (acd_ctx::Retired *r = ctx->retired) {
+    ctx->retired = r->next;
+    if (r->free_fn)
+      r->free_fn(r->p, r->user);
+    else
+      cudaFree(r->p);
+    delete r;
+  }
   cudaFree(ctx->control);
   delete ctx;
   return ACD_OK;
@@ -375,9 +419,9 @@ acd_status acd_ctx_set_allocator(acd_ctx *ctx, acd_alloc_fn alloc, acd_free_fn f
     return fail(ACD_ERR_INVALID, "acd_ctx_set_allocator: alloc and free must both be set or both be NULL");
   DeviceGuard g(ctx->device);
   ACD_CUDA(cudaDeviceSynchronize());
-  dev_free(ctx, ctx->scratch);
-  dev_free(ctx, ctx->counters);
-  dev_free(ctx, ctx->flags);
+  release(ctx, ctx->scratch);
+  release(ctx, ctx->counters);
+  release(ctx, ctx->flags);
   ctx->scratch = nullptr;
   ctx->scratch_bytes = 0;
   ctx->counters = nullptr;

@@ -83,7 +83,11 @@ typedef struct acd_desc {
 
 /* Opaque per-device context: owns the reduction/scan workspace and the
  * device status word.  Calls that share one context must be ordered on one
- * stream (the workspace is reused without locking). */
+ * stream (the workspace is reused without locking).  The workspace grows on
+ * demand, which waits for the stream; in a stream capture a call that needs
+ * more returns ACD_ERR_ALLOC, so make each call once before capturing it.  What
+ * a captured graph uses stays allocated until the context is destroyed, which
+ * has to be after the graph's last replay. */
 typedef struct acd_ctx acd_ctx;
 
 /* cudaStream_t, passed as an opaque pointer so this header needs no CUDA headers. */
