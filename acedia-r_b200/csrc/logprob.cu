@@ -187,7 +187,7 @@ struct TopList {
     }
     refresh(k);
   }
-  // Every lane offers one logit (index `none` to offer nothing).
+  // Every lane offers one logit, or nothing (not `valid`).
   __device__ __forceinline__ void offer(A x, int xi, bool valid, A floor, int k) {
     unsigned mask = __ballot_sync(~0u, valid && x >= floor && better(x, xi, kv, ki));
     while (mask) {
@@ -196,23 +196,6 @@ struct TopList {
       mask &= mask - 1;
       mask &= __ballot_sync(~0u, better(x, xi, kv, ki));
     }
-  }
-  // 32 unsorted logits, one a lane: sorted the other way round, then merged.
-  __device__ __forceinline__ void merge_unsorted(A x, int xi) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-      for (int q = size >> 1; q; q >>= 1) {
-        const A ov = __shfl_xor_sync(~0u, x, q);
-        const int oi = __shfl_xor_sync(~0u, xi, q);
-        const bool worse = ((lane & size) == 0) == ((lane & q) == 0);  // this lane keeps the worse one
-        if (worse == better(x, xi, ov, oi)) {
-          x = ov;
-          xi = oi;
-        }
-      }
-    merge_reversed(x, xi);
   }
   // Another sorted list, lane q holding its entry 31 - q: the better of each
   // pair is a bitonic sequence of the 32 best; five exchanges sort it.

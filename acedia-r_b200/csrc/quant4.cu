@@ -96,11 +96,6 @@ constexpr int kMaxStages = 4;
 template <bool X16, int NT>
 struct Q4Vectors { static constexpr int value = X16 ? 8 * NT : 8 * NT / 3; };
 
-template <bool X16>
-struct Q4Type { using H2 = __half2; };
-template <>
-struct Q4Type<false> { using H2 = __nv_bfloat162; };
-
 // (q & m) | o in one instruction (the truth table of a lop3).
 __device__ __forceinline__ uint32_t and_or(uint32_t q, uint32_t m, uint32_t o) {
   uint32_t r;
