@@ -393,7 +393,10 @@ acd_status acd_argmax_keys_decode(acd_ctx *ctx, const acd_desc *out_index, const
  * acd_softmax.  "Row tensors" hold one value a row: shape of the view without
  * the axis, or with extent 1 there, contiguous.  Statistics are FLOAT32 for
  * FLOAT16/FLOAT32 rows and FLOAT64 for FLOAT64 rows; sums are held in that
- * type too.  The reference has none of these operators. */
+ * type too, in an order that follows from the shapes, strides and alignment of
+ * the operands and from the device: a call repeated on the same tensors gives
+ * the same bits, the same values at another alignment or pitch may round
+ * differently.  The reference has none of these operators. */
 
 /* Log probability of one given token a row under softmax(scale * logits),
  * with the entropy of that distribution, its log-sum-exp and its k most
@@ -463,8 +466,7 @@ acd_status acd_residual_norm(acd_ctx *ctx, const acd_desc *h, const acd_desc *y,
  *   d_gate  = sum t b'                            over each gate row's rows
  * d_h NULL: the loss sees h through y only.  d_w_pre, d_w_post, d_gate have
  * their operand's shape, in the statistics' dtype, contiguous; each may be
- * NULL.  Their sums run in an order set by the shapes alone: the same inputs
- * give the same bits.  d_residual may be d_h's own view and d_block d_y's. */
+ * NULL.  d_residual may be d_h's own view and d_block d_y's. */
 acd_status acd_residual_norm_grad(acd_ctx *ctx, const acd_desc *d_residual, const acd_desc *d_block,
                                   const acd_desc *d_w_pre, const acd_desc *d_w_post, const acd_desc *d_gate,
                                   const acd_desc *d_h, const acd_desc *d_y, const acd_desc *h, const acd_desc *block,
@@ -481,9 +483,10 @@ acd_status acd_residual_norm_grad(acd_ctx *ctx, const acd_desc *d_residual, cons
  * FLOAT16 or FLOAT32 of shape [ceil(in / group), out], contiguous; zeros may
  * be NULL.  group is a positive multiple of 32.  x: [in] or [in, n], out:
  * [out] or [out, n], FLOAT16 or FLOAT32 each, any strides, not overlapping.
- * Products are summed in float32 in an order set by the shapes alone.  An
- * infinite or NaN activation reaches its own column only; with zeros an
- * infinite one may give NaN (the zero points are summed apart). */
+ * Products are summed in float32, in a fixed order as the sums of the rows above.
+ * An infinite or NaN activation reaches its own column only; with zeros an
+ * infinite one, or sums beyond float32's range, may give NaN (the zero points
+ * are summed apart). */
 acd_status acd_quant4_matvec(acd_ctx *ctx, const acd_desc *out, const acd_desc *weights, const acd_desc *scales,
                              const acd_desc *zeros, const acd_desc *x, int32_t group, acd_stream stream);
 /* Makes weights, scales (and zeros) from w, an [out, in] view of FLOAT16,
