@@ -169,8 +169,9 @@ def residual_norm(residual, block, w_pre, w_post=None, gate=None, axis=1, alpha=
 
     Without w_post the block is added as it is, without gate unscaled.  gate
     has one element for each of a row, or the residual's shape with 1 on any
-    leading axes other than `axis` (a gate for each sample).  inplace=True
-    writes h over the residual and y over the block.  Returns ResidualNorm;
+    leading axes other than `axis` (a gate for each sample; an axis in the
+    middle leaves extents other than 1 to one side of it).  inplace=True writes
+    h over the residual and y over the block.  Returns ResidualNorm;
     rstd_h and rstd_block are what residual_norm_grad takes."""
     a = _axis0(block, axis)
     dev, st, shape = block.device, _stat_dtype(block), _row_shape(block, a)

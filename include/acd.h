@@ -450,7 +450,9 @@ acd_status acd_token_logprob_grad(acd_ctx *ctx, const acd_desc *grad, const acd_
  * elements of the rows' dtype (FLOAT32, FLOAT64, FLOAT16), contiguous.  gate:
  * D elements, or the residual's shape with extent 1 on any number of leading
  * axes other than `axis`, so that each of its G rows of D elements holds for
- * rows/G consecutive rows.  rstd_h and rstd_block are row tensors (either may
+ * rows/G consecutive rows.  Its rows must be one stride apart: where `axis`
+ * stands in the middle, extents other than 1 on one side of it only
+ * (ACD_ERR_UNSUPPORTED otherwise).  rstd_h and rstd_block are row tensors (either may
  * be NULL) that the gradient takes.  h may be the residual's own view and y
  * the block's; otherwise outputs must not overlap inputs. */
 acd_status acd_residual_norm(acd_ctx *ctx, const acd_desc *h, const acd_desc *y, const acd_desc *rstd_h,
