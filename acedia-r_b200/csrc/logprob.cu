@@ -1243,9 +1243,13 @@ static acd_status launch_lanes(acd_ctx *ctx, const LogprobArgs &a, cudaStream_t 
   k_logprob_lanes<T, V, TOP><<<(unsigned)(blocks * la.chunks), 256, 0, s>>>(la);
   if (!join) return ACD_OK;
   if constexpr (TOP && sizeof(T) < 8) {
-    // a thread a row from four warps an SM on (65536 rows of 4096 float32, five
-    // alternatives: the warp kernel takes 190 us for this part)
-    if (a.k <= 8 && a.s.rows() >= (int64_t)ctx->sm_count * 128) {
+    // A thread a row where there are rows to hide its scattered reads: more of them
+    // the more alternatives there are.  Rows of 4096 float32, a thread or a warp a
+    // row, 1, 3, 5 and 8 alternatives: 9472 rows 46, 63, 79, 91 or 49, 53, 57, 58 us;
+    // 18944 rows 80, 93, 106, 128 or 93, 91, 96, 105 us; 37888 rows 151, 176, 196,
+    // 219 or 178, 191, 201, 216 us; 65536 rows 202, 235, 264, 294 or 252, 273, 289,
+    // 315 us.
+    if (a.k <= 8 && a.s.rows() >= (int64_t)ctx->sm_count * 32 * (a.k + 1)) {
       const unsigned grid = (unsigned)((a.s.rows() + 127) / 128);
       switch (a.k) {
         case 1: k_logprob_pick<T, 1><<<grid, 128, 0, s>>>(la); break;
