@@ -422,9 +422,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 8 ? 2 : TOP ? 3 : 4) k_logpr
 // warps' sums and lists are joined in each block, the blocks' in the first one
 // through distributed shared memory, always in the same order.  Bound by the
 // reads where there are many rows (4096 x 50001 float32 in 123 us, 1.02 of a
-// copy's rate), by the latency of a block's share and of the joins where there
-// are few: one row of 131072 float16 with 20 alternatives in 17.5 us (36 us with
-// one block a row, 28 with two, 22 with four, against eight).
+// copy's rate).  One row of 131072 float16 takes 3.8 us without alternatives, 6.8
+// with one, 9.3 with five and 17.5 with twenty: the lists take their candidates
+// one after the other.  (Twenty with one block a row 36 us, with two 28, with four
+// 22.)
 template <typename T, int V, bool TOP, int NW>
 __global__ void __launch_bounds__(NW * 32, sizeof(T) == 8 ? 2 : TOP ? 3 : 4) k_logprob_cta(LogprobArgs a) {
   using A = typename AccOf<T>::type;
@@ -1307,6 +1308,8 @@ template <typename T>
 static acd_status launch_logprob(acd_ctx *ctx, const LogprobArgs &a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   // eight lanes fill a 32-byte sector of float32 (half of one of float16)
+  // (fewer rows are read an element at a time: 2, 4 and 7 rows of 131072 float16 in
+  // 6.4, 6.7 and 9.0 us, 8 rows across the lanes in 10.6)
   if (a.x.sd != 1 && a.x.sl == 1 && a.s.L >= 8)
     return a.k ? launch_lanes_any<T, true>(ctx, a, s) : launch_lanes_any<T, false>(ctx, a, s);
   if (a.x.sd == 1) return a.k ? launch_rows<T, V, true>(ctx, a, s) : launch_rows<T, V, false>(ctx, a, s);

@@ -512,9 +512,11 @@ __device__ __forceinline__ void store_sums(A *dst, int64_t sd, int tid, int n, i
 // next row is under way while one is worked on.  Both means of a row come from
 // one reduction of three sums: the mean of the post norm's gradient splits into
 // two that do not wait for the other mean.  16384 x 4096 float16 with 16 gate rows
-// in 184 us, 0.67 of a copy's rate: its registers leave one block of 512 threads
+// in 186 us, 0.66 of a copy's rate: its registers leave one block of 512 threads
 // an SM, which waits at the reduction's barrier.  Rows of odd width are
-// read an element at a time: 5000 x 1001 float32 in 37 us, 0.50.
+// read an element at a time: 5000 x 1001 float32 in 36.5 us, 0.50.  (1024 threads,
+// for rows that the ring cannot take, have 64 registers each and spill up to 488
+// bytes.)
 template <typename T, int TPR, int G>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 256 || sizeof(T) == 8 ? 1 : 2)
     k_norm_grad_vec(NormGradArgs a, GradPlan plan) {
@@ -610,11 +612,17 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR > 512 ? 1 : TPR > 2
 // to the column sums of NV pieces a thread and allows two blocks on an SM, whose
 // barriers then overlap.  The rows' sums go to the other blocks by asynchronous
 // stores that count on a barrier there.
-//   What bounds it is that exchange, once a row, where a row's bytes do not
-// cover it: 16384 x 4096 float32 in 264 us (0.93 of a copy's rate), 16384 x 8192
-// float16 in 494 us (0.50), x 5120 in 485 us (0.32).  One piece a thread and
-// twice the blocks: 378, 605 and 610 us; k_norm_grad_vec with 1024 threads: 383,
-// 593 and 514 us.
+//   A block takes 512 pieces, the last one what is left, so the time is that of a
+// row of full blocks: 16384 rows of 4160, 5120, 6144 and 8192 float16 columns take
+// 434, 430, 427 and 429 us (0.29 to 0.57 of a copy's rate), of 4096 float32 251 us
+// (0.98), without gate rows.  8192 float16 and 4096 float32 columns have the same
+// bytes and the same number of exchanges: what the first wait for is its
+// instructions.  They are 1.63 times as many (an element is widened and
+// multiplied twice, and 72 bytes a thread are spilled), issued at the same rate,
+// 41% and 43% of the slots, with 16 warps an SM to hide their latency.  One piece
+// a thread and twice the blocks took 1.4 times as long for 4096 float32, 1.2 for
+// 8192 and 1.3 for 5120 float16; k_norm_grad_vec with 1024 threads 1.45, 1.2 and
+// 1.06.
 constexpr uint64_t kRingWaitNs = 1000000000ull;  // 1 s
 constexpr int kRingWaitCode = 6;
 constexpr int kRingStages = 3;
@@ -942,6 +950,9 @@ static acd_status launch_norm(acd_ctx *ctx, const NormArgs &a, cudaStream_t s) {
            whole_weights<T>(a.w_pre, a.w_post, a.gate, a.gate_sd, a.gate_sg, n);
   });
   const int64_t pieces = (a.s.D + V - 1) / V;
+  // (Rows across the lanes come here too, G = 1: each element of a warp's lies in
+  // a sector of its own.  16384 x 4096 float16 with axis = 2 takes 1653 us, the
+  // gradient 11250 us, against 101 and 186 us along the first axis.)
   if (pieces <= 4096) {
     // A warp a row up to three pieces a lane, whose sums need no barrier, then
     // one to four pieces a thread.  16384 rows of float16 with a warp or 128
@@ -1061,7 +1072,7 @@ static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStre
   });
   const int64_t pieces = (a.s.D + V - 1) / V;
   // Up to 512 pieces of 16 bytes a row a block keeps the row in registers, one
-  // piece a thread (16384 rows of float16: 256 pieces 94 us, 512 pieces 184 us; a
+  // piece a thread (16384 rows of float16: 256 pieces 94 us, 512 pieces 186 us; a
   // single block of the ring 113 and 207 us); see k_norm_grad_ring for wider rows.
   constexpr int block = kRingPieces * kRingThreads;
   if (g == V && pieces > block && pieces <= block * kRingCluster)
@@ -1074,6 +1085,10 @@ static acd_status launch_norm_grad(acd_ctx *ctx, const NormGradArgs &a, cudaStre
     if (pieces <= 512) return launch_norm_grad_vec<T, 512>(ctx, a, g, s);
     return launch_norm_grad_vec<T, 1024>(ctx, a, g, s);
   }
+  // Wider rows that are not on 16 bytes throughout (or longer than 64 KB): a
+  // kernel for the means, one for the column sums, one for the rows, which read
+  // their tensors ten times in all.  Far from the floor: 8192 x 8194 float16 1741 us
+  // (123), 8192 x 4099 float32 1436 us (123).
   void *scratch;
   ACD_TRY(get_scratch(ctx, sizeof(A) * (size_t)a.s.rows(), s, &scratch));
   A *means = static_cast<A *>(scratch);

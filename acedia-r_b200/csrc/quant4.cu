@@ -69,6 +69,11 @@ __device__ __forceinline__ void store_f(void *p, bool half, int64_t i, float v) 
 // unevenly.  One block a cluster took 57 us there, two 61, three (the rule's) 54,
 // four 65, eight 89.  Scales through shared memory, by the lanes or by
 // asynchronous copies of aligned pieces, made the first two slower (82 us).
+//   Made for some tens of columns: each set of 32 (float32: 10) reads and unpacks all
+// weights again.  4096 x 4096 float16 takes 12.3 us for 8 columns, 33 for 32, 39
+// for 128 and 902 for 4096.  Three and four instructions' columns (17 to 32
+// float16, 6 to 10 float32) spill, with groups of 32 and zero points up to 1090
+// bytes a thread.
 constexpr int kRowsPerBlock = 64;
 constexpr int kTileBytes = 128;                       // of one output: 256 inputs, 8 chunks of 32
 constexpr int kBoxBytes = kRowsPerBlock * kTileBytes;
@@ -103,7 +108,9 @@ __device__ __forceinline__ uint32_t and_or(uint32_t q, uint32_t m, uint32_t o) {
   return r;
 }
 
-// Eight weights of a word: w[i] holds inputs i and i + 4 as n - 8.
+// Eight weights of a word: w[i] holds inputs i and i + 4 as n - 8.  (The usual way
+// to make floating-point values of small integers: as the last bits of a mantissa
+// whose unit is 1.)
 template <bool X16>
 __device__ __forceinline__ void unpack8(uint32_t q, uint32_t (&w)[4]) {
   if constexpr (X16) {
