@@ -1021,8 +1021,9 @@ __device__ __forceinline__ GradRow<A> grad_row(const LogprobGradArgs &a, int64_t
   }
   // a row without mass: p = 0 everywhere and no token term.  So is one masked
   // throughout by a large finite value: at -2^20 (float64: -2^49) lse has three
-  // binary digits left after the point, at -2^24 (-2^53) none for ln S.
-  if (g.lse <= LpMath<A>::kFar) {
+  // binary digits left after the point, at -2^24 (-2^53) none for ln S.  (A scale
+  // above 1 takes ordinary logits that far: then it is the logits that count.)
+  if (g.lse <= LpMath<A>::kFar * LpMath<A>::max2(c, A(1))) {
     g.lse = A(INFINITY);
     g.a0 = g.a1 = g.gt = A(0);
   }

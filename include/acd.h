@@ -432,9 +432,9 @@ acd_status acd_token_logprob(acd_ctx *ctx, const acd_desc *logprob, const acd_de
  * lse) is as exact as lse, whose rounding to the statistics' type makes p_v off
  * by up to |lse| 2^-24 (FLOAT64: 2^-53) of itself, and never above 1 by more
  * than 2^-15.  A row without mass has gradient 0, and so has one whose lse is
- * -2^20 (FLOAT64: -2^49) or lower, which has no digits left for the sum: every
- * logit of it is masked by a large finite value such as -1e9.  tokens goes with
- * d_logprob, entropy with d_entropy. */
+ * -2^20 (FLOAT64: -2^49) times the larger of 1 and scale, or lower, which has no
+ * digits left for the sum: every logit of it is masked by a large finite value
+ * such as -1e9.  tokens goes with d_logprob, entropy with d_entropy. */
 acd_status acd_token_logprob_grad(acd_ctx *ctx, const acd_desc *grad, const acd_desc *logits, const acd_desc *tokens,
                                   int32_t axis, double scale, const acd_desc *lse, const acd_desc *entropy,
                                   const acd_desc *d_logprob, const acd_desc *d_entropy, const acd_desc *d_lse,

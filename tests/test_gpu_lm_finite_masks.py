@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 NP = {"float": np.float32, "float16": np.float16, "double": np.float64}
 FILLS = {"float": [-1e9, -1e10, -1e30, -3.4028234663852886e38], "float16": [-65504.0],
          "double": [-1e17, -1e30, -1.7976931348623157e308]}
-# at this lse and below no digits are left for what log probabilities are made of
+# at this lse (times a scale above 1) and below no digits are left for what log
+# probabilities are made of
 FAR = {"float": -2.0 ** 20, "float16": -2.0 ** 20, "double": -2.0 ** 49}
 
 
@@ -49,9 +50,8 @@ def test_rows_masked_throughout(acd, dtype, axis, rows, V, stride, scale):
     lse, H = r.logsumexp.as_array().reshape(-1), r.entropy.as_array().reshape(-1)
     g, gH, gl = (rng.uniform(0.5, 1.5, rows).astype(st) for _ in range(3))
     f = lambda v: None if v is None else v.astype(np.float64)  # noqa: E731
-    far = lse <= FAR[dtype]
-    if dtype != "float16" or scale > 20:
-        assert far.sum() == len(FILLS[dtype])
+    far = lse <= FAR[dtype] * max(1.0, scale)
+    assert far.sum() == (0 if dtype == "float16" else len(FILLS[dtype]))
     for gHk, glk, inplace in ((None, None, False), (gH, gl, True)):
         got = gradient(acd, x, dtype, axis, tokens, lse, H, g, gHk, glk, scale, stride, inplace)
         exp = O.logprob_grad(x[~far], tokens[~far], f(lse[~far]), f(H[~far]), f(g[~far]),
@@ -63,6 +63,32 @@ def test_rows_masked_throughout(acd, dtype, axis, rows, V, stride, scale):
         assert not got[far].any(), "masked rows"
     zero = np.zeros(rows, st)
     assert not gradient(acd, x, dtype, axis, tokens, lse, H, zero, zero, zero, scale, stride).any(), "zero gradients"
+
+
+@pytest.mark.parametrize("dtype", ["float", "float16"])
+@pytest.mark.parametrize("axis", [1, 2])
+@pytest.mark.parametrize("scale", [1e3, 1e5, 1e6])
+def test_ordinary_logits_at_low_temperatures(acd, dtype, axis, scale):
+    """A large scale takes lse far down too; the row still has its likeliest token."""
+    V, rows = 300, 16
+    rng = np.random.default_rng(5)
+    x = rng.integers(-60, -31, (rows, V)).astype(NP[dtype])
+    best = rng.integers(0, V, rows)
+    x[np.arange(rows), best] = -30
+    tokens = best + 1
+    tokens[::2] = 1 + (best[::2] + 1) % V  # another one
+    a = np.asfortranarray(x.T) if axis == 1 else x
+    r = acd.token_logprob(acd.as_tensor(a, dtype=dtype), acd.as_tensor(tokens, dtype="int64"), axis=axis, scale=scale)
+    lse = r.logsumexp.as_array().reshape(-1)
+    g = np.full(rows, 1.0 / scale, np.float32)
+    got = gradient(acd, x, dtype, axis, tokens, lse, None, g, None, None, scale).astype(np.float64)
+    # p of the likeliest token is 1 to within |lse| 2^-24 (lse's rounding) and as much for scale's
+    off = np.expm1(2 * 30 * scale * 2.0 ** -24) + 2.0 ** -10
+    want = np.zeros((rows, V))
+    want[np.arange(rows), best] -= 1
+    want[np.arange(rows), tokens - 1] += 1
+    assert np.abs(got - want).max() <= off
+    assert np.abs(got[np.arange(rows), tokens - 1][::2] - 1).max() <= 2.0 ** -10
 
 
 @pytest.mark.parametrize("dtype,top", [("float", 1e9), ("float", 1e30), ("float16", 65504.0), ("double", 1e30)])
